@@ -86,6 +86,24 @@ _SIGNATURES = {
     "cppinf_linear_argmax_noalloc": [_ptr, _ptr, _ptr, _i64, _i64, _ptr, _ptr],
     "cppinf_decoder_attention": [_ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _ptr],
     "cppinf_decoder_attention_tc": [_ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _ptr, _ptr],
+    "cppinf_cache_attention_scratch_bytes": [_i64, _i64, _i64, _i64, _i64, _i64, _int],
+    "cppinf_tree_attention": [
+        _ptr, _ptr, ctypes.POINTER(_i64), _ptr, ctypes.POINTER(_i64), _ptr, _ptr, _i64, _ptr, _ptr, _i64, _i64, _i64,
+        _i64, _i64, _i64, _ptr, _i64, _ptr, _ptr,
+    ],
+    "cppinf_tree_accept": [_ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64, _i64, _ptr],
+    "cppinf_tree_commit": [
+        _int, _ptr, ctypes.POINTER(_i64), _ptr, ctypes.POINTER(_i64), _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64, _i64,
+        _ptr,
+    ],
+    "cppinf_decoder_attention_weights": [
+        _ptr, _ptr, ctypes.POINTER(_i64), _ptr, ctypes.POINTER(_i64), _ptr, _ptr, _ptr, _ptr, _i64, _i64, _i64, _i64,
+        _i64, _i64, _ptr, _i64, _ptr, _ptr,
+    ],
+    "cppinf_cache_evict": [
+        _int, _ptr, ctypes.POINTER(_i64), _ptr, ctypes.POINTER(_i64), _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _i64,
+        _i64, _i64, _i64, _i64, _i64, _i64, _i64, _ptr,
+    ],
     "cppinf_embedding": [_ptr, _i64, _i64, _ptr, _i64, _ptr, _ptr],
     "cppinf_qwen3_create": [ctypes.c_void_p, _i64, ctypes.POINTER(_ptr)],
     "cppinf_qwen3_destroy": [_ptr],
@@ -110,6 +128,7 @@ _RESTYPES = {
     "cppinf_launch_count": ctypes.c_uint64,
     "cppinf_set_wait_poll_limit": ctypes.c_uint32,
     "cppinf_linear_argmax_scratch_bytes": _i64,
+    "cppinf_cache_attention_scratch_bytes": _i64,
     "cppinf_qwen3_destroy": None,
     "cppinf_qwen3_length": _i64,
     "cppinf_qwen3_step_launches": _i64,

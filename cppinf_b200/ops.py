@@ -453,6 +453,221 @@ def decoder_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
     return ctx
 
 
+# ---- batches of cached sequences: drafted trees, attention weights, eviction -------------------------------------
+
+
+def _same_device(op: str, *tensors: torch.Tensor | None) -> torch.device:
+    first = tensors[0]
+    for t in tensors:
+        if t is not None:
+            _require_cuda(t)
+            if t.device != first.device:
+                raise ValueError(f"{op} requires all tensors on one device.")
+    return first.device
+
+
+def _row_counts(t: torch.Tensor | None, batch: int, op: str, name: str) -> torch.Tensor | None:
+    if t is None:
+        return None
+    if t.dtype != torch.int64 or t.shape != (batch,):
+        raise ValueError(f"{op} requires int64 {name} of one per sequence.")
+    return t.contiguous()
+
+
+def _cache_strides(t: torch.Tensor) -> tuple[int, int, int] | None:
+    """Element strides {batch, row, head} of a cache that the kernels can read and write in place, else None. The
+    stride of a dimension of one entry is never followed and is given as if the tensor were dense."""
+    b, n, h, d = t.shape
+    if t.stride(3) != 1 and d != 1:
+        return None
+    sb, sn, sh = t.stride()[:3]
+    sh = sh if h > 1 else d
+    sn = sn if n > 1 else h * sh
+    sb = sb if b > 1 else n * sn
+    vec = 16 // t.element_size()
+    if sh < d or min(sb, sn) < d or (sb | sn | sh) % vec or t.data_ptr() % 16:
+        return None
+    return sb, sn, sh
+
+
+def _validate_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, op: str) -> None:
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+        raise ValueError(f"{op} requires K and V caches of [batch, capacity, heads, head size].")
+    if k_cache.dtype != v_cache.dtype:
+        raise ValueError(f"{op} requires matching tensor dtypes.")
+
+
+def _readable_cache(t: torch.Tensor) -> tuple[torch.Tensor, tuple[int, int, int]]:
+    strides = _cache_strides(t)
+    if strides is None:
+        t = materialize(t) if not t.is_contiguous() else t.clone()
+        strides = (t.stride(0), t.stride(1), t.stride(2))
+    return t, strides
+
+
+def _cache_attention(op: str, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
+                     counts: torch.Tensor | None, extra: torch.Tensor, error: torch.Tensor | None):
+    """Checks that tree_attention and decoder_attention_weights share; returns what their calls need."""
+    _validate_caches(k_cache, v_cache, op)
+    if q.dim() != 4:
+        raise ValueError(f"{op} requires queries of [batch, tokens, heads, head size].")
+    if q.dtype != torch.bfloat16 or k_cache.dtype != torch.bfloat16:
+        raise ValueError(f"{op} requires bf16 queries and caches.")
+    if q.shape[0] != k_cache.shape[0]:
+        raise ValueError(f"{op} requires as many cached sequences as queries have.")
+    if q.shape[3] != k_cache.shape[3]:
+        raise ValueError(f"{op} requires matching query/key/value head sizes.")
+    if lengths is None:
+        raise ValueError(f"{op} requires int64 lengths of one per sequence.")
+    if error is not None and (error.dtype != torch.int32 or error.numel() != 1):
+        raise ValueError(f"{op} requires an int32 error word.")
+    device = _same_device(op, q, k_cache, v_cache, lengths, counts, extra, error)
+    lengths = _row_counts(lengths, q.shape[0], op, "lengths")
+    counts = _row_counts(counts, q.shape[0], op, "counts")
+    return device, lengths, counts
+
+
+def _address(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
+                   mask: torch.Tensor, nodes: torch.Tensor | None = None,
+                   error: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of drafted trees over a batch of caches (cppinf_tree_attention): q [B, T, Hq, D] holds one row per
+    drafted node, whose keys and values are cache rows lengths[b] .. lengths[b] + T - 1 of [B, capacity, Hkv, D]; node t
+    sees every committed row and the nodes j with mask[b, t, j] (bool [B, T, T], or [T, T] for one tree shape), as far
+    as nodes[b] (int64 [B]) reaches. Returns the bf16 context [B, T, Hq, D], zeros where a node is padding or sees
+    nothing. `error` (int32 [1]) is set when a wait of the kernel ran out of its poll limit."""
+    op = "tree_attention"
+    if mask.dtype != torch.bool or q.dim() != 4 or mask.dim() not in (2, 3) or \
+            mask.shape[-2:] != (q.shape[1], q.shape[1]) or (mask.dim() == 3 and mask.shape[0] != q.shape[0]):
+        raise ValueError("tree_attention requires a bool mask of [tokens, tokens], shared or one per sequence.")
+    device, lengths, nodes = _cache_attention(op, q, k_cache, v_cache, lengths, nodes, mask, error)
+    batch, tokens, q_heads, d = q.shape
+    capacity, kv_heads = k_cache.shape[1:3]
+    with torch.cuda.device(device):
+        q, mask = materialize(q), mask.contiguous()
+        k, ks = _readable_cache(k_cache)
+        v, vs = _readable_cache(v_cache)
+        ctx = torch.empty_like(q)
+        nbytes = int(capi.load().cppinf_cache_attention_scratch_bytes(batch, tokens, q_heads, kv_heads, d, capacity, 0))
+        scratch = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=device)
+        capi.call("cppinf_tree_attention", q.data_ptr(), k.data_ptr(), capi.i64_array(ks), v.data_ptr(),
+                  capi.i64_array(vs), lengths.data_ptr(), mask.data_ptr(),
+                  tokens * tokens if mask.dim() == 3 else 0, _address(nodes), ctx.data_ptr(), batch, tokens, q_heads,
+                  kv_heads, d, capacity, scratch.data_ptr(), nbytes, _address(error), _stream())
+    return ctx
+
+
+def tree_accept(token_ids: torch.Tensor, parents: torch.Tensor, predicted: torch.Tensor,
+                nodes: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The drafted nodes that greedy decoding agrees with (cppinf_tree_accept): int64 [B, T] drafted tokens, parent
+    nodes and the model's greedy token after each node. Returns (path [B, T], nodes passed from the root on and then -1;
+    counts [B]; next token [B])."""
+    op = "tree_accept"
+    if token_ids.dim() != 2 or token_ids.shape != parents.shape or token_ids.shape != predicted.shape:
+        raise ValueError("tree_accept requires tokens, parents and predictions of [batch, nodes].")
+    if any(t.dtype != torch.int64 for t in (token_ids, parents, predicted)):
+        raise ValueError("tree_accept requires int64 tokens, parents and predictions.")
+    device = _same_device(op, token_ids, parents, predicted, nodes)
+    batch, tokens = token_ids.shape
+    nodes = _row_counts(nodes, batch, op, "nodes")
+    with torch.cuda.device(device):
+        token_ids, parents, predicted = token_ids.contiguous(), parents.contiguous(), predicted.contiguous()
+        path = torch.empty((batch, tokens), dtype=torch.int64, device=device)
+        counts, following = torch.empty((2, batch), dtype=torch.int64, device=device).unbind(0)
+        capi.call("cppinf_tree_accept", token_ids.data_ptr(), parents.data_ptr(), predicted.data_ptr(), _address(nodes),
+                  path.data_ptr(), counts.data_ptr(), following.data_ptr(), batch, tokens, _stream())
+    return path, counts, following
+
+
+def tree_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor, path: torch.Tensor,
+                counts: torch.Tensor) -> None:
+    """Moves an accepted path's rows behind the committed ones, in place (cppinf_tree_commit): cache row
+    lengths[b] + i takes row lengths[b] + path[b, i] for i < counts[b]. The caller adds counts to lengths once every
+    layer's cache is committed."""
+    op = "tree_commit"
+    _validate_caches(k_cache, v_cache, op)
+    code = _dtype_code(k_cache, op)
+    batch, capacity, heads, d = k_cache.shape
+    if path.dtype != torch.int64 or path.dim() != 2 or path.shape[0] != batch:
+        raise ValueError("tree_commit requires an int64 path of [batch, nodes].")
+    device = _same_device(op, k_cache, v_cache, lengths, path, counts)
+    lengths = _row_counts(lengths, batch, op, "lengths")
+    counts = _row_counts(counts, batch, op, "counts")
+    ks, vs = _cache_strides(k_cache), _cache_strides(v_cache)
+    if ks is None or vs is None:
+        raise ValueError("tree_commit requires caches with dense 16-byte aligned rows.")
+    with torch.cuda.device(device):
+        path = path.contiguous()
+        capi.call("cppinf_tree_commit", code, k_cache.data_ptr(), capi.i64_array(ks), v_cache.data_ptr(),
+                  capi.i64_array(vs), lengths.data_ptr(), path.data_ptr(), counts.data_ptr(), batch, path.shape[1],
+                  heads, d, capacity, _stream())
+
+
+def decoder_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
+                              weights: torch.Tensor, counts: torch.Tensor | None = None,
+                              error: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of new tokens over a batch of caches (cppinf_decoder_attention_weights): query t of
+    q [B, T, Hq, D] sees rows 0 .. lengths[b] + t of caches [B, capacity, Hkv, D]. Adds to weights (f32
+    [B, Hkv, capacity], in place) each row's probabilities, summed over the queries and the query heads of its
+    key-value head, and returns the bf16 context [B, T, Hq, D]. Queries from counts[b] (int64 [B]) on are padding.
+    `error` as in tree_attention."""
+    op = "decoder_attention_weights"
+    device, lengths, counts = _cache_attention(op, q, k_cache, v_cache, lengths, counts, weights, error)
+    batch, tokens, q_heads, d = q.shape
+    capacity, kv_heads = k_cache.shape[1:3]
+    if weights.dtype != torch.float32 or weights.shape != (batch, kv_heads, capacity) or not weights.is_contiguous():
+        raise ValueError("decoder_attention_weights requires contiguous f32 weights of [batch, heads, capacity].")
+    with torch.cuda.device(device):
+        q = materialize(q)
+        k, ks = _readable_cache(k_cache)
+        v, vs = _readable_cache(v_cache)
+        ctx = torch.empty_like(q)
+        nbytes = int(capi.load().cppinf_cache_attention_scratch_bytes(batch, tokens, q_heads, kv_heads, d, capacity, 1))
+        scratch = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=device)
+        capi.call("cppinf_decoder_attention_weights", q.data_ptr(), k.data_ptr(), capi.i64_array(ks), v.data_ptr(),
+                  capi.i64_array(vs), lengths.data_ptr(), _address(counts), ctx.data_ptr(), weights.data_ptr(), batch,
+                  tokens, q_heads, kv_heads, d, capacity, scratch.data_ptr(), nbytes, _address(error), _stream())
+    return ctx
+
+
+def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Tensor, lengths: torch.Tensor, keep: int,
+                recent: int, sinks: int = 0, capacity: int | None = None):
+    """Cuts each sequence of a cache to `keep` rows, per key-value head (cppinf_cache_evict): the first `sinks`, the
+    last `recent` and the rows of the highest weight (f32 [B, Hkv, capacity]) between them stay, in their order.
+    Returns a new cache of `capacity` (default: keep) rows: (K [B, capacity, Hkv, D], V, weights [B, Hkv, capacity],
+    lengths [B], index [B, Hkv, keep] of the kept rows, -1 behind a shorter sequence's); unused rows are zeros."""
+    op = "cache_evict"
+    _validate_caches(k_cache, v_cache, op)
+    code = _dtype_code(k_cache, op)
+    batch, rows, heads, d = k_cache.shape
+    keep, recent, sinks = int(keep), int(recent), int(sinks)
+    capacity = keep if capacity is None else int(capacity)
+    if weights.dtype != torch.float32 or weights.shape != (batch, heads, rows):
+        raise ValueError("cache_evict requires f32 weights of [batch, heads, capacity].")
+    if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
+        raise ValueError("cache_evict requires keep to be at least one and to cover recent and sinks.")
+    if capacity < keep:
+        raise IndexError("cache_evict output is too small for the kept rows.")
+    device = _same_device(op, k_cache, v_cache, weights, lengths)
+    lengths = _row_counts(lengths, batch, op, "lengths")
+    with torch.cuda.device(device):
+        weights = materialize(weights)
+        k, ks = _readable_cache(k_cache)
+        v, vs = _readable_cache(v_cache)
+        k_out = torch.empty((batch, capacity, heads, d), dtype=k.dtype, device=device)
+        v_out = torch.empty_like(k_out)
+        w_out = torch.empty((batch, heads, capacity), dtype=torch.float32, device=device)
+        left = torch.empty(batch, dtype=torch.int64, device=device)
+        index = torch.empty((batch, heads, keep), dtype=torch.int64, device=device)
+        capi.call("cppinf_cache_evict", code, k.data_ptr(), capi.i64_array(ks), v.data_ptr(), capi.i64_array(vs),
+                  weights.data_ptr(), lengths.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), w_out.data_ptr(),
+                  left.data_ptr(), index.data_ptr(), batch, heads, d, rows, keep, recent, sinks, capacity, _stream())
+    return k_out, v_out, w_out, left, index
+
+
 def embedding(table: torch.Tensor, token_ids: torch.Tensor) -> torch.Tensor:
     """Embedding lookup, src/models/qwen3/qwen3_model.cpp:132-165 (ids must be in range; they are checked here)."""
     if table.dim() != 2:

@@ -267,6 +267,91 @@ CPPINF_API int cppinf_decoder_attention_tc(const void* q, const void* k_cache, c
                                            int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
                                            int64_t position, int64_t capacity, unsigned int* error, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Batches of cached sequences: verification of drafted trees, attention weights and eviction. No counterpart in the
+ * reference, whose decoding feeds one token per sequence and whose caches only grow.
+ *
+ * A cache is a K and a V tensor of [batch, capacity, kv_heads, head_dim] whose rows of head_dim elements are dense;
+ * `k_strides` / `v_strides` are HOST arrays of 3 element strides {batch, row, head}, so views of a larger cache (one
+ * layer of many, K and V interleaved) are read and written in place. Strides must be multiples of 16 bytes and the
+ * base addresses 16-byte aligned. `lengths` (DEVICE int64, one per sequence) are the committed rows; the new tokens of
+ * a call occupy the rows after them. They are read on the device, so a captured call follows them from replay to
+ * replay; they cannot be refused there, so a length is taken as 0 below 0 and as the capacity above it, and a new token
+ * whose row would lie past the capacity counts as padding. Query head h reads key-value head
+ * h / (q_heads / kv_heads); up to 128 query heads share one. Rows of a cache that no query sees may hold anything, NaN
+ * and infinities included.
+ * ------------------------------------------------------------------------------------------------------------- */
+
+/* Device scratch, in bytes, that cppinf_tree_attention (with_weights 0) or cppinf_decoder_attention_weights (1) needs
+ * for these sizes on the current device; 16-byte aligned, contents arbitrary, not shared by calls that overlap in time.
+ * A negative number: sizes that the entry points refuse. */
+CPPINF_API int64_t cppinf_cache_attention_scratch_bytes(int64_t batch, int64_t tokens, int64_t q_heads,
+                                                        int64_t kv_heads, int64_t head_dim, int64_t capacity,
+                                                        int with_weights);
+
+/* Attention of drafted trees: q [batch, tokens, q_heads, head_dim] bf16, one row per node (after q-norm and RoPE at
+ * the node's depth), whose keys and values are cache rows lengths[b] + node. Node t sees every committed row and the
+ * drafted node j where mask[b * mask_batch_stride + t * tokens + j] is not 0 (DEVICE bytes; stride 0 shares one mask;
+ * a tree's mask has each node's ancestors and the node itself). `nodes` (DEVICE int64, may be NULL: all) counts each
+ * sequence's nodes; later ones are padding, seen by none, and their rows of ctx are zeros, as is the row of a node that
+ * sees nothing. ctx [batch, tokens, q_heads, head_dim] bf16 = softmax(q k^T / sqrt(head_dim)) v. tokens <= 256,
+ * head_dim 64, 128 or 256. `error` (DEVICE, may be NULL) is set to 1 when a wait of the kernel ran out of its poll
+ * limit (cppinf_set_wait_poll_limit). */
+CPPINF_API int cppinf_tree_attention(const void* q, const void* k_cache, const int64_t* k_strides,
+                                     const void* v_cache, const int64_t* v_strides, const int64_t* lengths,
+                                     const uint8_t* mask, int64_t mask_batch_stride, const int64_t* nodes, void* ctx,
+                                     int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads,
+                                     int64_t head_dim, int64_t capacity, void* scratch, int64_t scratch_bytes,
+                                     unsigned int* error, void* stream);
+
+/* The drafted tokens that greedy decoding agrees with. tokens, parents, predicted: DEVICE int64 [batch,
+ * tokens_per_sequence]: each node's drafted token, its parent's node index (node 0 is the root, the token that the
+ * model produced last) and the model's greedy token after it (the argmax of the node's logits). From the root, the walk
+ * goes to the lowest child c of the current node p (a higher index than p) with tokens[c] == predicted[p], as long as
+ * there is one. path [batch, tokens_per_sequence] receives the nodes passed, the root first, then -1; counts [batch]
+ * their number; next [batch] predicted[last node]. A sequence of no nodes gives 0 and -1. `nodes` as in
+ * cppinf_tree_attention. tokens_per_sequence <= 256. */
+CPPINF_API int cppinf_tree_accept(const int64_t* tokens, const int64_t* parents, const int64_t* predicted,
+                                  const int64_t* nodes, int64_t* path, int64_t* counts, int64_t* next, int64_t batch,
+                                  int64_t tokens_per_sequence, void* stream);
+
+/* Moves an accepted path's cache rows behind the committed ones, in place: row lengths[b] + i of K and V takes row
+ * lengths[b] + path[b, i] for i < counts[b] (path [batch, tokens] and counts as cppinf_tree_accept writes them;
+ * ascending, path[b, i] >= i; an entry outside that order or past the new rows is skipped). Other rows, and `lengths`,
+ * are left as they are: the caller adds counts to lengths when every layer's cache has been committed. */
+CPPINF_API int cppinf_tree_commit(cppinf_dtype dtype, void* k_cache, const int64_t* k_strides, void* v_cache,
+                                  const int64_t* v_strides, const int64_t* lengths, const int64_t* path,
+                                  const int64_t* counts, int64_t batch, int64_t tokens, int64_t kv_heads,
+                                  int64_t head_dim, int64_t capacity, void* stream);
+
+/* Causal attention of new tokens over a batch of caches, with the weight that each cached row received: query t of
+ * sequence b (q [batch, tokens, q_heads, head_dim] bf16) sees rows 0 .. lengths[b] + t, ctx as in
+ * cppinf_tree_attention, and weights[b, h, j] (f32 dense [batch, kv_heads, capacity]) grows by the sum, over the
+ * sequence's queries and the query heads of key-value head h, of row j's probability (f32, in an order that does not
+ * change from call to call). Rows past the new tokens keep their weight. `counts` (DEVICE int64, may be NULL: all)
+ * are the valid queries of each sequence; later ones are padding: zero rows of ctx, no weight. head_dim 64, 128 or
+ * 256; any number of tokens. `error` as in cppinf_tree_attention. */
+CPPINF_API int cppinf_decoder_attention_weights(const void* q, const void* k_cache, const int64_t* k_strides,
+                                                const void* v_cache, const int64_t* v_strides, const int64_t* lengths,
+                                                const int64_t* counts, void* ctx, float* weights, int64_t batch,
+                                                int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
+                                                int64_t capacity, void* scratch, int64_t scratch_bytes,
+                                                unsigned int* error, void* stream);
+
+/* Cuts each sequence of a cache to `keep` rows, per key-value head: the first `sinks` rows, the last `recent` and, of
+ * the others, those of the highest weight (f32 dense [batch, kv_heads, capacity]; equal weights: the lowest rows; NaN
+ * below every number) stay, in their order; a sequence of no more than `keep` rows stays whole. Kept rows go to k_out
+ * and v_out (dense [batch, out_capacity, kv_heads, head_dim], out_capacity >= keep, not overlapping the cache), their
+ * weights to weights_out (f32 [batch, kv_heads, out_capacity]); what follows the kept rows is zeros. lengths_out
+ * [batch] = min(lengths, keep); index (int64 [batch, kv_heads, keep]) the kept rows, then -1. Keys carry their rotary
+ * position with them, so later queries keep their own positions. Needs keep >= 1, sinks + recent <= keep. */
+CPPINF_API int cppinf_cache_evict(cppinf_dtype dtype, const void* k_cache, const int64_t* k_strides,
+                                  const void* v_cache, const int64_t* v_strides, const float* weights,
+                                  const int64_t* lengths, void* k_out, void* v_out, float* weights_out,
+                                  int64_t* lengths_out, int64_t* index, int64_t batch, int64_t kv_heads,
+                                  int64_t head_dim, int64_t capacity, int64_t keep, int64_t recent, int64_t sinks,
+                                  int64_t out_capacity, void* stream);
+
 /* Embedding lookup (src/models/qwen3/qwen3_model.cpp:132-165): out[t] = table[token_ids[t]], table [vocab, hidden]
  * bf16, token_ids a DEVICE int64 array. Ids are validated on the host by the model; here they are clamped into
  * range. hidden must be a multiple of 8. */
