@@ -7,16 +7,37 @@
 // With s_j = q k_j / sqrt(D) over the rows j that a query sees, M their maximum and l = sum exp(s_j - M):
 // ctx = sum exp(s_j - M) v_j / l, and row j's weight is the sum over the queries and the query heads of a key-value
 // head of exp(s_j - M) / l. Scores, M, l and both sums are f32; exponentials are taken in base 2 with log2(e) / sqrt(D)
-// folded into one factor.
+// folded into one factor. Probabilities are rounded to bf16 for their product with V (the tensor cores' operand type;
+// the sum l keeps them in f32), contexts once at the end.
 //
-// One warp per (query, head) walks the visible rows with the running maximum and sum of a softmax, lanes over the head
-// dimension; a second kernel, one warp per cached row and key-value head, reads the queries back with each one's M and
-// l and adds the row's probabilities up in a fixed order.
+// Attention on the tensor cores (cache_attention_kernel). The G query heads of a key-value head share its K and V, so
+// the rows (token, query head of the group) of one key-value head are packed into tiles of 128, the rows of a
+// tcgen05.mma; a warpgroup of four warps owns such a tile's softmax, one thread per row. One pass over the keys, in
+// tiles that TMA brings into a ring of shared-memory slots:
+//     S = Q K^T (tensor memory) -> running maximum, P = exp2(...) written over S as bf16 -> O += P V (P from tensor
+//     memory, V as an MN-major operand straight from its TMA tile).
+// Two such chains run side by side and hide each other's softmax behind the other's matrix products: with up to 128
+// rows per head, two key tiles in turn for one row tile (their sums are joined at the end); with more, two row tiles
+// on the same K and V tiles, which are then read once for 256 rows. Head size 256 has room for one chain.
+// O is rescaled only when a row's maximum has grown by more than 2^8 since the last time.
+//
+// All key tiles of all (sequence, row tile, key-value head) items form one line that is cut into equal parts, one per
+// CTA (one CTA per SM), so ragged lengths and few sequences load all SMs alike. A CTA that takes only part of an item
+// leaves its rows' maximum, sum and unnormalised O in the scratch, and a second kernel joins the parts of the items
+// that a cut went through, in the order of their keys.
+//
+// Rows past a sequence's end and drafted rows that only some queries see may hold anything: scores there are replaced
+// before the softmax, and V tiles in which some row is hidden from some query are cleared of such values in shared
+// memory before the product (0 * NaN would be NaN); values that are not finite in a row that a query does see are added
+// to its O afterwards.
 #include "common.cuh"
 #include "runtime.h"
+#include "tcgen05.cuh"
 
 namespace cppinf::device {
 namespace {
+
+using namespace tc;
 
 constexpr int kMaxNodes = 256;  // drafted tokens of a sequence
 constexpr int kMaxGroup = 128;  // query heads of a key-value head
@@ -32,13 +53,26 @@ struct CacheAttentionParams {
     const uint8_t* mask;     // tree: [T, T] at mask + b * mask_stride; null: causal
     int64_t mask_stride;
     bf16* ctx;        // [B, T, Hq, D]
-    float2* stats;    // [B, T, Hq] (M in base 2, 1 / l), or null
+    float2* stats;    // [B, Hkv, T, G] (M in base 2, 1 / l), or null
     float* weights;   // [B, Hkv, capacity]
     int64_t batch;
     int64_t tokens;
     int64_t q_heads;
     int64_t kv_heads;
     int64_t capacity;
+    // Tiling (plan()) and scratch.
+    int group;            // query heads of a key-value head
+    int tile_tokens;      // tokens of a 128-row tile
+    int item_tokens;      // tokens of an item: one or two tiles
+    int row_tiles;        // items along the tokens
+    int q_box_tokens;     // tokens of one TMA box of q
+    int part_rows;        // rows of a part in the scratch
+    int4* cuts;           // [CTAs] where each CTA's part of the line begins: sequence, row tile, head, key tile
+    int64_t* line;        // length of the line
+    float2* part_ml;      // [2 CTAs][part_rows] (M in base 2, l)
+    float* part_o;        // [2 CTAs][part_rows][D]
+    unsigned int* error;
+    uint32_t poll_limit;
 };
 
 // Committed rows and valid queries of a sequence, forced into the ranges that keep every access inside the cache: a
@@ -55,9 +89,740 @@ __device__ __forceinline__ int64_t valid_queries(const CacheAttentionParams& p, 
     return n < 0 ? 0 : (n > most ? most : n);
 }
 
-// Whether query t sees new row j (0 <= j < the sequence's valid queries).
-__device__ __forceinline__ bool sees(const CacheAttentionParams& p, int64_t b, int64_t t, int64_t j) {
-    return p.mask == nullptr ? j <= t : p.mask[b * p.mask_stride + t * p.tokens + j] != 0;
+// What one item needs to know about its sequence (capacities lie below 2^31).
+struct ItemRange {
+    int len;       // committed rows
+    int valid;     // valid queries
+    int first;     // first token of the item
+    int full_end;  // keys below are seen by every valid query of the item
+    int kv_end;    // keys from here on are seen by none
+};
+
+__device__ __forceinline__ ItemRange item_range(const CacheAttentionParams& p, int b, int row_tile) {
+    ItemRange r;
+    r.len = static_cast<int>(committed_rows(p, b));
+    r.valid = static_cast<int>(valid_queries(p, b));
+    r.first = row_tile * p.item_tokens;
+    if (r.first >= r.valid) {
+        r.full_end = 0;
+        r.kv_end = 0;
+    } else if (p.mask != nullptr) {
+        r.full_end = r.len;
+        r.kv_end = r.len + r.valid;
+    } else {
+        const int last = r.first + p.item_tokens;
+        r.full_end = r.len + r.first + 1;
+        r.kv_end = r.len + (last < r.valid ? last : r.valid);
+    }
+    return r;
+}
+
+// Key tiles of an item; one without visible keys still takes a tile, in which its rows become zeros.
+template <int kKeys>
+__device__ __forceinline__ int item_tiles(const ItemRange& r) {
+    return r.kv_end > 0 ? (r.kv_end + kKeys - 1) / kKeys : 1;
+}
+
+// Head size's tiling: keys of a tile, chains side by side, slots of the K/V ring, shared memory.
+template <int D, bool kPair>
+struct Tiling {
+    static constexpr int kKeys = D == 256 ? 64 : 128;
+    static constexpr int kStreams = D == 256 ? 1 : 2;
+    static constexpr int kAtoms = D / 64;
+    static constexpr int kQTiles = kPair ? 2 : 1;
+    static constexpr int kAhead = kPair ? 1 : kStreams;  // K tiles loaded before the first V tile
+    static constexpr int kSlots = D == 64 ? 8 : 4;
+    static constexpr int kThreads = 128 + 128 * kStreams;
+    static constexpr uint32_t kQAtom = 128 * 128;                // [128 rows][64 dims]
+    static constexpr uint32_t kKvAtom = kKeys * 128;             // [keys][64 dims]
+    static constexpr uint32_t kSlot = kKvAtom * kAtoms;
+    static constexpr uint32_t kQ = 0;
+    static constexpr uint32_t kRing = kQ + kQTiles * kAtoms * kQAtom;
+    static constexpr uint32_t kExchange = kRing + kSlots * kSlot;  // O columns of the second chain, [128][33] f32
+    static constexpr uint32_t kMask = kExchange + (kStreams == 2 && !kPair ? 128 * 33 * 4 : 0);  // [chains][128][9]
+    static constexpr uint32_t kMl = kMask + kStreams * 128 * 9 * 4;
+    static constexpr uint32_t kFlags = kMl + 128 * 8;
+    static constexpr uint32_t kBars = kFlags + 2 * 16 * 4;
+    static constexpr std::size_t kBytes = 1024 + kBars + 256;
+    // Tensor memory columns: the chains' S (P over it), then their O.
+    static constexpr uint32_t kTmemO = kStreams * kKeys;
+    static_assert(kStreams * (kKeys + D) <= 512, "tensor memory has 512 columns");
+    static_assert(kBytes <= 232448, "shared memory of a CTA");
+};
+
+constexpr uint32_t kTmemAll = 512;
+
+// Where a CTA's part of the line is, item by item; every role of the CTA walks it for itself.
+struct Walk {
+    int b;
+    int row_tile;
+    int h;
+    int tile;       // first key tile of the current segment
+    int64_t left;   // key tiles of the part still to come, the current segment's included
+    uint32_t fills; // ring slots filled before the current segment
+    int index;      // segments before the current one
+};
+
+__device__ __forceinline__ void advance(const CacheAttentionParams& p, Walk& w, int count, int tiles) {
+    w.left -= count;
+    w.fills += 2u * static_cast<uint32_t>(count);
+    ++w.index;
+    w.tile += count;
+    if (w.tile >= tiles) {
+        w.tile = 0;
+        if (++w.h == static_cast<int>(p.kv_heads)) {
+            w.h = 0;
+            if (++w.row_tile == p.row_tiles) {
+                w.row_tile = 0;
+                ++w.b;
+            }
+        }
+    }
+}
+
+// Fill numbers of a segment's K and V tiles: `ahead` K tiles first, then V and K tiles in turn.
+__device__ __forceinline__ uint32_t fill_of_k(uint32_t fills, int i, int ahead) {
+    return fills + static_cast<uint32_t>(i < ahead ? i : 2 * i - ahead + 1);
+}
+
+__device__ __forceinline__ uint32_t fill_of_v(uint32_t fills, int i, int ahead, int count) {
+    const int lead = count < ahead ? count : ahead;
+    const int k = i < count - lead ? i : count - lead;
+    return fills + static_cast<uint32_t>(lead + i + k);
+}
+
+// Bounded waits: one that runs out of the poll limit sets the error word and waits again with the default limit; if
+// that runs out too, `stop` ends all later waits of the CTA at once, so that it always comes to its end.
+struct Waiter {
+    unsigned int* error;
+    uint32_t limit;
+    volatile uint32_t* stop;
+
+    __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t phase) const {
+        if (mbar_wait_bounded(bar, phase, limit < 64u ? limit : 64u) || *stop != 0u) {
+            return;
+        }
+        if (mbar_wait_bounded(bar, phase, limit)) {
+            return;
+        }
+        if (error != nullptr) {
+            atomicOr(error, 1u);
+        }
+        if (!mbar_wait_bounded(bar, phase)) {
+            *stop = 1u;
+        }
+    }
+};
+
+// Visible keys [key, key + 32) of a row as a bit mask. Tree: committed keys, then the row's mask bits (9 words, the last
+// empty); causal: keys below `limit`.
+__device__ __forceinline__ uint32_t visible_bits(const uint32_t* row, int key, int len, int limit) {
+    if (row == nullptr) {
+        const int n = limit - key;
+        return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
+    }
+    const int j = key - len;
+    if (j <= -32) {
+        return 0xffffffffu;
+    }
+    if (j < 0) {
+        return (row[0] << -j) | ((1u << -j) - 1u);
+    }
+    const int word = j >> 5;
+    return word >= 8 ? 0u : __funnelshift_r(row[word], row[word + 1], static_cast<uint32_t>(j & 31));
+}
+
+// A pair of bf16 values with +0 in the place of each that is not finite.
+__device__ __forceinline__ uint32_t finite_pair(uint32_t pair) {
+    return ((pair & 0x7f80u) == 0x7f80u ? 0u : pair & 0xffffu) |
+           ((pair & 0x7f800000u) == 0x7f800000u ? 0u : pair & 0xffff0000u);
+}
+
+template <int D, bool kPair>
+__global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
+    cache_attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                           const __grid_constant__ CUtensorMap map_v, const CacheAttentionParams p) {
+    using L = Tiling<D, kPair>;
+    constexpr int kStreams = L::kStreams;
+    constexpr int kKeys = L::kKeys;
+    constexpr int kAhead = L::kAhead;
+    extern __shared__ __align__(16) unsigned char raw[];
+    unsigned char* sm = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
+    uint32_t* s_mask = reinterpret_cast<uint32_t*>(sm + L::kMask);
+    float2* s_ml = reinterpret_cast<float2*>(sm + L::kMl);
+    float* s_exchange = reinterpret_cast<float*>(sm + L::kExchange);
+    uint32_t* s_flags = reinterpret_cast<uint32_t*>(sm + L::kFlags);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::kBars);
+    uint64_t* bar_full = bars;                    // [slots] a K or V tile has landed
+    uint64_t* bar_empty = bars + L::kSlots;       // [slots] its products are done
+    uint64_t* bar_q_full = bars + 2 * L::kSlots;
+    uint64_t* bar_q_empty = bar_q_full + 1;
+    uint64_t* bar_s = bar_q_empty + 1;            // [chains] S is complete
+    uint64_t* bar_p = bar_s + kStreams;           // [chains] P is written
+    uint64_t* bar_o = bar_p + kStreams;           // [chains] the segment's O is complete
+    __shared__ uint32_t s_tmem;
+    __shared__ uint32_t s_stop;
+    __shared__ Walk s_walk;
+
+    const int tid = threadIdx.x;
+    const int warp = tid >> 5;
+    const int lane = tid & 31;
+    if (tid == 0) {
+        s_stop = 0u;
+        for (int i = 0; i < L::kSlots; ++i) {
+            mbar_init(bar_full + i, 1);
+            mbar_init(bar_empty + i, 1);
+        }
+        mbar_init(bar_q_full, 1);
+        mbar_init(bar_q_empty, 1);
+        for (int w = 0; w < kStreams; ++w) {
+            mbar_init(bar_s + w, 1);
+            mbar_init(bar_p + w, 4);
+            mbar_init(bar_o + w, 1);
+        }
+    }
+    if (warp == 2) {
+        tmem_alloc(&s_tmem, kTmemAll);
+    }
+    grid_dependency_begin();
+    if (warp == 0) {  // the line's length, and where this CTA's part of it begins
+        const int64_t entries = p.batch * p.row_tiles;
+        const auto tiles_at = [&](int64_t e) -> int64_t {
+            if (e >= entries) {
+                return 0;
+            }
+            const int b = static_cast<int>(e / p.row_tiles);
+            return item_tiles<kKeys>(item_range(p, b, static_cast<int>(e - int64_t{b} * p.row_tiles))) * p.kv_heads;
+        };
+        int64_t total = 0;
+        for (int64_t e = lane; e - lane < entries; e += 32) {
+            total += tiles_at(e);
+        }
+        for (int offset = 16; offset > 0; offset >>= 1) {
+            total += __shfl_xor_sync(0xffffffffu, total, offset);
+        }
+        const int64_t begin = total * blockIdx.x / gridDim.x;
+        const int64_t end = total * (blockIdx.x + 1) / gridDim.x;
+        int64_t before = 0;
+        for (int64_t e0 = 0; e0 < entries; e0 += 32) {
+            const int64_t mine = tiles_at(e0 + lane);
+            int64_t sum = mine;
+            for (int offset = 1; offset < 32; offset <<= 1) {
+                const int64_t other = __shfl_up_sync(0xffffffffu, sum, offset);
+                sum += lane >= offset ? other : 0;
+            }
+            const int64_t lo = before + sum - mine;
+            if (begin >= lo && begin < lo + mine) {
+                const int64_t e = e0 + lane;
+                const int64_t each = mine / p.kv_heads;
+                Walk w;
+                w.b = static_cast<int>(e / p.row_tiles);
+                w.row_tile = static_cast<int>(e % p.row_tiles);
+                w.h = static_cast<int>((begin - lo) / each);
+                w.tile = static_cast<int>((begin - lo) % each);
+                w.left = end - begin;
+                w.fills = 0;
+                w.index = 0;
+                s_walk = w;
+                p.cuts[blockIdx.x] = make_int4(w.b, w.row_tile, w.h, w.tile);
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
+            if (before > begin) {
+                break;
+            }
+        }
+        if (blockIdx.x == 0 && lane == 0) {
+            *p.line = total;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    const Waiter wait{p.error, p.poll_limit, &s_stop};
+    Walk at = s_walk;
+    // Chains at work in a segment of `count` key tiles.
+    const auto chains_of = [&](const ItemRange& r, int count) {
+        return kStreams == 1 ? 1 : kPair ? (r.first + p.tile_tokens < p.tokens ? 2 : 1) : (count < 2 ? count : 2);
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {  // ---- loads
+            uint32_t fill = 0;
+            const auto load = [&](const CUtensorMap* map, int b, int h, int tile) {
+                const uint32_t slot = fill % L::kSlots;
+                const uint32_t round = fill / L::kSlots;
+                if (round > 0) {
+                    wait(bar_empty + slot, (round - 1) & 1u);
+                }
+                mbar_arrive_expect_tx(bar_full + slot, L::kSlot);
+                unsigned char* dst = sm + L::kRing + slot * L::kSlot;
+                for (int a = 0; a < L::kAtoms; ++a) {
+                    tma_load_4d(dst + a * L::kKvAtom, map, a * 64, h, tile * kKeys, b, bar_full + slot);
+                }
+                ++fill;
+            };
+            while (at.left > 0) {
+                const ItemRange r = item_range(p, at.b, at.row_tile);
+                const int tiles = item_tiles<kKeys>(r);
+                const int count = static_cast<int>(tiles - at.tile < at.left ? tiles - at.tile : at.left);
+                if (at.index > 0) {
+                    wait(bar_q_empty, static_cast<uint32_t>(at.index - 1) & 1u);
+                }
+                const int q_tiles = kPair ? chains_of(r, count) : 1;
+                const uint32_t box = static_cast<uint32_t>(p.q_box_tokens * p.group) * 128u;
+                mbar_arrive_expect_tx(bar_q_full, box * L::kAtoms * q_tiles);
+                for (int i = 0; i < q_tiles; ++i) {
+                    for (int a = 0; a < L::kAtoms; ++a) {
+                        tma_load_4d(sm + L::kQ + (i * L::kAtoms + a) * L::kQAtom, &map_q, a * 64, at.h * p.group,
+                                    r.first + i * p.tile_tokens, at.b, bar_q_full);
+                    }
+                }
+                const int lead = count < kAhead ? count : kAhead;
+                for (int i = 0; i < lead; ++i) {
+                    load(&map_k, at.b, at.h, at.tile + i);
+                }
+                for (int i = 0; i < count; ++i) {
+                    load(&map_v, at.b, at.h, at.tile + i);
+                    if (i + lead < count) {
+                        load(&map_k, at.b, at.h, at.tile + i + lead);
+                    }
+                }
+                advance(p, at, count, tiles);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {  // ---- matrix products
+            constexpr uint32_t s_idesc = idesc_bf16_f32(kKeys);
+            constexpr uint32_t o_idesc = idesc_bf16_f32_bmn(D);
+            uint32_t p_phase[kStreams] = {};
+            const auto slot_of = [&](uint32_t fill) { return fill % L::kSlots; };
+            const auto landed = [&](uint32_t fill) {
+                wait(bar_full + slot_of(fill), (fill / L::kSlots) & 1u);
+                tc_fence_after();
+            };
+            // S of chain w = its Q tile times the K tile of `fill`.
+            const auto scores = [&](int w, uint32_t fill) {
+                const unsigned char* q = sm + L::kQ + (kPair ? w * L::kAtoms * L::kQAtom : 0);
+                const unsigned char* k = sm + L::kRing + slot_of(fill) * L::kSlot;
+#pragma unroll
+                for (int i = 0; i < D / kUmmaK; ++i) {
+                    const uint32_t in = static_cast<uint32_t>(i & 3) * 32u;
+                    umma_bf16(tmem + w * kKeys, smem_desc_sw128(q, (i >> 2) * L::kQAtom + in),
+                              smem_desc_sw128(k, (i >> 2) * L::kKvAtom + in), s_idesc, i > 0 ? 1u : 0u);
+                }
+                umma_commit(bar_s + w);
+            };
+            // O of chain w += its P times the V tile of `fill`.
+            const auto product = [&](int w, uint32_t fill, bool first) {
+                wait(bar_p + w, p_phase[w]);
+                p_phase[w] ^= 1u;
+                tc_fence_after();
+                const unsigned char* v = sm + L::kRing + slot_of(fill) * L::kSlot;
+#pragma unroll
+                for (int i = 0; i < kKeys / kUmmaK; ++i) {
+                    umma_bf16_ta(tmem + L::kTmemO + w * D, tmem + w * kKeys + i * 8,
+                                 smem_desc_sw128_mn(v, i * 2048u, L::kKvAtom), o_idesc, (!first || i > 0) ? 1u : 0u);
+                }
+            };
+            while (at.left > 0) {
+                const ItemRange r = item_range(p, at.b, at.row_tile);
+                const int tiles = item_tiles<kKeys>(r);
+                const int count = static_cast<int>(tiles - at.tile < at.left ? tiles - at.tile : at.left);
+                const int chains = chains_of(r, count);
+                wait(bar_q_full, static_cast<uint32_t>(at.index) & 1u);
+                tc_fence_after();
+                const int lead = count < kAhead ? count : kAhead;
+                for (int i = 0; i < lead; ++i) {
+                    const uint32_t fill = fill_of_k(at.fills, i, lead);
+                    landed(fill);
+                    for (int w = kPair ? 0 : i; w < (kPair ? chains : i + 1); ++w) {
+                        scores(w, fill);
+                    }
+                    umma_commit(bar_empty + slot_of(fill));
+                }
+                if (count == lead) {
+                    umma_commit(bar_q_empty);
+                }
+                for (int i = 0; i < count; ++i) {
+                    const uint32_t vf = fill_of_v(at.fills, i, lead, count);
+                    const uint32_t kf = fill_of_k(at.fills, i + lead, lead);
+                    const bool more = i + lead < count;
+                    landed(vf);
+                    const int w0 = kPair ? 0 : i % kStreams;
+                    const int w1 = kPair ? chains : w0 + 1;
+                    for (int w = w0; w < w1; ++w) {
+                        product(w, vf, kPair ? i == 0 : i < kStreams);
+                        if (w == w1 - 1) {
+                            umma_commit(bar_empty + slot_of(vf));
+                        }
+                        if (more) {
+                            if (w == w0) {
+                                landed(kf);
+                            }
+                            scores(w, kf);
+                        } else {
+                            umma_commit(bar_o + w);
+                        }
+                    }
+                    if (more) {
+                        umma_commit(bar_empty + slot_of(kf));
+                        if (i + lead == count - 1) {
+                            umma_commit(bar_q_empty);
+                        }
+                    }
+                }
+                advance(p, at, count, tiles);
+            }
+        }
+    } else if (warp >= 4) {  // ---- softmax: chain w, one thread per row
+        const int w = (warp - 4) >> 2;
+        const int row = tid & 127;
+        const int g = row % p.group;
+        const int token_in_tile = row / p.group;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t t_s = tmem + lanes + w * kKeys;
+        const uint32_t t_o = tmem + lanes + L::kTmemO + w * D;
+        const float c2 = 1.4426950408889634f / sqrtf(static_cast<float>(D));
+        uint32_t s_phase = 0;
+        uint32_t o_phase = 0;
+        while (at.left > 0) {
+            const ItemRange r = item_range(p, at.b, at.row_tile);
+            const int tiles = item_tiles<kKeys>(r);
+            const int count = static_cast<int>(tiles - at.tile < at.left ? tiles - at.tile : at.left);
+            const int chains = chains_of(r, count);
+            if (w >= chains) {
+                advance(p, at, count, tiles);
+                continue;
+            }
+            const int token0 = r.first + (kPair ? w * p.tile_tokens : 0);
+            const int t = token0 + token_in_tile;
+            const bool inside = token_in_tile < p.tile_tokens && t < p.tokens;  // a row of ctx
+            const bool valid = inside && t < r.valid;
+            const bool busy = __any_sync(0xffffffffu, inside);
+            const int limit = valid ? r.len + t + 1 : 0;
+            const int lead = count < kAhead ? count : kAhead;
+            const int part0 = r.full_end / kKeys * kKeys;  // first key of the first tile in which a key may be hidden
+            const bool hides = (at.tile + count) * kKeys > r.full_end;  // the segment has such tiles
+            const uint32_t* bits_row = nullptr;
+            if (hides) {
+                if (row < 16) {
+                    s_flags[w * 16 + row] = 0u;
+                }
+                if (p.mask != nullptr) {  // the tile's mask rows as bits
+                    uint32_t* words = s_mask + w * 128 * 9;
+                    const uint8_t* mask = p.mask + at.b * p.mask_stride;
+                    for (int i = warp & 3; i < p.tile_tokens; i += 4) {
+                        const int64_t tt = token0 + i;
+                        bool on[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const int j = k * 32 + lane;
+                            on[k] = tt < r.valid && j < r.valid && mask[tt * p.tokens + j] != 0;
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            const uint32_t word = __ballot_sync(0xffffffffu, on[k]);
+                            if (lane == k) {
+                                words[i * 9 + k] = word;
+                            }
+                        }
+                        if (lane == 8) {
+                            words[i * 9 + 8] = 0u;
+                        }
+                    }
+                    bits_row = words + (token_in_tile < p.tile_tokens ? token_in_tile : 0) * 9;
+                }
+                named_barrier(1 + w, 128);
+            }
+            float top = -INFINITY;  // the maximum that P is taken against, in units of S
+            float sum = 0.0f;
+            for (int i = kPair ? 0 : w; i < count; i += kPair ? 1 : kStreams) {
+                const int key0 = (at.tile + i) * kKeys;
+                const bool partial = key0 + kKeys > r.full_end;
+                wait(bar_s + w, s_phase);
+                s_phase ^= 1u;
+                tc_fence_after();
+                if (busy) {
+                    float tile_top = -INFINITY;
+#pragma unroll 1
+                    for (int c = 0; c < kKeys / 32; ++c) {
+                        float x[32];
+                        tmem_load32(t_s + c * 32, x);
+                        const uint32_t see =
+                            partial ? visible_bits(bits_row, key0 + c * 32, r.len, limit) : 0xffffffffu;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            tile_top = fmaxf(tile_top, (see >> j & 1u) != 0u ? x[j] : -INFINITY);
+                        }
+                    }
+                    const float new_top = fmaxf(top, tile_top);
+                    const bool first = i < kStreams && (!kPair || i == 0);
+                    const bool grown = first || (new_top - top) * c2 > 8.0f;
+                    if (!first && __any_sync(0xffffffffu, grown)) {
+                        const float f = grown ? exp2_approx((top - new_top) * c2) : 1.0f;
+                        sum *= f;
+#pragma unroll 1
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t o[16];
+                            tmem_load16(t_o + c * 16, o);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                            }
+                            tmem_store16(t_o + c * 16, o);
+                        }
+                    }
+                    top = grown ? new_top : top;
+                    const float shift = top == -INFINITY ? 0.0f : top * c2;
+                    float part[4] = {};
+#pragma unroll 1
+                    for (int c = 0; c < kKeys / 32; ++c) {
+                        float x[32];
+                        tmem_load32(t_s + c * 32, x);
+                        const uint32_t see =
+                            partial ? visible_bits(bits_row, key0 + c * 32, r.len, limit) : 0xffffffffu;
+                        uint32_t packed[16];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            x[j] = (see >> j & 1u) != 0u ? exp2_approx(__fmaf_rn(x[j], c2, -shift)) : 0.0f;
+                            part[j & 3] += x[j];
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            packed[j] = pack_bf16x2(x[2 * j], x[2 * j + 1]);
+                        }
+                        tmem_store16(t_s + c * 16, packed);
+                    }
+                    sum += (part[0] + part[1]) + (part[2] + part[3]);
+                    tmem_store_wait();
+                }
+                if (partial) {  // V rows that nobody sees become zeros, values that are not finite are set aside
+                    const uint32_t fill = fill_of_v(at.fills, i, lead, count);
+                    wait(bar_full + fill % L::kSlots, (fill / L::kSlots) & 1u);
+                    unsigned char* v = sm + L::kRing + fill % L::kSlots * L::kSlot;
+                    const int sharing = kPair ? chains : 1;  // chains that read this tile
+                    for (int key = row * sharing + (kPair ? w % sharing : 0); key < kKeys; key += 128 * sharing) {
+                        const bool unseen = key0 + key >= r.kv_end;
+                        bool flag = false;
+                        for (int a = 0; a < L::kAtoms; ++a) {
+#pragma unroll
+                            for (int ch = 0; ch < 8; ++ch) {
+                                uint4* at16 =
+                                    reinterpret_cast<uint4*>(v + a * L::kKvAtom + key * 128 + ((ch ^ (key & 7)) << 4));
+                                const uint4 x = *at16;
+                                const uint4 y = make_uint4(finite_pair(x.x), finite_pair(x.y), finite_pair(x.z),
+                                                           finite_pair(x.w));
+                                const bool bad = x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w;
+                                if (unseen) {
+                                    *at16 = make_uint4(0u, 0u, 0u, 0u);
+                                } else if (bad) {
+                                    *at16 = y;
+                                    flag = true;
+                                }
+                            }
+                        }
+                        if (flag) {
+                            const int bit = key0 + key - part0;
+                            atomicOr(&s_flags[w * 16 + (bit >> 5)], 1u << (bit & 31));
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    if (kPair && sharing == 2) {
+                        named_barrier(3, 256);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(bar_p + w);
+                }
+            }
+            wait(bar_o + w, o_phase);
+            o_phase ^= 1u;
+            tc_fence_after();
+            // Values that are not finite, in rows that this row sees: added to O as they are.
+            uint32_t flagged = 0u;
+            if (hides) {
+                named_barrier(1 + w, 128);  // the flags of all the chain's threads
+                for (int i = 0; i < 32; ++i) {
+                    flagged |= kPair || (i >> 4) == w ? s_flags[i] : 0u;
+                }
+            }
+            const auto add_set_aside = [&](float (&o)[32], int d0) {
+                for (int i = 0; i < 32; ++i) {
+                    uint32_t word = kPair ? (i < 16 ? s_flags[i] | (chains > 1 ? s_flags[16 + i] : 0u) : 0u)
+                                          : (i < 16 ? s_flags[w * 16 + i] : 0u);
+                    while (word != 0u) {
+                        const int key = part0 + i * 32 + __ffs(word) - 1;
+                        word &= word - 1u;
+                        const bool sees_it = valid && (visible_bits(bits_row, key, r.len, limit) & 1u) != 0u;
+                        const bf16* v = p.v + at.b * p.vs[0] + key * p.vs[1] + at.h * p.vs[2] + d0;
+                        for (int j = 0; j < 32; ++j) {
+                            const float x = __bfloat162float(v[j]);
+                            if (sees_it && !(fabsf(x) < INFINITY)) {
+                                o[j] += x;
+                            }
+                        }
+                    }
+                }
+            };
+            float scaled_top = top == -INFINITY ? -INFINITY : top * c2;
+            const bool whole = at.tile == 0 && count == tiles;
+            const bool joins = !kPair && chains == 2;
+            const int64_t item_row = static_cast<int64_t>(kPair ? w * 128 : 0) + row;
+            const int64_t part = 2 * static_cast<int64_t>(blockIdx.x) + (at.index == 0 ? 0 : 1);
+            float f0 = 1.0f;
+            float f1 = 0.0f;
+            if (joins) {  // the two chains' sums: the second hands its maximum, sum and O to the first
+                if (w == 1) {
+                    s_ml[row] = make_float2(scaled_top, sum);
+                }
+                named_barrier(3, 256);
+                if (w == 0) {
+                    const float2 other = s_ml[row];
+                    const float most = fmaxf(scaled_top, other.x);
+                    f0 = scaled_top == -INFINITY ? 0.0f : exp2_approx(scaled_top - most);
+                    f1 = other.x == -INFINITY ? 0.0f : exp2_approx(other.x - most);
+                    sum = __fmaf_rn(other.y, f1, sum * f0);
+                    scaled_top = most;
+                }
+            }
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                float o[32];
+                if (busy) {
+                    tmem_load32(t_o + c * 32, o);
+                    if (flagged != 0u) {
+                        add_set_aside(o, c * 32);
+                        __syncwarp();
+                    }
+                }
+                if (joins) {
+                    if (w == 1 && busy) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            s_exchange[row * 33 + j] = o[j];
+                        }
+                    }
+                    named_barrier(3, 256);
+                    if (w == 0 && busy) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            o[j] = __fmaf_rn(s_exchange[row * 33 + j], f1, o[j] * f0);
+                        }
+                    }
+                    named_barrier(3, 256);
+                }
+                if (inside && whole && !(joins && w == 1)) {
+                    bf16* dst = p.ctx + ((at.b * p.tokens + t) * p.q_heads + at.h * p.group + g) * D + c * 32;
+                    const float scale = valid ? inv : 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t x[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            x[e] = valid ? pack_bf16x2(o[8 * j + 2 * e] * scale, o[8 * j + 2 * e + 1] * scale) : 0u;
+                        }
+                        st_v4(dst + 8 * j, make_uint4(x[0], x[1], x[2], x[3]));
+                    }
+                } else if (inside && !(joins && w == 1)) {
+                    float* dst = p.part_o + (part * p.part_rows + item_row) * D + c * 32;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        st_v4(dst + 4 * j,
+                              make_uint4(__float_as_uint(o[4 * j]), __float_as_uint(o[4 * j + 1]),
+                                         __float_as_uint(o[4 * j + 2]), __float_as_uint(o[4 * j + 3])));
+                    }
+                }
+                __syncwarp();  // the next tensor-memory load is warp-collective
+            }
+            if (inside && !(joins && w == 1)) {
+                if (!whole) {
+                    p.part_ml[part * p.part_rows + item_row] = make_float2(scaled_top, sum);
+                } else if (p.stats != nullptr) {
+                    p.stats[((at.b * p.kv_heads + at.h) * p.tokens + t) * p.group + g] =
+                        valid ? make_float2(scaled_top == -INFINITY ? 0.0f : scaled_top, inv) : make_float2(0.0f, 0.0f);
+                }
+            }
+            tc_fence_before();
+            if (kPair && chains == 2) {
+                named_barrier(3, 256);  // both chains are done with the flags
+            } else if (hides) {
+                named_barrier(1 + w, 128);
+            }
+            advance(p, at, count, tiles);
+        }
+    }
+    tc_fence_before();
+    __syncwarp();
+    __syncthreads();
+    if (warp == 2) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemAll);
+    }
+}
+
+// Joins the parts of the items that a cut of the line went through: block (c, i) takes rows from 256 / (D / 4) * i on
+// of the item that cut c + 1 is the first to go through. D / 4 threads a row, four columns each.
+template <int D, int kKeys>
+__global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAttentionParams p, int ctas) {
+    grid_dependency_begin();
+    const int cut = static_cast<int>(blockIdx.x) + 1;
+    const int64_t total = *p.line;
+    const auto begin_of = [&](int c) { return total * c / ctas; };
+    const int64_t begin = begin_of(cut);
+    if (begin >= total) {
+        return;
+    }
+    const int4 where = p.cuts[cut];
+    const int64_t first = begin - where.w;  // the item's first tile on the line
+    if (where.w == 0 || (cut > 1 && begin_of(cut - 1) > first)) {
+        return;
+    }
+    const ItemRange r = item_range(p, where.x, where.y);
+    const int64_t end = first + item_tiles<kKeys>(r);
+    constexpr int kLanes = D / 4;
+    const int row = static_cast<int>(blockIdx.y) * (256 / kLanes) + static_cast<int>(threadIdx.x) / kLanes;
+    const int d = static_cast<int>(threadIdx.x) % kLanes * 4;
+    const int tile = row >> 7;
+    const int token_in_tile = (row & 127) / p.group;
+    const int64_t t = r.first + tile * p.tile_tokens + token_in_tile;
+    if (row >= p.part_rows || token_in_tile >= p.tile_tokens || t >= p.tokens) {
+        return;
+    }
+    float top = -INFINITY;
+    float sum = 0.0f;
+    float o[4] = {};
+    for (int c = cut - 1; c < ctas && begin_of(c) < end; ++c) {
+        if (begin_of(c) == begin_of(c + 1)) {
+            continue;
+        }
+        const int64_t slot = 2 * static_cast<int64_t>(c) + (begin_of(c) >= first ? 0 : 1);
+        const float2 ml = p.part_ml[slot * p.part_rows + row];
+        const float4 x = *reinterpret_cast<const float4*>(p.part_o + (slot * p.part_rows + row) * D + d);
+        const float most = fmaxf(top, ml.x);
+        const float f0 = top == -INFINITY ? 0.0f : exp2_approx(top - most);
+        const float f1 = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - most);
+        top = most;
+        sum = __fmaf_rn(ml.y, f1, sum * f0);
+        o[0] = __fmaf_rn(x.x, f1, o[0] * f0);
+        o[1] = __fmaf_rn(x.y, f1, o[1] * f0);
+        o[2] = __fmaf_rn(x.z, f1, o[2] * f0);
+        o[3] = __fmaf_rn(x.w, f1, o[3] * f0);
+    }
+    const bool valid = t < r.valid;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int g = (row & 127) % p.group;
+    bf16* dst = p.ctx + ((where.x * p.tokens + t) * p.q_heads + where.z * p.group + g) * D + d;
+    *reinterpret_cast<uint2*>(dst) = valid ? make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv),
+                                                        pack_bf16x2(o[2] * inv, o[3] * inv))
+                                           : make_uint2(0u, 0u);
+    if (d == 0 && p.stats != nullptr) {
+        p.stats[((where.x * p.kv_heads + where.z) * p.tokens + t) * p.group + g] =
+            valid ? make_float2(top == -INFINITY ? 0.0f : top, inv) : make_float2(0.0f, 0.0f);
+    }
 }
 
 template <int kDims>
@@ -65,61 +830,6 @@ __device__ __forceinline__ void load_row(const bf16* row, int lane, float (&f)[k
 #pragma unroll
     for (int i = 0; i < kDims / 32; ++i) {
         f[i] = __bfloat162float(row[i * 32 + lane]);
-    }
-}
-
-template <int kDims>
-__global__ void __launch_bounds__(128) cache_attention_kernel(const CacheAttentionParams p) {
-    grid_dependency_begin();
-    const int lane = threadIdx.x & 31;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);  // (b, t, head)
-    if (row >= p.batch * p.tokens * p.q_heads) {
-        return;
-    }
-    const int64_t h = row % p.q_heads;
-    const int64_t t = row / p.q_heads % p.tokens;
-    const int64_t b = row / p.q_heads / p.tokens;
-    const int64_t kvh = h / (p.q_heads / p.kv_heads);
-    const int64_t len = committed_rows(p, b);
-    const int64_t n = valid_queries(p, b);
-    const float c = 1.4426950408889634f / sqrtf(static_cast<float>(kDims));
-    float q[kDims / 32];
-    float o[kDims / 32] = {};
-    load_row<kDims>(p.q + row * kDims, lane, q);
-    const bf16* k = p.k + b * p.ks[0] + kvh * p.ks[2];
-    const bf16* v = p.v + b * p.vs[0] + kvh * p.vs[2];
-    float top = -INFINITY;
-    float sum = 0.0f;
-    for (int64_t j = 0; t < n && j < len + n; ++j) {
-        if (j >= len && !sees(p, b, t, j - len)) {
-            continue;
-        }
-        float kf[kDims / 32];
-        load_row<kDims>(k + j * p.ks[1], lane, kf);
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kDims / 32; ++i) {
-            s = __fmaf_rn(q[i], kf[i], s);
-        }
-        s = group_sum<32>(s) * c;
-        const float m = fmaxf(top, s);
-        const float old = top == -INFINITY ? 0.0f : exp2f(top - m);
-        const float e = exp2f(s - m);
-        top = m;
-        sum = __fmaf_rn(sum, old, e);
-        load_row<kDims>(v + j * p.vs[1], lane, kf);
-#pragma unroll
-        for (int i = 0; i < kDims / 32; ++i) {
-            o[i] = __fmaf_rn(o[i], old, e * kf[i]);
-        }
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-    for (int i = 0; i < kDims / 32; ++i) {
-        p.ctx[row * kDims + i * 32 + lane] = __float2bfloat16(o[i] * inv);
-    }
-    if (p.stats != nullptr && lane == 0) {
-        p.stats[row] = make_float2(top == -INFINITY ? 0.0f : top, inv);
     }
 }
 
@@ -155,7 +865,7 @@ __global__ void __launch_bounds__(128) cache_weights_kernel(const CacheAttention
                 s = __fmaf_rn(q[i], kf[i], s);
             }
             s = group_sum<32>(s) * c;
-            const float2 st = p.stats[row];
+            const float2 st = p.stats[((b * p.kv_heads + kvh) * p.tokens + t) * group + g];
             sum = __fmaf_rn(exp2f(s - st.x), st.y, sum);
         }
     }
@@ -164,11 +874,91 @@ __global__ void __launch_bounds__(128) cache_weights_kernel(const CacheAttention
     }
 }
 
-template <int kDims>
-cudaError_t launch_cache_attention(const CacheAttentionParams& p, cudaStream_t s) {
-    const int64_t rows = p.batch * p.tokens * p.q_heads;
-    return runtime::launch(cache_attention_kernel<kDims>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), s, 1u,
-                           p);
+// The tiling of a call, and where its scratch lies (offsets in bytes; `bytes` in all).
+struct Plan {
+    bool pair;         // two row tiles on each K and V tile
+    int ctas;
+    int tile_tokens;
+    int item_tokens;
+    int row_tiles;
+    int part_rows;
+    int64_t cuts;
+    int64_t ml;
+    int64_t o;
+    int64_t stats;
+    int64_t bytes;
+};
+
+Plan plan(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t capacity,
+          bool with_stats) {
+    Plan pl{};
+    const int64_t group = q_heads / kv_heads;
+    const int64_t keys = head_dim == 256 ? 64 : 128;
+    pl.tile_tokens = static_cast<int>(kBM / group);
+    pl.pair = head_dim != 256 && tokens > pl.tile_tokens;
+    pl.item_tokens = pl.tile_tokens * (pl.pair ? 2 : 1);
+    pl.row_tiles = static_cast<int>(runtime::ceil_div(tokens, pl.item_tokens));
+    pl.part_rows = pl.pair ? 2 * kBM : static_cast<int>((tokens < pl.tile_tokens ? tokens : pl.tile_tokens) * group);
+    const int64_t most = batch * pl.row_tiles * kv_heads * runtime::ceil_div(capacity, keys);  // of the line's tiles
+    pl.ctas = static_cast<int>(most < runtime::sm_count() ? most : runtime::sm_count());
+    const auto up = [](int64_t n) { return (n + 127) / 128 * 128; };
+    pl.cuts = 128;  // after the line's length
+    pl.ml = pl.cuts + up(pl.ctas * static_cast<int64_t>(sizeof(int4)));
+    pl.o = pl.ml + up(2 * pl.ctas * pl.part_rows * static_cast<int64_t>(sizeof(float2)));
+    pl.stats = pl.o + 2 * pl.ctas * pl.part_rows * head_dim * static_cast<int64_t>(sizeof(float));
+    pl.bytes = pl.stats + (with_stats ? up(batch * tokens * q_heads * static_cast<int64_t>(sizeof(float2))) : 0);
+    return pl;
+}
+
+bool encode_4d(CUtensorMap* map, const void* base, const int64_t (&dims)[4], const int64_t (&strides)[3],
+               const int (&box)[4]) {
+    const EncodeTiled encode = encode_tiled();
+    if (encode == nullptr) {
+        return false;
+    }
+    cuuint64_t d[4];
+    cuuint64_t s[3];
+    cuuint32_t b[4];
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 4; ++i) {
+        d[i] = static_cast<cuuint64_t>(dims[i]);
+        b[i] = static_cast<cuuint32_t>(box[i]);
+    }
+    for (int i = 0; i < 3; ++i) {
+        s[i] = static_cast<cuuint64_t>(strides[i]) * 2;
+    }
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), d, s, b, ones,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool kPair>
+cudaError_t launch_cache_attention(const CacheAttentionParams& p, const Plan& pl, cudaStream_t s) {
+    using L = Tiling<D, kPair>;
+    CUtensorMap mq{};
+    CUtensorMap mk{};
+    CUtensorMap mv{};
+    if (!encode_4d(&mq, p.q, {D, p.q_heads, p.tokens, p.batch}, {D, p.q_heads * D, p.tokens * p.q_heads * D},
+                   {64, p.group, p.q_box_tokens, 1}) ||
+        !encode_4d(&mk, p.k, {D, p.kv_heads, p.capacity, p.batch}, {p.ks[2], p.ks[1], p.ks[0]}, {64, 1, L::kKeys, 1}) ||
+        !encode_4d(&mv, p.v, {D, p.kv_heads, p.capacity, p.batch}, {p.vs[2], p.vs[1], p.vs[0]}, {64, 1, L::kKeys, 1})) {
+        return cudaErrorInvalidValue;
+    }
+    cudaError_t err = cudaFuncSetAttribute(cache_attention_kernel<D, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           static_cast<int>(L::kBytes));
+    if (err != cudaSuccess) {
+        return err;
+    }
+    err = runtime::launch_smem(cache_attention_kernel<D, kPair>, dim3(static_cast<unsigned>(pl.ctas)),
+                               dim3(L::kThreads), L::kBytes, s, 1u, mq, mk, mv, p);
+    if (err != cudaSuccess || pl.ctas == 1) {
+        return err;
+    }
+    runtime::count_launches(1);
+    const unsigned rows = 256 / (D / 4);
+    return runtime::launch(cache_attention_join_kernel<D, L::kKeys>,
+                           dim3(static_cast<unsigned>(pl.ctas - 1), (static_cast<unsigned>(p.part_rows) + rows - 1) / rows),
+                           dim3(256), s, 1u, p, pl.ctas);
 }
 
 template <int kDims>
@@ -202,18 +992,47 @@ int check_cache(const char* op, const void* cache, const int64_t* strides) {
     const std::string name(op);
     CPPINF_REQUIRE(cache && strides, CPPINF_ERR_INVALID_ARGUMENT, name + " received a null pointer.");
     for (int i = 0; i < 3; ++i) {
-        CPPINF_REQUIRE(strides[i] >= 0, CPPINF_ERR_INVALID_ARGUMENT, name + " requires non-negative cache strides.");
-        CPPINF_REQUIRE(strides[i] % 8 == 0, CPPINF_ERR_UNSUPPORTED,
-                       name + " requires cache strides in multiples of 8 elements.");
+        CPPINF_REQUIRE(strides[i] > 0, CPPINF_ERR_INVALID_ARGUMENT, name + " requires positive cache strides.");
+        CPPINF_REQUIRE(strides[i] % 8 == 0 && strides[i] < (int64_t{1} << 38), CPPINF_ERR_UNSUPPORTED,
+                       name + " requires cache strides in multiples of 8 elements, below 2^38.");
     }
     CPPINF_REQUIRE(runtime::aligned16(cache), CPPINF_ERR_UNSUPPORTED, name + " requires 16-byte aligned caches.");
     return CPPINF_OK;
 }
 
-int run_attention(const char* op, const CacheAttentionParams& p, int64_t head_dim, cudaStream_t s) {
-    const cudaError_t err = head_dim == 64    ? launch_cache_attention<64>(p, s)
-                            : head_dim == 128 ? launch_cache_attention<128>(p, s)
-                                              : launch_cache_attention<256>(p, s);
+int run_attention(const char* op, CacheAttentionParams& p, int64_t head_dim, void* scratch, int64_t scratch_bytes,
+                  cudaStream_t s) {
+    const std::string name(op);
+    const Plan pl = plan(p.batch, p.tokens, p.q_heads, p.kv_heads, head_dim, p.capacity, p.weights != nullptr);
+    CPPINF_REQUIRE(scratch && scratch_bytes >= pl.bytes, CPPINF_ERR_INVALID_ARGUMENT,
+                   name + " requires a scratch of cppinf_cache_attention_scratch_bytes.");
+    CPPINF_REQUIRE(runtime::aligned16(scratch), CPPINF_ERR_UNSUPPORTED, name + " requires a 16-byte aligned scratch.");
+    char* base = static_cast<char*>(scratch);
+    p.group = static_cast<int>(p.q_heads / p.kv_heads);
+    p.tile_tokens = pl.tile_tokens;
+    p.item_tokens = pl.item_tokens;
+    p.row_tiles = pl.row_tiles;
+    p.q_box_tokens = static_cast<int>(p.tokens < pl.tile_tokens ? p.tokens : pl.tile_tokens);
+    p.part_rows = pl.part_rows;
+    p.line = reinterpret_cast<int64_t*>(base);
+    p.cuts = reinterpret_cast<int4*>(base + pl.cuts);
+    p.part_ml = reinterpret_cast<float2*>(base + pl.ml);
+    p.part_o = reinterpret_cast<float*>(base + pl.o);
+    p.stats = p.weights != nullptr ? reinterpret_cast<float2*>(base + pl.stats) : nullptr;
+    p.poll_limit = runtime::wait_poll_limit();
+    if (p.capacity == 0) {  // no rows: every query is padding
+        const auto bytes = static_cast<std::size_t>(p.batch * p.tokens * p.q_heads * head_dim) * sizeof(bf16);
+        CPPINF_CUDA_TRY(cudaMemsetAsync(p.ctx, 0, bytes, s));
+        return runtime::ok();
+    }
+    cudaError_t err = cudaSuccess;
+    if (head_dim == 64) {
+        err = pl.pair ? launch_cache_attention<64, true>(p, pl, s) : launch_cache_attention<64, false>(p, pl, s);
+    } else if (head_dim == 128) {
+        err = pl.pair ? launch_cache_attention<128, true>(p, pl, s) : launch_cache_attention<128, false>(p, pl, s);
+    } else {
+        err = launch_cache_attention<256, false>(p, pl, s);
+    }
     return runtime::launched(err, op);
 }
 
@@ -238,7 +1057,10 @@ int64_t cppinf_cache_attention_scratch_bytes(int64_t batch, int64_t tokens, int6
         CPPINF_OK) {
         return -1;
     }
-    return with_weights ? batch * tokens * q_heads * static_cast<int64_t>(sizeof(float2)) : 0;
+    if (batch == 0 || tokens == 0) {
+        return 0;
+    }
+    return plan(batch, tokens, q_heads, kv_heads, head_dim, capacity, with_weights != 0).bytes;
 }
 
 int cppinf_tree_attention(const void* q, const void* k_cache, const int64_t* k_strides, const void* v_cache,
@@ -247,9 +1069,6 @@ int cppinf_tree_attention(const void* q, const void* k_cache, const int64_t* k_s
                           int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t capacity, void* scratch,
                           int64_t scratch_bytes, unsigned int* error, void* stream) {
     constexpr const char* kOp = "tree_attention";
-    (void)scratch;
-    (void)scratch_bytes;
-    (void)error;
     if (const int st = check_sizes(kOp, batch, tokens, q_heads, kv_heads, head_dim, capacity); st != CPPINF_OK) {
         return st;
     }
@@ -287,7 +1106,8 @@ int cppinf_tree_attention(const void* q, const void* k_cache, const int64_t* k_s
     p.q_heads = q_heads;
     p.kv_heads = kv_heads;
     p.capacity = capacity;
-    return run_attention(kOp, p, head_dim, rt::as_stream(stream));
+    p.error = error;
+    return run_attention(kOp, p, head_dim, scratch, scratch_bytes, rt::as_stream(stream));
 }
 
 int cppinf_decoder_attention_weights(const void* q, const void* k_cache, const int64_t* k_strides, const void* v_cache,
@@ -296,7 +1116,6 @@ int cppinf_decoder_attention_weights(const void* q, const void* k_cache, const i
                                      int64_t head_dim, int64_t capacity, void* scratch, int64_t scratch_bytes,
                                      unsigned int* error, void* stream) {
     constexpr const char* kOp = "decoder_attention_weights";
-    (void)error;
     if (const int st = check_sizes(kOp, batch, tokens, q_heads, kv_heads, head_dim, capacity); st != CPPINF_OK) {
         return st;
     }
@@ -313,12 +1132,6 @@ int cppinf_decoder_attention_weights(const void* q, const void* k_cache, const i
     }
     CPPINF_REQUIRE(rt::aligned16(q) && rt::aligned16(ctx), CPPINF_ERR_UNSUPPORTED,
                    "decoder_attention_weights requires 16-byte aligned queries and contexts.");
-    const int64_t need =
-        cppinf_cache_attention_scratch_bytes(batch, tokens, q_heads, kv_heads, head_dim, capacity, 1);
-    CPPINF_REQUIRE(scratch_bytes >= need && (need == 0 || scratch), CPPINF_ERR_INVALID_ARGUMENT,
-                   "decoder_attention_weights requires a scratch of cppinf_cache_attention_scratch_bytes.");
-    CPPINF_REQUIRE(rt::aligned16(scratch), CPPINF_ERR_UNSUPPORTED,
-                   "decoder_attention_weights requires a 16-byte aligned scratch.");
     CacheAttentionParams p{};
     p.q = static_cast<const bf16*>(q);
     p.k = static_cast<const bf16*>(k_cache);
@@ -330,14 +1143,15 @@ int cppinf_decoder_attention_weights(const void* q, const void* k_cache, const i
     p.lengths = lengths;
     p.counts = counts;
     p.ctx = static_cast<bf16*>(ctx);
-    p.stats = static_cast<float2*>(scratch);
+    p.error = error;
     p.weights = weights;
     p.batch = batch;
     p.tokens = tokens;
     p.q_heads = q_heads;
     p.kv_heads = kv_heads;
     p.capacity = capacity;
-    if (const int st = run_attention(kOp, p, head_dim, rt::as_stream(stream)); st != CPPINF_OK) {
+    if (const int st = run_attention(kOp, p, head_dim, scratch, scratch_bytes, rt::as_stream(stream));
+        st != CPPINF_OK || capacity == 0) {
         return st;
     }
     return run_weights(kOp, p, head_dim, rt::as_stream(stream));

@@ -50,7 +50,7 @@ def weights(lib, batch=1, tokens=4, q_heads=4, kv_heads=2, d=64, capacity=16, q=
     (capi.ERR_UNSUPPORTED, "aligned", {"q": P + 8}),
     (capi.ERR_UNSUPPORTED, "aligned", {"k": P + 2}),
     (capi.ERR_UNSUPPORTED, "multiples of 8", {"ks": (2048, 132, 64)}),
-    (capi.ERR_INVALID_ARGUMENT, "non-negative cache strides", {"ks": (2048, -128, 64)}),
+    (capi.ERR_INVALID_ARGUMENT, "positive cache strides", {"ks": (2048, -128, 64)}),
 ])
 def test_attention_refusals(lib, call, status, message, change):
     assert call(lib, **change) == status
