@@ -71,6 +71,9 @@ struct CacheAttentionParams {
     int64_t* line;        // length of the line
     float2* part_ml;      // [2 CTAs][part_rows] (M in base 2, l)
     float* part_o;        // [2 CTAs][part_rows][D]
+    unsigned int* tickets;  // [weight CTAs] parts of a unit that have been left, zeroed by the attention kernel
+    float* part_sums;       // [2 weight CTAs][128]
+    int weight_ctas;
     unsigned int* error;
     uint32_t poll_limit;
 };
@@ -331,8 +334,13 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 break;
             }
         }
-        if (blockIdx.x == 0 && lane == 0) {
-            *p.line = total;
+        if (blockIdx.x == 0) {
+            if (lane == 0) {
+                *p.line = total;
+            }
+            for (int i = lane; i < p.weight_ctas; i += 32) {
+                p.tickets[i] = 0u;
+            }
         }
     }
     tc_fence_before();
@@ -825,52 +833,417 @@ __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAt
     }
 }
 
-template <int kDims>
-__device__ __forceinline__ void load_row(const bf16* row, int lane, float (&f)[kDims / 32]) {
-#pragma unroll
-    for (int i = 0; i < kDims / 32; ++i) {
-        f[i] = __bfloat162float(row[i * 32 + lane]);
+// ---- weights --------------------------------------------------------------------------------------------------------
+
+// The weight kernel's tiling: S^T = K Q^T, so that a thread owns a key (a row of the product) and adds its
+// probabilities over the queries in registers. A key tile of 128 rows is the A operand and stays in shared memory while
+// the sequence's query tiles that see any of it pass through a ring; two warpgroups take turns with the products, which
+// alternate between four tensor-memory buffers.
+template <int D>
+struct WeightTiling {
+    static constexpr int kAtoms = D / 64;
+    static constexpr int kKeySlots = D == 256 ? 1 : 2;
+    static constexpr int kSlots = D == 64 ? 8 : D == 128 ? 4 : 2;
+    static constexpr int kBuffers = 4;
+    static constexpr int kThreads = 384;
+    static constexpr uint32_t kAtom = 128 * 128;
+    static constexpr uint32_t kTile = kAtom * kAtoms;
+    static constexpr uint32_t kK = 0;
+    static constexpr uint32_t kRing = kK + kKeySlots * kTile;
+    static constexpr uint32_t kStats = kRing + kSlots * kTile;     // [groups][2][128] (-M, 1 / l)
+    static constexpr uint32_t kSum = kStats + 2 * 2 * 128 * 8;     // [128] the second group's sums
+    static constexpr uint32_t kBars = kSum + 128 * 4;
+    static constexpr std::size_t kBytes = 1024 + kBars + 256;
+    static_assert(kBytes <= 232448, "shared memory of a CTA");
+};
+
+// A sequence's key tiles: each has the query tiles from its first visible token's on.
+struct KeyRange {
+    int len;
+    int valid;
+    int q_tiles;    // query tiles of the sequence
+    int key_tiles;
+
+    __device__ __forceinline__ int first(int kt, int tile_tokens) const {  // the first query tile that sees key tile kt
+        const int past = kt * 128 - len;
+        return past > 0 ? past / tile_tokens : 0;
     }
+};
+
+__device__ __forceinline__ KeyRange key_range(const CacheAttentionParams& p, int64_t b) {
+    KeyRange r;
+    r.len = static_cast<int>(committed_rows(p, b));
+    r.valid = static_cast<int>(valid_queries(p, b));
+    r.q_tiles = (r.valid + p.tile_tokens - 1) / p.tile_tokens;
+    r.key_tiles = r.valid > 0 ? (r.len + r.valid + 127) / 128 : 0;
+    return r;
 }
 
-template <int kDims>
-__global__ void __launch_bounds__(128) cache_weights_kernel(const CacheAttentionParams p) {
-    grid_dependency_begin();
-    const int lane = threadIdx.x & 31;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);  // (b, kv head, cached row)
-    if (at >= p.batch * p.kv_heads * p.capacity) {
-        return;
+// Products of one head of a sequence: whole rows of query tiles for the key tiles that begin in committed rows.
+__device__ __forceinline__ int64_t head_products(const CacheAttentionParams& p, const KeyRange& r) {
+    if (r.valid == 0) {
+        return 0;
     }
-    const int64_t j = at % p.capacity;
-    const int64_t kvh = at / p.capacity % p.kv_heads;
-    const int64_t b = at / p.capacity / p.kv_heads;
-    const int64_t len = committed_rows(p, b);
-    const int64_t n = valid_queries(p, b);
-    if (j >= len + n) {
-        return;
+    int kt = r.len / 128 + 1;
+    kt = kt < r.key_tiles ? kt : r.key_tiles;
+    int64_t sum = int64_t{kt} * r.q_tiles;
+    for (; kt < r.key_tiles; ++kt) {
+        sum += r.q_tiles - r.first(kt, p.tile_tokens);
     }
-    const int64_t group = p.q_heads / p.kv_heads;
-    const float c = 1.4426950408889634f / sqrtf(static_cast<float>(kDims));
-    float kf[kDims / 32];
-    load_row<kDims>(p.k + b * p.ks[0] + j * p.ks[1] + kvh * p.ks[2], lane, kf);
-    float sum = 0.0f;
-    for (int64_t t = j < len ? 0 : j - len; t < n; ++t) {
-        for (int64_t g = 0; g < group; ++g) {
-            const int64_t row = (b * p.tokens + t) * p.q_heads + kvh * group + g;
-            float q[kDims / 32];
-            load_row<kDims>(p.q + row * kDims, lane, q);
-            float s = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kDims / 32; ++i) {
-                s = __fmaf_rn(q[i], kf[i], s);
-            }
-            s = group_sum<32>(s) * c;
-            const float2 st = p.stats[((b * p.kv_heads + kvh) * p.tokens + t) * group + g];
-            sum = __fmaf_rn(exp2f(s - st.x), st.y, sum);
+    return sum;
+}
+
+// The line of products is cut like the attention's; a unit is one key tile of one head.
+struct UnitWalk {
+    int b;
+    int kt;
+    int h;
+    int q;          // first query tile of the current segment, counted from the unit's first
+    int64_t left;
+    int64_t begin;  // the current segment's place on the line
+    int64_t total;
+    uint32_t products;  // before the current segment
+    int index;
+};
+
+template <int D>
+__global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
+    cache_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                         const CacheAttentionParams p) {
+    using L = WeightTiling<D>;
+    extern __shared__ __align__(16) unsigned char raw[];
+    unsigned char* sm = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
+    float2* s_stats = reinterpret_cast<float2*>(sm + L::kStats);
+    float* s_sum = reinterpret_cast<float*>(sm + L::kSum);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::kBars);
+    uint64_t* bar_full = bars;                    // [slots] a query tile has landed
+    uint64_t* bar_empty = bars + L::kSlots;
+    uint64_t* bar_k_full = bars + 2 * L::kSlots;  // [key slots]
+    uint64_t* bar_k_empty = bar_k_full + L::kKeySlots;
+    uint64_t* bar_s = bar_k_empty + L::kKeySlots;  // [buffers] a product is complete
+    uint64_t* bar_free = bar_s + L::kBuffers;      // [buffers] and read
+    __shared__ uint32_t s_tmem;
+    __shared__ uint32_t s_stop;
+    __shared__ uint32_t s_last[2];
+    __shared__ UnitWalk s_walk;
+
+    const int tid = threadIdx.x;
+    const int warp = tid >> 5;
+    const int lane = tid & 31;
+    const int columns = p.q_box_tokens * p.group;       // rows of a query tile, columns of the product
+    const int chunks = (columns + 31) / 32;
+    if (tid == 0) {
+        s_stop = 0u;
+        for (int i = 0; i < L::kSlots; ++i) {
+            mbar_init(bar_full + i, 1);
+            mbar_init(bar_empty + i, 1);
+        }
+        for (int i = 0; i < L::kKeySlots; ++i) {
+            mbar_init(bar_k_full + i, 1);
+            mbar_init(bar_k_empty + i, 1);
+        }
+        for (int i = 0; i < L::kBuffers; ++i) {
+            mbar_init(bar_s + i, 1);
+            mbar_init(bar_free + i, 4);
         }
     }
-    if (lane == 0) {
-        p.weights[at] += sum;
+    if (warp == 2) {
+        tmem_alloc(&s_tmem, kTmemAll);
+    }
+    // Rows of the query slots that no tile fills: zeros, so that their columns are finite and count for nothing.
+    for (int i = tid; i < L::kSlots * L::kAtoms * (128 - columns) * 8; i += L::kThreads) {
+        const int chunk = i & 7;
+        const int row = columns + (i >> 3) % (128 - columns);
+        const int atom = (i >> 3) / (128 - columns);
+        *reinterpret_cast<uint4*>(sm + L::kRing + atom * L::kAtom + row * 128 + chunk * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_proxy_async_smem();
+    grid_dependency_begin();
+    const auto begin_of = [&](int64_t total, int64_t c) { return total * c / gridDim.x; };
+    if (warp == 0) {
+        int64_t total = 0;
+        for (int64_t b = lane; b < p.batch; b += 32) {
+            total += head_products(p, key_range(p, b)) * p.kv_heads;
+        }
+        for (int offset = 16; offset > 0; offset >>= 1) {
+            total += __shfl_xor_sync(0xffffffffu, total, offset);
+        }
+        const int64_t begin = begin_of(total, blockIdx.x);
+        const int64_t end = begin_of(total, blockIdx.x + 1);
+        if (lane == 0) {
+            UnitWalk w{};
+            w.total = total;
+            s_walk = w;
+        }
+        __syncwarp();
+        int64_t before = 0;
+        for (int64_t b0 = 0; b0 < p.batch && begin < end; b0 += 32) {
+            const KeyRange r = b0 + lane < p.batch ? key_range(p, b0 + lane) : KeyRange{};
+            const int64_t mine = head_products(p, r) * p.kv_heads;
+            int64_t sum = mine;
+            for (int offset = 1; offset < 32; offset <<= 1) {
+                const int64_t other = __shfl_up_sync(0xffffffffu, sum, offset);
+                sum += lane >= offset ? other : 0;
+            }
+            const int64_t lo = before + sum - mine;
+            if (begin >= lo && begin < lo + mine) {
+                // Order within a sequence: key tile, head, query tile.
+                int64_t rest = begin - lo;
+                int kt = 0;
+                const int64_t whole = int64_t{r.q_tiles} * p.kv_heads;
+                int64_t skip = rest / whole;
+                const int64_t most = r.len / 128 < r.key_tiles - 1 ? r.len / 128 : r.key_tiles - 1;
+                skip = skip < most ? skip : most;
+                kt = static_cast<int>(skip);
+                rest -= skip * whole;
+                for (;;) {
+                    const int64_t here = (r.q_tiles - r.first(kt, p.tile_tokens)) * p.kv_heads;
+                    if (rest < here) {
+                        break;
+                    }
+                    rest -= here;
+                    ++kt;
+                }
+                const int each = r.q_tiles - r.first(kt, p.tile_tokens);
+                UnitWalk w;
+                w.b = static_cast<int>(b0 + lane);
+                w.kt = kt;
+                w.h = static_cast<int>(rest / each);
+                w.q = static_cast<int>(rest % each);
+                w.left = end - begin;
+                w.begin = begin;
+                w.total = total;
+                w.products = 0;
+                w.index = 0;
+                s_walk = w;
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
+            if (before > begin) {
+                break;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    const Waiter wait{p.error, p.poll_limit, &s_stop};
+    UnitWalk at = s_walk;
+    KeyRange r = at.left > 0 ? key_range(p, at.b) : KeyRange{};
+    const auto step = [&](int count, int tiles) {
+        at.left -= count;
+        at.begin += count;
+        at.products += static_cast<uint32_t>(count);
+        ++at.index;
+        at.q += count;
+        if (at.q < tiles) {
+            return;
+        }
+        at.q = 0;
+        if (++at.h < static_cast<int>(p.kv_heads)) {
+            return;
+        }
+        at.h = 0;
+        if (++at.kt < r.key_tiles) {
+            return;
+        }
+        at.kt = 0;
+        while (at.left > 0 && ++at.b < static_cast<int>(p.batch)) {
+            r = key_range(p, at.b);
+            if (r.key_tiles > 0) {
+                break;
+            }
+        }
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {  // ---- loads
+            while (at.left > 0) {
+                const int q0 = r.first(at.kt, p.tile_tokens);
+                const int tiles = r.q_tiles - q0;
+                const int count = static_cast<int>(tiles - at.q < at.left ? tiles - at.q : at.left);
+                const uint32_t ks = static_cast<uint32_t>(at.index) % L::kKeySlots;
+                const uint32_t kr = static_cast<uint32_t>(at.index) / L::kKeySlots;
+                if (kr > 0) {
+                    wait(bar_k_empty + ks, (kr - 1) & 1u);
+                }
+                mbar_arrive_expect_tx(bar_k_full + ks, L::kTile);
+                for (int a = 0; a < L::kAtoms; ++a) {
+                    tma_load_4d(sm + L::kK + ks * L::kTile + a * L::kAtom, &map_k, a * 64, at.h, at.kt * 128, at.b,
+                                bar_k_full + ks);
+                }
+                for (int i = 0; i < count; ++i) {
+                    const uint32_t fill = at.products + static_cast<uint32_t>(i);
+                    const uint32_t slot = fill % L::kSlots;
+                    if (fill >= static_cast<uint32_t>(L::kSlots)) {
+                        wait(bar_empty + slot, (fill / L::kSlots - 1) & 1u);
+                    }
+                    mbar_arrive_expect_tx(bar_full + slot, static_cast<uint32_t>(columns) * 128u * L::kAtoms);
+                    for (int a = 0; a < L::kAtoms; ++a) {
+                        tma_load_4d(sm + L::kRing + slot * L::kTile + a * L::kAtom, &map_q, a * 64, at.h * p.group,
+                                    (q0 + at.q + i) * p.tile_tokens, at.b, bar_full + slot);
+                    }
+                }
+                step(count, tiles);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {  // ---- matrix products
+            const uint32_t idesc = idesc_bf16_f32(chunks * 32);
+            while (at.left > 0) {
+                const int tiles = r.q_tiles - r.first(at.kt, p.tile_tokens);
+                const int count = static_cast<int>(tiles - at.q < at.left ? tiles - at.q : at.left);
+                const uint32_t ks = static_cast<uint32_t>(at.index) % L::kKeySlots;
+                wait(bar_k_full + ks, static_cast<uint32_t>(at.index) / L::kKeySlots & 1u);
+                for (int i = 0; i < count; ++i) {
+                    const uint32_t n = at.products + static_cast<uint32_t>(i);
+                    const uint32_t slot = n % L::kSlots;
+                    const uint32_t buffer = n % L::kBuffers;
+                    if (n >= static_cast<uint32_t>(L::kBuffers)) {
+                        wait(bar_free + buffer, (n / L::kBuffers - 1) & 1u);
+                    }
+                    wait(bar_full + slot, n / L::kSlots & 1u);
+                    tc_fence_after();
+                    const unsigned char* k = sm + L::kK + ks * L::kTile;
+                    const unsigned char* q = sm + L::kRing + slot * L::kTile;
+#pragma unroll
+                    for (int j = 0; j < D / kUmmaK; ++j) {
+                        const uint32_t off = (j >> 2) * L::kAtom + static_cast<uint32_t>(j & 3) * 32u;
+                        umma_bf16(tmem + buffer * 128, smem_desc_sw128(k, off), smem_desc_sw128(q, off), idesc,
+                                  j > 0 ? 1u : 0u);
+                    }
+                    umma_commit(bar_s + buffer);
+                    umma_commit(bar_empty + slot);
+                }
+                umma_commit(bar_k_empty + ks);
+                step(count, tiles);
+            }
+        }
+    } else if (warp >= 4) {  // ---- probabilities: one thread per key, the products in turn with the other group
+        const int w = (warp - 4) >> 2;
+        const int row = tid & 127;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const float c2 = 1.4426950408889634f / sqrtf(static_cast<float>(D));
+        uint32_t turn = 0;  // which of the group's two copies of the statistics
+        while (at.left > 0) {
+            const int q0 = r.first(at.kt, p.tile_tokens);
+            const int tiles = r.q_tiles - q0;
+            const int count = static_cast<int>(tiles - at.q < at.left ? tiles - at.q : at.left);
+            const int key = at.kt * 128 + row;
+            float part[4] = {};
+            bool mine = false;
+            for (int i = 0; i < count; ++i) {
+                const uint32_t n = at.products + static_cast<uint32_t>(i);
+                if ((n & 1u) != static_cast<uint32_t>(w)) {
+                    continue;
+                }
+                mine = true;
+                const uint32_t buffer = n % L::kBuffers;
+                const int token0 = (q0 + at.q + i) * p.tile_tokens;
+                const int inside = r.valid - token0 < p.tile_tokens ? r.valid - token0 : p.tile_tokens;
+                const int high = inside * p.group;  // columns from here on count for nothing
+                float2 st = make_float2(0.0f, 0.0f);
+                if (row < high) {
+                    st = p.stats[((at.b * p.kv_heads + at.h) * p.tokens + token0) * p.group + row];
+                }
+                float2* stats = s_stats + (w * 2 + turn) * 128;
+                turn ^= 1u;
+                stats[row] = make_float2(-st.x, st.y);
+                named_barrier(1 + w, 128);
+                wait(bar_s + buffer, n / L::kBuffers & 1u);
+                tc_fence_after();
+                const bool partial = inside < p.tile_tokens || at.kt * 128 + 127 - r.len > token0;
+                const int low = (key - r.len - token0) * p.group;  // columns below do not see the key
+#pragma unroll 1
+                for (int c = 0; c < chunks; ++c) {
+                    float x[32];
+                    tmem_load32(tmem + lanes + buffer * 128 + c * 32, x);
+                    if (!partial) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const float2 s = stats[c * 32 + j];
+                            part[j & 3] = __fmaf_rn(exp2_approx(__fmaf_rn(x[j], c2, s.x)), s.y, part[j & 3]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const int column = c * 32 + j;
+                            const float2 s = stats[column];
+                            const float e = exp2_approx(__fmaf_rn(x[j], c2, s.x)) * s.y;
+                            part[j & 3] += column >= low && column < high ? e : 0.0f;
+                        }
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(bar_free + buffer);
+                }
+            }
+            float sum = (part[0] + part[1]) + (part[2] + part[3]);
+            bool writes = mine;
+            if (count > 1) {  // both groups had products of the unit: the second hands its sums to the first
+                if (w == 1) {
+                    s_sum[row] = sum;
+                }
+                named_barrier(3, 256);
+                sum = w == 0 ? sum + s_sum[row] : sum;
+                writes = w == 0;
+                named_barrier(3, 256);
+            }
+            if (writes) {
+                const bool seen = key < r.len + r.valid;
+                float* out = p.weights + (at.b * p.kv_heads + at.h) * p.capacity + key;
+                if (count == tiles) {
+                    if (seen) {
+                        *out += sum;
+                    }
+                } else {
+                    // A cut went through the unit: whoever leaves the last of its parts adds them up in their order.
+                    const int64_t first = at.begin - at.q;
+                    const int64_t end = first + tiles;
+                    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (at.index == 0 ? 0 : 1);
+                    p.part_sums[slot * 128 + row] = sum;
+                    int64_t c0 = first * gridDim.x / at.total;  // the part of the line that `first` lies in
+                    while (begin_of(at.total, c0) > first) {
+                        --c0;
+                    }
+                    while (begin_of(at.total, c0 + 1) <= first) {
+                        ++c0;
+                    }
+                    uint32_t parts = 0;
+                    for (int64_t c = c0; c < gridDim.x && begin_of(at.total, c) < end; ++c) {
+                        parts += begin_of(at.total, c) < begin_of(at.total, c + 1) ? 1u : 0u;
+                    }
+                    __threadfence();
+                    named_barrier(1 + w, 128);
+                    if (row == 0) {
+                        s_last[w] = atomicAdd(p.tickets + c0, 1u) == parts - 1u ? 1u : 0u;
+                    }
+                    named_barrier(1 + w, 128);
+                    if (s_last[w] != 0u) {
+                        __threadfence();
+                        float all = 0.0f;
+                        for (int64_t c = c0; c < gridDim.x && begin_of(at.total, c) < end; ++c) {
+                            if (begin_of(at.total, c) < begin_of(at.total, c + 1)) {
+                                all += __ldcg(p.part_sums + (2 * c + (begin_of(at.total, c) >= first ? 0 : 1)) * 128 + row);
+                            }
+                        }
+                        if (seen) {
+                            *out += all;
+                        }
+                    }
+                }
+            }
+            step(count, tiles);
+        }
+    }
+    tc_fence_before();
+    __syncwarp();
+    __syncthreads();
+    if (warp == 2) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemAll);
     }
 }
 
@@ -886,7 +1259,9 @@ struct Plan {
     int64_t ml;
     int64_t o;
     int64_t stats;
+    int64_t sums;
     int64_t bytes;
+    int weight_ctas;
 };
 
 Plan plan(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t capacity,
@@ -906,7 +1281,14 @@ Plan plan(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads, int6
     pl.ml = pl.cuts + up(pl.ctas * static_cast<int64_t>(sizeof(int4)));
     pl.o = pl.ml + up(2 * pl.ctas * pl.part_rows * static_cast<int64_t>(sizeof(float2)));
     pl.stats = pl.o + 2 * pl.ctas * pl.part_rows * head_dim * static_cast<int64_t>(sizeof(float));
-    pl.bytes = pl.stats + (with_stats ? up(batch * tokens * q_heads * static_cast<int64_t>(sizeof(float2))) : 0);
+    pl.bytes = pl.stats;
+    if (with_stats) {
+        const int64_t products = batch * kv_heads * runtime::ceil_div(capacity, 128) * runtime::ceil_div(tokens, pl.tile_tokens);
+        pl.weight_ctas = static_cast<int>(products < runtime::sm_count() ? products : runtime::sm_count());
+        pl.sums = pl.stats + up(batch * tokens * q_heads * static_cast<int64_t>(sizeof(float2)));
+        // The parts of the units, then the tickets.
+        pl.bytes = pl.sums + up(pl.weight_ctas * static_cast<int64_t>(2 * 128 * sizeof(float) + sizeof(unsigned int)));
+    }
     return pl;
 }
 
@@ -961,10 +1343,23 @@ cudaError_t launch_cache_attention(const CacheAttentionParams& p, const Plan& pl
                            dim3(256), s, 1u, p, pl.ctas);
 }
 
-template <int kDims>
+template <int D>
 cudaError_t launch_cache_weights(const CacheAttentionParams& p, cudaStream_t s) {
-    const int64_t rows = p.batch * p.kv_heads * p.capacity;
-    return runtime::launch(cache_weights_kernel<kDims>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), s, 1u, p);
+    using L = WeightTiling<D>;
+    CUtensorMap mq{};
+    CUtensorMap mk{};
+    if (!encode_4d(&mq, p.q, {D, p.q_heads, p.tokens, p.batch}, {D, p.q_heads * D, p.tokens * p.q_heads * D},
+                   {64, p.group, p.q_box_tokens, 1}) ||
+        !encode_4d(&mk, p.k, {D, p.kv_heads, p.capacity, p.batch}, {p.ks[2], p.ks[1], p.ks[0]}, {64, 1, 128, 1})) {
+        return cudaErrorInvalidValue;
+    }
+    const cudaError_t err = cudaFuncSetAttribute(cache_weights_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 static_cast<int>(L::kBytes));
+    if (err != cudaSuccess) {
+        return err;
+    }
+    return runtime::launch_smem(cache_weights_kernel<D>, dim3(static_cast<unsigned>(p.weight_ctas)), dim3(L::kThreads),
+                                L::kBytes, s, 1u, mq, mk, p);
 }
 
 int check_sizes(const char* op, int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,
@@ -1018,7 +1413,12 @@ int run_attention(const char* op, CacheAttentionParams& p, int64_t head_dim, voi
     p.cuts = reinterpret_cast<int4*>(base + pl.cuts);
     p.part_ml = reinterpret_cast<float2*>(base + pl.ml);
     p.part_o = reinterpret_cast<float*>(base + pl.o);
-    p.stats = p.weights != nullptr ? reinterpret_cast<float2*>(base + pl.stats) : nullptr;
+    if (p.weights != nullptr) {
+        p.stats = reinterpret_cast<float2*>(base + pl.stats);
+        p.weight_ctas = pl.weight_ctas;
+        p.part_sums = reinterpret_cast<float*>(base + pl.sums);
+        p.tickets = reinterpret_cast<unsigned int*>(p.part_sums + pl.weight_ctas * 2 * 128);
+    }
     p.poll_limit = runtime::wait_poll_limit();
     if (p.capacity == 0) {  // no rows: every query is padding
         const auto bytes = static_cast<std::size_t>(p.batch * p.tokens * p.q_heads * head_dim) * sizeof(bf16);
