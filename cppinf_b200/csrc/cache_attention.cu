@@ -70,7 +70,7 @@ struct CacheAttentionParams {
     int4* cuts;           // [CTAs] where each CTA's part of the line begins: sequence, row tile, head, key tile
     int64_t* line;        // length of the line
     float2* part_ml;      // [2 CTAs][part_rows] (M in base 2, l)
-    float* part_o;        // [2 CTAs][part_rows][D]
+    float* part_o;        // [2 CTAs][D / 4][part_rows][4]
     unsigned int* tickets;  // [weight CTAs] parts of a unit that have been left, zeroed by the attention kernel
     float* part_sums;       // [2 weight CTAs][128]
     int weight_ctas;
@@ -145,7 +145,8 @@ struct Tiling {
     static constexpr uint32_t kMask = kExchange + (kStreams == 2 && !kPair ? 128 * 33 * 4 : 0);  // [chains][128][9]
     static constexpr uint32_t kMl = kMask + kStreams * 128 * 9 * 4;
     static constexpr uint32_t kFlags = kMl + 128 * 8;
-    static constexpr uint32_t kBars = kFlags + 2 * 16 * 4;
+    static constexpr uint32_t kStage = kFlags + 2 * 16 * 4;  // a warp's context rows, [32][64 bytes]
+    static constexpr uint32_t kBars = kStage + kStreams * 4 * 2048;
     static constexpr std::size_t kBytes = 1024 + kBars + 256;
     // Tensor memory columns: the chains' S (P over it), then their O.
     static constexpr uint32_t kTmemO = kStreams * kKeys;
@@ -194,6 +195,20 @@ __device__ __forceinline__ uint32_t fill_of_v(uint32_t fills, int i, int ahead, 
     return fills + static_cast<uint32_t>(lead + i + k);
 }
 
+// A line of `total` pieces cut into `parts` that differ by one piece at most.
+struct Cuts {
+    int64_t each;
+    int64_t extra;  // the first `extra` parts have one more
+
+    __device__ __forceinline__ Cuts(int64_t total, unsigned parts) : each(total / parts), extra(total - each * parts) {}
+    __device__ __forceinline__ int64_t begin(int64_t part) const { return part * each + (part < extra ? part : extra); }
+    __device__ __forceinline__ bool empty(int64_t part) const { return each == 0 && part >= extra; }
+    __device__ __forceinline__ int64_t of(int64_t piece) const {  // the part that a piece lies in
+        const int64_t longer = extra * (each + 1);
+        return piece < longer ? piece / (each + 1) : extra + (piece - longer) / each;
+    }
+};
+
 // Bounded waits: one that runs out of the poll limit sets the error word and waits again with the default limit; if
 // that runs out too, `stop` ends all later waits of the CTA at once, so that it always comes to its end.
 struct Waiter {
@@ -239,6 +254,13 @@ __device__ __forceinline__ uint32_t visible_bits(const uint32_t* row, int key, i
 __device__ __forceinline__ uint32_t finite_pair(uint32_t pair) {
     return ((pair & 0x7f80u) == 0x7f80u ? 0u : pair & 0xffffu) |
            ((pair & 0x7f800000u) == 0x7f800000u ? 0u : pair & 0xffff0000u);
+}
+
+// acc + 0 * x for both values of a pair.
+__device__ __forceinline__ uint32_t zero_times(uint32_t pair, uint32_t acc) {
+    uint32_t d;
+    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(pair), "r"(0u), "r"(acc));
+    return d;
 }
 
 template <int D, bool kPair>
@@ -304,8 +326,13 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
         for (int offset = 16; offset > 0; offset >>= 1) {
             total += __shfl_xor_sync(0xffffffffu, total, offset);
         }
-        const int64_t begin = total * blockIdx.x / gridDim.x;
-        const int64_t end = total * (blockIdx.x + 1) / gridDim.x;
+        const Cuts cuts(total, gridDim.x);
+        const int64_t begin = cuts.begin(blockIdx.x);
+        const int64_t end = cuts.begin(blockIdx.x + 1);
+        if (lane == 0) {
+            s_walk = Walk{};  // a part of the line may be empty
+        }
+        __syncwarp();
         int64_t before = 0;
         for (int64_t e0 = 0; e0 < entries; e0 += 32) {
             const int64_t mine = tiles_at(e0 + lane);
@@ -353,7 +380,12 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
     const auto chains_of = [&](const ItemRange& r, int count) {
         return kStreams == 1 ? 1 : kPair ? (r.first + p.tile_tokens < p.tokens ? 2 : 1) : (count < 2 ? count : 2);
     };
-
+    // A row of S takes 128 registers: with two chains the control warps give up what they do not need of the 168
+    // registers a thread that 384 threads start with (128 * 88 + 256 * 208 = 384 * 168).
+    if (warp < 4) {
+        if constexpr (kStreams == 2) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        }
     if (warp == 0) {
         if (lane == 0) {  // ---- loads
             uint32_t fill = 0;
@@ -483,7 +515,11 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 advance(p, at, count, tiles);
             }
         }
-    } else if (warp >= 4) {  // ---- softmax: chain w, one thread per row
+        }
+    } else {  // ---- softmax: chain w, one thread per row
+        if constexpr (kStreams == 2) {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        }
         const int w = (warp - 4) >> 2;
         const int row = tid & 127;
         const int g = row % p.group;
@@ -552,18 +588,24 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 s_phase ^= 1u;
                 tc_fence_after();
                 if (busy) {
-                    float tile_top = -INFINITY;
-#pragma unroll 1
-                    for (int c = 0; c < kKeys / 32; ++c) {
-                        float x[32];
-                        tmem_load32(t_s + c * 32, x);
-                        const uint32_t see =
-                            partial ? visible_bits(bits_row, key0 + c * 32, r.len, limit) : 0xffffffffu;
+                    float x[kKeys];
+                    tmem_load_row<kKeys>(t_s, x);
+                    if (partial) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            tile_top = fmaxf(tile_top, (see >> j & 1u) != 0u ? x[j] : -INFINITY);
+                        for (int c = 0; c < kKeys / 32; ++c) {
+                            const uint32_t see = visible_bits(bits_row, key0 + c * 32, r.len, limit);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                x[c * 32 + j] = (see >> j & 1u) != 0u ? x[c * 32 + j] : -INFINITY;
+                            }
                         }
                     }
+                    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int j = 0; j < kKeys / 2; ++j) {
+                        tops[j & 3] = max3(tops[j & 3], x[2 * j], x[2 * j + 1]);
+                    }
+                    const float tile_top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                     const float new_top = fmaxf(top, tile_top);
                     const bool first = i < kStreams && (!kPair || i == 0);
                     const bool grown = first || (new_top - top) * c2 > 8.0f;
@@ -583,26 +625,23 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                     }
                     top = grown ? new_top : top;
                     const float shift = top == -INFINITY ? 0.0f : top * c2;
-                    float part[4] = {};
-#pragma unroll 1
+                    const float2 factor = make_float2(c2, c2);
+                    const float2 offset = make_float2(-shift, -shift);
+                    float2 sums[2] = {};
+#pragma unroll
                     for (int c = 0; c < kKeys / 32; ++c) {
-                        float x[32];
-                        tmem_load32(t_s + c * 32, x);
-                        const uint32_t see =
-                            partial ? visible_bits(bits_row, key0 + c * 32, r.len, limit) : 0xffffffffu;
                         uint32_t packed[16];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            x[j] = (see >> j & 1u) != 0u ? exp2_approx(__fmaf_rn(x[j], c2, -shift)) : 0.0f;
-                            part[j & 3] += x[j];
-                        }
-#pragma unroll
                         for (int j = 0; j < 16; ++j) {
-                            packed[j] = pack_bf16x2(x[2 * j], x[2 * j + 1]);
+                            const int k = c * 32 + 2 * j;
+                            float2 e = __ffma2_rn(make_float2(x[k], x[k + 1]), factor, offset);
+                            e = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+                            sums[j & 1] = __fadd2_rn(sums[j & 1], e);
+                            packed[j] = pack_bf16x2(e.x, e.y);
                         }
                         tmem_store16(t_s + c * 16, packed);
                     }
-                    sum += (part[0] + part[1]) + (part[2] + part[3]);
+                    sum += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
                     tmem_store_wait();
                 }
                 if (partial) {  // V rows that nobody sees become zeros, values that are not finite are set aside
@@ -610,27 +649,28 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                     wait(bar_full + fill % L::kSlots, (fill / L::kSlots) & 1u);
                     unsigned char* v = sm + L::kRing + fill % L::kSlots * L::kSlot;
                     const int sharing = kPair ? chains : 1;  // chains that read this tile
-                    for (int key = row * sharing + (kPair ? w % sharing : 0); key < kKeys; key += 128 * sharing) {
-                        const bool unseen = key0 + key >= r.kv_end;
-                        bool flag = false;
-                        for (int a = 0; a < L::kAtoms; ++a) {
+                    for (int u = (sharing == 2 ? w * 128 : 0) + row; u < kKeys * L::kAtoms; u += 128 * sharing) {
+                        const int key = u % kKeys;  // this thread's: 64 dims of a row
+                        uint4* at16 = reinterpret_cast<uint4*>(v + u / kKeys * L::kKvAtom + key * 128);
+                        if (key0 + key >= r.kv_end) {
 #pragma unroll
                             for (int ch = 0; ch < 8; ++ch) {
-                                uint4* at16 =
-                                    reinterpret_cast<uint4*>(v + a * L::kKvAtom + key * 128 + ((ch ^ (key & 7)) << 4));
-                                const uint4 x = *at16;
-                                const uint4 y = make_uint4(finite_pair(x.x), finite_pair(x.y), finite_pair(x.z),
-                                                           finite_pair(x.w));
-                                const bool bad = x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w;
-                                if (unseen) {
-                                    *at16 = make_uint4(0u, 0u, 0u, 0u);
-                                } else if (bad) {
-                                    *at16 = y;
-                                    flag = true;
-                                }
+                                at16[ch ^ (key & 7)] = make_uint4(0u, 0u, 0u, 0u);
                             }
+                            continue;
                         }
-                        if (flag) {
+                        uint32_t bad = 0u;  // sum of 0 * x: not zero where some x is not finite
+#pragma unroll
+                        for (int ch = 0; ch < 8; ++ch) {
+                            const uint4 x = at16[ch ^ (key & 7)];
+                            bad = zero_times(x.x, zero_times(x.y, zero_times(x.z, zero_times(x.w, bad))));
+                        }
+                        if ((bad & 0x7fff7fffu) != 0u) {
+                            for (int ch = 0; ch < 8; ++ch) {
+                                const uint4 x = at16[ch];
+                                at16[ch] = make_uint4(finite_pair(x.x), finite_pair(x.y), finite_pair(x.z),
+                                                      finite_pair(x.w));
+                            }
                             const int bit = key0 + key - part0;
                             atomicOr(&s_flags[w * 16 + (bit >> 5)], 1u << (bit & 31));
                         }
@@ -697,6 +737,14 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 }
             }
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            uint4* stage = reinterpret_cast<uint4*>(sm + L::kStage) + (warp - 4) * 128;
+            // Where the four rows that this lane writes a piece of lie in ctx.
+            const int64_t place = inside ? ((at.b * p.tokens + t) * p.q_heads + at.h * p.group + g) * D : -1;
+            int64_t places[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                places[i] = __shfl_sync(0xffffffffu, place, i * 8 + (lane >> 2));
+            }
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
                 float o[32];
@@ -723,8 +771,8 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                     }
                     named_barrier(3, 256);
                 }
-                if (inside && whole && !(joins && w == 1)) {
-                    bf16* dst = p.ctx + ((at.b * p.tokens + t) * p.q_heads + at.h * p.group + g) * D + c * 32;
+                if (whole && !(joins && w == 1) && busy) {
+                    // The warp's 32 rows of 64 bytes change hands in shared memory, so that four lanes write a row.
                     const float scale = valid ? inv : 0.0f;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -733,13 +781,22 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                         for (int e = 0; e < 4; ++e) {
                             x[e] = valid ? pack_bf16x2(o[8 * j + 2 * e] * scale, o[8 * j + 2 * e + 1] * scale) : 0u;
                         }
-                        st_v4(dst + 8 * j, make_uint4(x[0], x[1], x[2], x[3]));
+                        stage[lane * 4 + (j ^ (lane >> 1 & 3))] = make_uint4(x[0], x[1], x[2], x[3]);
                     }
-                } else if (inside && !(joins && w == 1)) {
-                    float* dst = p.part_o + (part * p.part_rows + item_row) * D + c * 32;
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int from = i * 8 + (lane >> 2);
+                        const uint4 x = stage[from * 4 + ((lane & 3) ^ (from >> 1 & 3))];
+                        if (places[i] >= 0) {
+                            st_v4(p.ctx + places[i] + c * 32 + (lane & 3) * 8, x);
+                        }
+                    }
+                } else if (!whole && inside && !(joins && w == 1)) {
+                    float* dst = p.part_o + (part * D + c * 32) * p.part_rows + item_row * 4;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        st_v4(dst + 4 * j,
+                        st_v4(dst + 4 * j * p.part_rows,
                               make_uint4(__float_as_uint(o[4 * j]), __float_as_uint(o[4 * j + 1]),
                                          __float_as_uint(o[4 * j + 2]), __float_as_uint(o[4 * j + 3])));
                     }
@@ -772,64 +829,81 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
     }
 }
 
-// Joins the parts of the items that a cut of the line went through: block (c, i) takes rows from 256 / (D / 4) * i on
-// of the item that cut c + 1 is the first to go through. D / 4 threads a row, four columns each.
+// Joins the parts of the items that a cut of the line went through: block (c, i) takes rows 32 i to 32 i + 31 of the
+// item that cut c + 1 is the first to go through, a lane a row, the columns over the warps.
 template <int D, int kKeys>
 __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAttentionParams p, int ctas) {
+    constexpr int kPieces = D / 32;  // of four columns, for each thread
+    __shared__ uint2 s_rows[32][D / 4 + 1];
+    __shared__ int64_t s_places[32];
     grid_dependency_begin();
     const int cut = static_cast<int>(blockIdx.x) + 1;
     const int64_t total = *p.line;
-    const auto begin_of = [&](int c) { return total * c / ctas; };
-    const int64_t begin = begin_of(cut);
-    if (begin >= total) {
-        return;
-    }
     const int4 where = p.cuts[cut];
+    const Cuts cuts(total, static_cast<unsigned>(ctas));
+    const int64_t begin = cuts.begin(cut);
     const int64_t first = begin - where.w;  // the item's first tile on the line
-    if (where.w == 0 || (cut > 1 && begin_of(cut - 1) > first)) {
+    if (cuts.empty(cut) || where.w == 0 || cuts.begin(cut - 1) > first) {
         return;
     }
     const ItemRange r = item_range(p, where.x, where.y);
-    const int64_t end = first + item_tiles<kKeys>(r);
-    constexpr int kLanes = D / 4;
-    const int row = static_cast<int>(blockIdx.y) * (256 / kLanes) + static_cast<int>(threadIdx.x) / kLanes;
-    const int d = static_cast<int>(threadIdx.x) % kLanes * 4;
-    const int tile = row >> 7;
-    const int token_in_tile = (row & 127) / p.group;
-    const int64_t t = r.first + tile * p.tile_tokens + token_in_tile;
-    if (row >= p.part_rows || token_in_tile >= p.tile_tokens || t >= p.tokens) {
-        return;
-    }
+    const int64_t last = cuts.of(first + item_tiles<kKeys>(r) - 1);  // parts before it are not empty
+    const int lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5;
+    const int row = static_cast<int>(blockIdx.y) * 32 + lane;
+    const int in_tile = row & 127;
+    const int64_t t = r.first + (row >> 7) * p.tile_tokens + in_tile / p.group;
+    const int g = in_tile % p.group;
+    const bool inside = row < p.part_rows && in_tile / p.group < p.tile_tokens && t < p.tokens;
+    const bool valid = inside && t < r.valid;
     float top = -INFINITY;
     float sum = 0.0f;
-    float o[4] = {};
-    for (int c = cut - 1; c < ctas && begin_of(c) < end; ++c) {
-        if (begin_of(c) == begin_of(c + 1)) {
-            continue;
+    float o[kPieces][4] = {};
+    if (inside) {
+#pragma unroll 2
+        for (int64_t c = cut - 1; c <= last; ++c) {
+            const int64_t slot = 2 * c + (cuts.begin(c) >= first ? 0 : 1);
+            const float2 ml = p.part_ml[slot * p.part_rows + row];
+            float4 x[kPieces];
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                x[i] = reinterpret_cast<const float4*>(p.part_o)[(slot * (D / 4) + warp * kPieces + i) * p.part_rows +
+                                                                 row];
+            }
+            const float most = fmaxf(top, ml.x);
+            const float f0 = top == -INFINITY ? 0.0f : exp2_approx(top - most);
+            const float f1 = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - most);
+            top = most;
+            sum = __fmaf_rn(ml.y, f1, sum * f0);
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i) {
+                o[i][0] = __fmaf_rn(x[i].x, f1, o[i][0] * f0);
+                o[i][1] = __fmaf_rn(x[i].y, f1, o[i][1] * f0);
+                o[i][2] = __fmaf_rn(x[i].z, f1, o[i][2] * f0);
+                o[i][3] = __fmaf_rn(x[i].w, f1, o[i][3] * f0);
+            }
         }
-        const int64_t slot = 2 * static_cast<int64_t>(c) + (begin_of(c) >= first ? 0 : 1);
-        const float2 ml = p.part_ml[slot * p.part_rows + row];
-        const float4 x = *reinterpret_cast<const float4*>(p.part_o + (slot * p.part_rows + row) * D + d);
-        const float most = fmaxf(top, ml.x);
-        const float f0 = top == -INFINITY ? 0.0f : exp2_approx(top - most);
-        const float f1 = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - most);
-        top = most;
-        sum = __fmaf_rn(ml.y, f1, sum * f0);
-        o[0] = __fmaf_rn(x.x, f1, o[0] * f0);
-        o[1] = __fmaf_rn(x.y, f1, o[1] * f0);
-        o[2] = __fmaf_rn(x.z, f1, o[2] * f0);
-        o[3] = __fmaf_rn(x.w, f1, o[3] * f0);
     }
-    const bool valid = t < r.valid;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int g = (row & 127) % p.group;
-    bf16* dst = p.ctx + ((where.x * p.tokens + t) * p.q_heads + where.z * p.group + g) * D + d;
-    *reinterpret_cast<uint2*>(dst) = valid ? make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv),
-                                                        pack_bf16x2(o[2] * inv, o[3] * inv))
-                                           : make_uint2(0u, 0u);
-    if (d == 0 && p.stats != nullptr) {
-        p.stats[((where.x * p.kv_heads + where.z) * p.tokens + t) * p.group + g] =
-            valid ? make_float2(top == -INFINITY ? 0.0f : top, inv) : make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        s_rows[lane][warp * kPieces + i] =
+            valid ? make_uint2(pack_bf16x2(o[i][0] * inv, o[i][1] * inv), pack_bf16x2(o[i][2] * inv, o[i][3] * inv))
+                  : make_uint2(0u, 0u);
+    }
+    if (warp == 0) {
+        s_places[lane] = inside ? ((where.x * p.tokens + t) * p.q_heads + where.z * p.group + g) * D : -1;
+        if (inside && p.stats != nullptr) {
+            p.stats[((where.x * p.kv_heads + where.z) * p.tokens + t) * p.group + g] =
+                valid ? make_float2(top == -INFINITY ? 0.0f : top, inv) : make_float2(0.0f, 0.0f);
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * (D / 4); i += 256) {
+        const int64_t place = s_places[i / (D / 4)];
+        if (place >= 0) {
+            reinterpret_cast<uint2*>(p.ctx + place)[i % (D / 4)] = s_rows[i / (D / 4)][i % (D / 4)];
+        }
     }
 }
 
@@ -959,7 +1033,6 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
     }
     fence_proxy_async_smem();
     grid_dependency_begin();
-    const auto begin_of = [&](int64_t total, int64_t c) { return total * c / gridDim.x; };
     if (warp == 0) {
         int64_t total = 0;
         for (int64_t b = lane; b < p.batch; b += 32) {
@@ -968,8 +1041,9 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
         for (int offset = 16; offset > 0; offset >>= 1) {
             total += __shfl_xor_sync(0xffffffffu, total, offset);
         }
-        const int64_t begin = begin_of(total, blockIdx.x);
-        const int64_t end = begin_of(total, blockIdx.x + 1);
+        const Cuts cuts(total, gridDim.x);
+        const int64_t begin = cuts.begin(blockIdx.x);
+        const int64_t end = cuts.begin(blockIdx.x + 1);
         if (lane == 0) {
             UnitWalk w{};
             w.total = total;
@@ -1204,30 +1278,20 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
                     const int64_t end = first + tiles;
                     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (at.index == 0 ? 0 : 1);
                     p.part_sums[slot * 128 + row] = sum;
-                    int64_t c0 = first * gridDim.x / at.total;  // the part of the line that `first` lies in
-                    while (begin_of(at.total, c0) > first) {
-                        --c0;
-                    }
-                    while (begin_of(at.total, c0 + 1) <= first) {
-                        ++c0;
-                    }
-                    uint32_t parts = 0;
-                    for (int64_t c = c0; c < gridDim.x && begin_of(at.total, c) < end; ++c) {
-                        parts += begin_of(at.total, c) < begin_of(at.total, c + 1) ? 1u : 0u;
-                    }
+                    const Cuts cuts(at.total, gridDim.x);
+                    const int64_t c0 = cuts.of(first);
+                    const int64_t c1 = cuts.of(end - 1);  // parts between them are not empty
                     __threadfence();
                     named_barrier(1 + w, 128);
                     if (row == 0) {
-                        s_last[w] = atomicAdd(p.tickets + c0, 1u) == parts - 1u ? 1u : 0u;
+                        s_last[w] = atomicAdd(p.tickets + c0, 1u) == static_cast<unsigned>(c1 - c0) ? 1u : 0u;
                     }
                     named_barrier(1 + w, 128);
                     if (s_last[w] != 0u) {
                         __threadfence();
                         float all = 0.0f;
-                        for (int64_t c = c0; c < gridDim.x && begin_of(at.total, c) < end; ++c) {
-                            if (begin_of(at.total, c) < begin_of(at.total, c + 1)) {
-                                all += __ldcg(p.part_sums + (2 * c + (begin_of(at.total, c) >= first ? 0 : 1)) * 128 + row);
-                            }
+                        for (int64_t c = c0; c <= c1; ++c) {
+                            all += __ldcg(p.part_sums + (2 * c + (cuts.begin(c) >= first ? 0 : 1)) * 128 + row);
                         }
                         if (seen) {
                             *out += all;
@@ -1337,9 +1401,8 @@ cudaError_t launch_cache_attention(const CacheAttentionParams& p, const Plan& pl
         return err;
     }
     runtime::count_launches(1);
-    const unsigned rows = 256 / (D / 4);
     return runtime::launch(cache_attention_join_kernel<D, L::kKeys>,
-                           dim3(static_cast<unsigned>(pl.ctas - 1), (static_cast<unsigned>(p.part_rows) + rows - 1) / rows),
+                           dim3(static_cast<unsigned>(pl.ctas - 1), (static_cast<unsigned>(p.part_rows) + 31) / 32),
                            dim3(256), s, 1u, p, pl.ctas);
 }
 
