@@ -68,7 +68,7 @@ struct CacheAttentionParams {
     int q_box_tokens;     // tokens of one TMA box of q
     int part_rows;        // rows of a part in the scratch
     int4* cuts;           // [CTAs] where each CTA's part of the line begins: sequence, row tile, head, key tile
-    int64_t* line;        // length of the line
+    int* line;            // length of the line
     float2* part_ml;      // [2 CTAs][part_rows] (M in base 2, l)
     float* part_o;        // [2 CTAs][D / 4][part_rows][4]
     unsigned int* tickets;  // [weight CTAs] parts of a unit that have been left, zeroed by the attention kernel
@@ -101,10 +101,10 @@ struct ItemRange {
     int kv_end;    // keys from here on are seen by none
 };
 
-__device__ __forceinline__ ItemRange item_range(const CacheAttentionParams& p, int b, int row_tile) {
+__device__ __forceinline__ ItemRange item_range(const CacheAttentionParams& p, int len, int valid, int row_tile) {
     ItemRange r;
-    r.len = static_cast<int>(committed_rows(p, b));
-    r.valid = static_cast<int>(valid_queries(p, b));
+    r.len = len;
+    r.valid = valid;
     r.first = row_tile * p.item_tokens;
     if (r.first >= r.valid) {
         r.full_end = 0;
@@ -133,25 +133,33 @@ struct Tiling {
     static constexpr int kStreams = D == 256 ? 1 : 2;
     static constexpr int kAtoms = D / 64;
     static constexpr int kQTiles = kPair ? 2 : 1;
-    static constexpr int kAhead = kPair ? 1 : kStreams;  // K tiles loaded before the first V tile
-    static constexpr int kSlots = D == 64 ? 8 : 4;
+    static constexpr int kStep = kPair ? 1 : kStreams;  // a chain takes every kStep-th key tile of a segment
+    // Slots for K tiles and as many for V tiles, in rings of their own for each pair of chains that shares tiles, or
+    // for each chain that has tiles of its own: whoever waits for a slot's n-th tile has then seen its tile before.
+    static constexpr int kRings = kPair ? 1 : kStreams;
+    static constexpr int kDepth = (D == 64 ? 4 : 2) / kRings;
+    static constexpr int kSlots = 2 * kRings * kDepth;
     static constexpr int kThreads = 128 + 128 * kStreams;
-    static constexpr uint32_t kQAtom = 128 * 128;                // [128 rows][64 dims]
-    static constexpr uint32_t kKvAtom = kKeys * 128;             // [keys][64 dims]
+    static constexpr uint32_t kQAtom = 128 * 128;    // [128 rows][64 dims]
+    static constexpr uint32_t kKvAtom = kKeys * 128;  // [keys][64 dims]
     static constexpr uint32_t kSlot = kKvAtom * kAtoms;
     static constexpr uint32_t kQ = 0;
     static constexpr uint32_t kRing = kQ + kQTiles * kAtoms * kQAtom;
-    static constexpr uint32_t kExchange = kRing + kSlots * kSlot;  // O columns of the second chain, [128][33] f32
-    static constexpr uint32_t kMask = kExchange + (kStreams == 2 && !kPair ? 128 * 33 * 4 : 0);  // [chains][128][9]
-    static constexpr uint32_t kMl = kMask + kStreams * 128 * 9 * 4;
-    static constexpr uint32_t kFlags = kMl + 128 * 8;
-    static constexpr uint32_t kStage = kFlags + 2 * 16 * 4;  // a warp's context rows, [32][64 bytes]
-    static constexpr uint32_t kBars = kStage + kStreams * 4 * 2048;
+    static constexpr uint32_t kMask = kRing + kSlots * kSlot;       // [chains][128][9] mask bits
+    static constexpr uint32_t kMl = kMask + kStreams * 128 * 9 * 4;  // [128] the second chain's (M, l)
+    static constexpr uint32_t kFlags = kMl + 128 * 8;               // [2][16]
+    static constexpr uint32_t kBars = kFlags + 2 * 16 * 4;
     static constexpr std::size_t kBytes = 1024 + kBars + 256;
     // Tensor memory columns: the chains' S (P over it), then their O.
     static constexpr uint32_t kTmemO = kStreams * kKeys;
-    static_assert(kStreams * (kKeys + D) <= 512, "tensor memory has 512 columns");
-    static_assert(kBytes <= 232448, "shared memory of a CTA");
+    static_assert(kDepth >= 1 && kStreams * (kKeys + D) <= 512, "tensor memory has 512 columns");
+
+    // The slot of a ring's n-th K or V tile, and the parity of its barriers' phase.
+    __device__ static __forceinline__ int k_slot(int ring, uint32_t n) { return ring * 2 * kDepth + static_cast<int>(n % kDepth); }
+    __device__ static __forceinline__ int v_slot(int ring, uint32_t n) { return k_slot(ring, n) + kDepth; }
+    __device__ static __forceinline__ uint32_t parity(uint32_t n) { return n / kDepth & 1u; }
+
+    static_assert(kBytes <= 232448 - 512, "shared memory of a CTA");
 };
 
 constexpr uint32_t kTmemAll = 512;
@@ -161,50 +169,46 @@ struct Walk {
     int b;
     int row_tile;
     int h;
-    int tile;       // first key tile of the current segment
-    int64_t left;   // key tiles of the part still to come, the current segment's included
-    uint32_t fills; // ring slots filled before the current segment
-    int index;      // segments before the current one
+    int tile;        // first key tile of the current segment
+    int left;        // key tiles of the part still to come, the current segment's included
+    int len;         // of sequence b
+    int valid;
+    int index;       // segments before the current one
 };
 
 __device__ __forceinline__ void advance(const CacheAttentionParams& p, Walk& w, int count, int tiles) {
     w.left -= count;
-    w.fills += 2u * static_cast<uint32_t>(count);
     ++w.index;
     w.tile += count;
-    if (w.tile >= tiles) {
-        w.tile = 0;
-        if (++w.h == static_cast<int>(p.kv_heads)) {
-            w.h = 0;
-            if (++w.row_tile == p.row_tiles) {
-                w.row_tile = 0;
-                ++w.b;
-            }
-        }
+    if (w.tile < tiles) {
+        return;
     }
-}
-
-// Fill numbers of a segment's K and V tiles: `ahead` K tiles first, then V and K tiles in turn.
-__device__ __forceinline__ uint32_t fill_of_k(uint32_t fills, int i, int ahead) {
-    return fills + static_cast<uint32_t>(i < ahead ? i : 2 * i - ahead + 1);
-}
-
-__device__ __forceinline__ uint32_t fill_of_v(uint32_t fills, int i, int ahead, int count) {
-    const int lead = count < ahead ? count : ahead;
-    const int k = i < count - lead ? i : count - lead;
-    return fills + static_cast<uint32_t>(lead + i + k);
+    w.tile = 0;
+    if (++w.h < static_cast<int>(p.kv_heads)) {
+        return;
+    }
+    w.h = 0;
+    if (++w.row_tile < p.row_tiles) {
+        return;
+    }
+    w.row_tile = 0;
+    ++w.b;
+    if (w.left > 0) {
+        w.len = static_cast<int>(committed_rows(p, w.b));
+        w.valid = static_cast<int>(valid_queries(p, w.b));
+    }
 }
 
 // A line of `total` pieces cut into `parts` that differ by one piece at most.
 struct Cuts {
-    int64_t each;
-    int64_t extra;  // the first `extra` parts have one more
+    int each;
+    int extra;  // the first `extra` parts have one more
 
-    __device__ __forceinline__ Cuts(int64_t total, unsigned parts) : each(total / parts), extra(total - each * parts) {}
-    __device__ __forceinline__ int64_t begin(int64_t part) const { return part * each + (part < extra ? part : extra); }
-    __device__ __forceinline__ bool empty(int64_t part) const { return each == 0 && part >= extra; }
-    __device__ __forceinline__ int64_t of(int64_t piece) const {  // the part that a piece lies in
-        const int64_t longer = extra * (each + 1);
+    __device__ __forceinline__ Cuts(int total, int parts) : each(total / parts), extra(total - each * parts) {}
+    __device__ __forceinline__ int begin(int part) const { return part * each + (part < extra ? part : extra); }
+    __device__ __forceinline__ bool empty(int part) const { return each == 0 && part >= extra; }
+    __device__ __forceinline__ int of(int piece) const {  // the part that a piece lies in
+        const int longer = extra * (each + 1);
         return piece < longer ? piece / (each + 1) : extra + (piece - longer) / each;
     }
 };
@@ -250,6 +254,51 @@ __device__ __forceinline__ uint32_t visible_bits(const uint32_t* row, int key, i
     return word >= 8 ? 0u : __funnelshift_r(row[word], row[word + 1], static_cast<uint32_t>(j & 31));
 }
 
+// Scores of keys that the row does not see become -inf; words of 32 keys that every row of the warp sees are left alone.
+template <int N>
+__device__ __forceinline__ void hide(float (&x)[N], const uint32_t* row, int key, int len, int limit) {
+#pragma unroll
+    for (int c = 0; c < N / 32; ++c) {
+        const uint32_t see = visible_bits(row, key + c * 32, len, limit);
+        if (!__all_sync(0xffffffffu, see == 0xffffffffu)) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                x[c * 32 + j] = (see >> j & 1u) != 0u ? x[c * 32 + j] : -INFINITY;
+            }
+        }
+    }
+}
+
+template <int N>
+__device__ __forceinline__ float largest(const float (&x)[N], float top) {
+    float tops[4] = {top, top, top, top};
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {
+        tops[j & 3] = max3(tops[j & 3], x[2 * j], x[2 * j + 1]);
+    }
+    return fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+}
+
+// P of N keys, 2^(x factor + offset), stored as bf16 pairs at `taddr`; returns their sum in f32.
+template <int N>
+__device__ __forceinline__ float probabilities(const float (&x)[N], float2 factor, float2 offset, uint32_t taddr) {
+    float2 sums[2] = {};
+#pragma unroll
+    for (int c = 0; c < N / 32; ++c) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int k = c * 32 + 2 * j;
+            float2 e = __ffma2_rn(make_float2(x[k], x[k + 1]), factor, offset);
+            e = make_float2(exp2_approx(e.x), exp2_approx(e.y));
+            sums[j & 1] = __fadd2_rn(sums[j & 1], e);
+            packed[j] = pack_bf16x2(e.x, e.y);
+        }
+        tmem_store16(taddr + c * 16, packed);
+    }
+    return (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
+}
+
 // A pair of bf16 values with +0 in the place of each that is not finite.
 __device__ __forceinline__ uint32_t finite_pair(uint32_t pair) {
     return ((pair & 0x7f80u) == 0x7f80u ? 0u : pair & 0xffffu) |
@@ -270,12 +319,11 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
     using L = Tiling<D, kPair>;
     constexpr int kStreams = L::kStreams;
     constexpr int kKeys = L::kKeys;
-    constexpr int kAhead = L::kAhead;
+    constexpr int kHalf = kKeys / 2;
     extern __shared__ __align__(16) unsigned char raw[];
     unsigned char* sm = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
     uint32_t* s_mask = reinterpret_cast<uint32_t*>(sm + L::kMask);
     float2* s_ml = reinterpret_cast<float2*>(sm + L::kMl);
-    float* s_exchange = reinterpret_cast<float*>(sm + L::kExchange);
     uint32_t* s_flags = reinterpret_cast<uint32_t*>(sm + L::kFlags);
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::kBars);
     uint64_t* bar_full = bars;                    // [slots] a K or V tile has landed
@@ -283,8 +331,8 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
     uint64_t* bar_q_full = bars + 2 * L::kSlots;
     uint64_t* bar_q_empty = bar_q_full + 1;
     uint64_t* bar_s = bar_q_empty + 1;            // [chains] S is complete
-    uint64_t* bar_p = bar_s + kStreams;           // [chains] P is written
-    uint64_t* bar_o = bar_p + kStreams;           // [chains] the segment's O is complete
+    uint64_t* bar_p = bar_s + kStreams;           // [chains][2] half of P is written
+    uint64_t* bar_o = bar_p + 2 * kStreams;       // [chains] the segment's O is complete
     __shared__ uint32_t s_tmem;
     __shared__ uint32_t s_stop;
     __shared__ Walk s_walk;
@@ -296,13 +344,14 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
         s_stop = 0u;
         for (int i = 0; i < L::kSlots; ++i) {
             mbar_init(bar_full + i, 1);
-            mbar_init(bar_empty + i, 1);
+            mbar_init(bar_empty + i, kPair ? 2 : 1);
         }
         mbar_init(bar_q_full, 1);
-        mbar_init(bar_q_empty, 1);
+        mbar_init(bar_q_empty, kStreams);
         for (int w = 0; w < kStreams; ++w) {
             mbar_init(bar_s + w, 1);
-            mbar_init(bar_p + w, 4);
+            mbar_init(bar_p + 2 * w, 4);
+            mbar_init(bar_p + 2 * w + 1, 4);
             mbar_init(bar_o + w, 1);
         }
     }
@@ -311,48 +360,52 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
     }
     grid_dependency_begin();
     if (warp == 0) {  // the line's length, and where this CTA's part of it begins
-        const int64_t entries = p.batch * p.row_tiles;
-        const auto tiles_at = [&](int64_t e) -> int64_t {
-            if (e >= entries) {
-                return 0;
+        const int heads = static_cast<int>(p.kv_heads);
+        const int entries = static_cast<int>(p.batch) * p.row_tiles;
+        const auto entry = [&](int e) {
+            Walk w{};
+            w.b = e / p.row_tiles;
+            w.row_tile = e - w.b * p.row_tiles;
+            if (e < entries) {
+                w.len = static_cast<int>(committed_rows(p, w.b));
+                w.valid = static_cast<int>(valid_queries(p, w.b));
             }
-            const int b = static_cast<int>(e / p.row_tiles);
-            return item_tiles<kKeys>(item_range(p, b, static_cast<int>(e - int64_t{b} * p.row_tiles))) * p.kv_heads;
+            return w;
         };
-        int64_t total = 0;
-        for (int64_t e = lane; e - lane < entries; e += 32) {
-            total += tiles_at(e);
+        const auto tiles_of = [&](int e, const Walk& w) {
+            return e < entries ? item_tiles<kKeys>(item_range(p, w.len, w.valid, w.row_tile)) * heads : 0;
+        };
+        Walk w = entry(lane);
+        int mine = tiles_of(lane, w);
+        int total = mine;
+        for (int e = lane + 32; e - lane < entries; e += 32) {
+            total += tiles_of(e, entry(e));
         }
-        for (int offset = 16; offset > 0; offset >>= 1) {
-            total += __shfl_xor_sync(0xffffffffu, total, offset);
-        }
-        const Cuts cuts(total, gridDim.x);
-        const int64_t begin = cuts.begin(blockIdx.x);
-        const int64_t end = cuts.begin(blockIdx.x + 1);
+        total = __reduce_add_sync(0xffffffffu, total);
+        const Cuts cuts(total, static_cast<int>(gridDim.x));
+        const int begin = cuts.begin(static_cast<int>(blockIdx.x));
+        const int end = cuts.begin(static_cast<int>(blockIdx.x) + 1);
         if (lane == 0) {
             s_walk = Walk{};  // a part of the line may be empty
         }
         __syncwarp();
-        int64_t before = 0;
-        for (int64_t e0 = 0; e0 < entries; e0 += 32) {
-            const int64_t mine = tiles_at(e0 + lane);
-            int64_t sum = mine;
+        int before = 0;
+        for (int e0 = 0; e0 < entries; e0 += 32) {
+            if (e0 > 0) {
+                w = entry(e0 + lane);
+                mine = tiles_of(e0 + lane, w);
+            }
+            int sum = mine;
             for (int offset = 1; offset < 32; offset <<= 1) {
-                const int64_t other = __shfl_up_sync(0xffffffffu, sum, offset);
+                const int other = __shfl_up_sync(0xffffffffu, sum, offset);
                 sum += lane >= offset ? other : 0;
             }
-            const int64_t lo = before + sum - mine;
+            const int lo = before + sum - mine;
             if (begin >= lo && begin < lo + mine) {
-                const int64_t e = e0 + lane;
-                const int64_t each = mine / p.kv_heads;
-                Walk w;
-                w.b = static_cast<int>(e / p.row_tiles);
-                w.row_tile = static_cast<int>(e % p.row_tiles);
-                w.h = static_cast<int>((begin - lo) / each);
-                w.tile = static_cast<int>((begin - lo) % each);
+                const int each = mine / heads;
+                w.h = (begin - lo) / each;
+                w.tile = (begin - lo) - w.h * each;
                 w.left = end - begin;
-                w.fills = 0;
-                w.index = 0;
                 s_walk = w;
                 p.cuts[blockIdx.x] = make_int4(w.b, w.row_tile, w.h, w.tile);
             }
@@ -376,9 +429,20 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
     const uint32_t tmem = s_tmem;
     const Waiter wait{p.error, p.poll_limit, &s_stop};
     Walk at = s_walk;
-    // Chains at work in a segment of `count` key tiles.
-    const auto chains_of = [&](const ItemRange& r, int count) {
-        return kStreams == 1 ? 1 : kPair ? (r.first + p.tile_tokens < p.tokens ? 2 : 1) : (count < 2 ? count : 2);
+    // The current segment: its item, the item's key tiles, the key tiles of them that it takes, the chains at work.
+    ItemRange r{};
+    int tiles = 0;
+    int count = 0;
+    int chains = 0;
+    const auto segment = [&]() {
+        if (at.left <= 0) {
+            return false;
+        }
+        r = item_range(p, at.len, at.valid, at.row_tile);
+        tiles = item_tiles<kKeys>(r);
+        count = tiles - at.tile < at.left ? tiles - at.tile : at.left;
+        chains = kStreams == 1 ? 1 : kPair ? (r.first + p.tile_tokens < p.tokens ? 2 : 1) : (count < 2 ? count : 2);
+        return true;
     };
     // A row of S takes 128 registers: with two chains the control warps give up what they do not need of the 168
     // registers a thread that 384 threads start with (128 * 88 + 256 * 208 = 384 * 168).
@@ -386,65 +450,79 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
         if constexpr (kStreams == 2) {
             asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         }
-    if (warp == 0) {
-        if (lane == 0) {  // ---- loads
-            uint32_t fill = 0;
-            const auto load = [&](const CUtensorMap* map, int b, int h, int tile) {
-                const uint32_t slot = fill % L::kSlots;
-                const uint32_t round = fill / L::kSlots;
-                if (round > 0) {
-                    wait(bar_empty + slot, (round - 1) & 1u);
+        if (warp == 0 && lane == 0) {  // ---- loads
+            uint32_t k_tiles[L::kRings] = {};  // loaded so far
+            uint32_t v_tiles[L::kRings] = {};
+            const auto load = [&](const CUtensorMap* map, int slot, uint32_t n, int tile) {
+                if (n >= static_cast<uint32_t>(L::kDepth)) {
+                    wait(bar_empty + slot, L::parity(n) ^ 1u);
                 }
                 mbar_arrive_expect_tx(bar_full + slot, L::kSlot);
                 unsigned char* dst = sm + L::kRing + slot * L::kSlot;
+#pragma unroll
                 for (int a = 0; a < L::kAtoms; ++a) {
-                    tma_load_4d(dst + a * L::kKvAtom, map, a * 64, h, tile * kKeys, b, bar_full + slot);
+                    tma_load_4d(dst + a * L::kKvAtom, map, a * 64, at.h, tile * kKeys, at.b, bar_full + slot);
                 }
-                ++fill;
             };
-            while (at.left > 0) {
-                const ItemRange r = item_range(p, at.b, at.row_tile);
-                const int tiles = item_tiles<kKeys>(r);
-                const int count = static_cast<int>(tiles - at.tile < at.left ? tiles - at.tile : at.left);
+            // Tile i of the segment; a tile that does not exist is left out.
+            const auto load_k = [&](int i) {
+                const int ring = i % L::kRings;
+                if (i < count) {
+                    load(&map_k, L::k_slot(ring, k_tiles[ring]), k_tiles[ring], at.tile + i);
+                    ++k_tiles[ring];
+                }
+            };
+            const auto load_v = [&](int i) {
+                const int ring = i % L::kRings;
+                if (i < count) {
+                    load(&map_v, L::v_slot(ring, v_tiles[ring]), v_tiles[ring], at.tile + i);
+                    ++v_tiles[ring];
+                }
+            };
+            for (; segment(); advance(p, at, count, tiles)) {
                 if (at.index > 0) {
                     wait(bar_q_empty, static_cast<uint32_t>(at.index - 1) & 1u);
                 }
-                const int q_tiles = kPair ? chains_of(r, count) : 1;
+                const int q_tiles = kPair ? chains : 1;
                 const uint32_t box = static_cast<uint32_t>(p.q_box_tokens * p.group) * 128u;
                 mbar_arrive_expect_tx(bar_q_full, box * L::kAtoms * q_tiles);
                 for (int i = 0; i < q_tiles; ++i) {
+#pragma unroll
                     for (int a = 0; a < L::kAtoms; ++a) {
                         tma_load_4d(sm + L::kQ + (i * L::kAtoms + a) * L::kQAtom, &map_q, a * 64, at.h * p.group,
                                     r.first + i * p.tile_tokens, at.b, bar_q_full);
                     }
                 }
-                const int lead = count < kAhead ? count : kAhead;
-                for (int i = 0; i < lead; ++i) {
-                    load(&map_k, at.b, at.h, at.tile + i);
+                // In the order in which slots come free: a chain's S lets go of its K tile, its O a step later of its V tile.
+                for (int i = 0; i < L::kStep; ++i) {
+                    load_k(i);
                 }
-                for (int i = 0; i < count; ++i) {
-                    load(&map_v, at.b, at.h, at.tile + i);
-                    if (i + lead < count) {
-                        load(&map_k, at.b, at.h, at.tile + i + lead);
-                    }
+                for (int i = 0; i < L::kStep; ++i) {
+                    load_v(i);
                 }
-                advance(p, at, count, tiles);
+                for (int i = L::kStep; i < 2 * L::kStep; ++i) {
+                    load_k(i);
+                }
+                for (int i = L::kStep; i < count; ++i) {
+                    load_v(i);
+                    load_k(i + L::kStep);
+                }
             }
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {  // ---- matrix products
+        } else if ((warp == 1 || (warp == 3 && kStreams == 2)) && lane == 0) {  // ---- matrix products of chain w
+            const int w = warp >> 1;
             constexpr uint32_t s_idesc = idesc_bf16_f32(kKeys);
             constexpr uint32_t o_idesc = idesc_bf16_f32_bmn(D);
-            uint32_t p_phase[kStreams] = {};
-            const auto slot_of = [&](uint32_t fill) { return fill % L::kSlots; };
-            const auto landed = [&](uint32_t fill) {
-                wait(bar_full + slot_of(fill), (fill / L::kSlots) & 1u);
+            const unsigned char* q = sm + L::kQ + (kPair ? w * L::kAtoms * L::kQAtom : 0);
+            const int ring = kPair ? 0 : w;
+            uint32_t n = 0;  // tiles of the chain before the current one
+            const auto landed = [&](int slot, uint32_t tile) {
+                wait(bar_full + slot, L::parity(tile));
                 tc_fence_after();
             };
-            // S of chain w = its Q tile times the K tile of `fill`.
-            const auto scores = [&](int w, uint32_t fill) {
-                const unsigned char* q = sm + L::kQ + (kPair ? w * L::kAtoms * L::kQAtom : 0);
-                const unsigned char* k = sm + L::kRing + slot_of(fill) * L::kSlot;
+            const auto scores = [&](uint32_t tile) {
+                const int slot = L::k_slot(ring, tile);
+                const unsigned char* k = sm + L::kRing + slot * L::kSlot;
+                landed(slot, tile);
 #pragma unroll
                 for (int i = 0; i < D / kUmmaK; ++i) {
                     const uint32_t in = static_cast<uint32_t>(i & 3) * 32u;
@@ -452,69 +530,52 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                               smem_desc_sw128(k, (i >> 2) * L::kKvAtom + in), s_idesc, i > 0 ? 1u : 0u);
                 }
                 umma_commit(bar_s + w);
+                umma_commit(bar_empty + slot);
             };
-            // O of chain w += its P times the V tile of `fill`.
-            const auto product = [&](int w, uint32_t fill, bool first) {
-                wait(bar_p + w, p_phase[w]);
-                p_phase[w] ^= 1u;
-                tc_fence_after();
-                const unsigned char* v = sm + L::kRing + slot_of(fill) * L::kSlot;
-#pragma unroll
-                for (int i = 0; i < kKeys / kUmmaK; ++i) {
-                    umma_bf16_ta(tmem + L::kTmemO + w * D, tmem + w * kKeys + i * 8,
-                                 smem_desc_sw128_mn(v, i * 2048u, L::kKvAtom), o_idesc, (!first || i > 0) ? 1u : 0u);
-                }
-            };
-            while (at.left > 0) {
-                const ItemRange r = item_range(p, at.b, at.row_tile);
-                const int tiles = item_tiles<kKeys>(r);
-                const int count = static_cast<int>(tiles - at.tile < at.left ? tiles - at.tile : at.left);
-                const int chains = chains_of(r, count);
+            uint32_t p_phase = 0;
+            for (; segment(); advance(p, at, count, tiles)) {
                 wait(bar_q_full, static_cast<uint32_t>(at.index) & 1u);
                 tc_fence_after();
-                const int lead = count < kAhead ? count : kAhead;
-                for (int i = 0; i < lead; ++i) {
-                    const uint32_t fill = fill_of_k(at.fills, i, lead);
-                    landed(fill);
-                    for (int w = kPair ? 0 : i; w < (kPair ? chains : i + 1); ++w) {
-                        scores(w, fill);
+                if (w >= chains) {  // this segment has nothing for the chain
+                    for (int i = 0; kPair && i < count; ++i, ++n) {
+                        landed(L::k_slot(ring, n), n);
+                        umma_commit(bar_empty + L::k_slot(ring, n));
+                        landed(L::v_slot(ring, n), n);
+                        umma_commit(bar_empty + L::v_slot(ring, n));
                     }
-                    umma_commit(bar_empty + slot_of(fill));
-                }
-                if (count == lead) {
                     umma_commit(bar_q_empty);
+                    continue;
                 }
-                for (int i = 0; i < count; ++i) {
-                    const uint32_t vf = fill_of_v(at.fills, i, lead, count);
-                    const uint32_t kf = fill_of_k(at.fills, i + lead, lead);
-                    const bool more = i + lead < count;
-                    landed(vf);
-                    const int w0 = kPair ? 0 : i % kStreams;
-                    const int w1 = kPair ? chains : w0 + 1;
-                    for (int w = w0; w < w1; ++w) {
-                        product(w, vf, kPair ? i == 0 : i < kStreams);
-                        if (w == w1 - 1) {
-                            umma_commit(bar_empty + slot_of(vf));
-                        }
-                        if (more) {
-                            if (w == w0) {
-                                landed(kf);
-                            }
-                            scores(w, kf);
-                        } else {
-                            umma_commit(bar_o + w);
+                const int first = kPair ? 0 : w;
+                scores(n);
+                for (int i = first; i < count; i += L::kStep, ++n) {
+                    const bool more = i + L::kStep < count;
+                    if (!more) {
+                        umma_commit(bar_q_empty);
+                    }
+                    const int slot = L::v_slot(ring, n);
+                    const unsigned char* v = sm + L::kRing + slot * L::kSlot;
+                    landed(slot, n);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        wait(bar_p + 2 * w + half, p_phase);
+                        tc_fence_after();
+#pragma unroll
+                        for (int j = half * (kHalf / kUmmaK); j < (half + 1) * (kHalf / kUmmaK); ++j) {
+                            umma_bf16_ta(tmem + L::kTmemO + w * D, tmem + w * kKeys + j * 8,
+                                         smem_desc_sw128_mn(v, j * 2048u, L::kKvAtom), o_idesc,
+                                         (i > first || j > 0) ? 1u : 0u);
                         }
                     }
+                    p_phase ^= 1u;
+                    umma_commit(bar_empty + slot);
                     if (more) {
-                        umma_commit(bar_empty + slot_of(kf));
-                        if (i + lead == count - 1) {
-                            umma_commit(bar_q_empty);
-                        }
+                        scores(n + 1);
+                    } else {
+                        umma_commit(bar_o + w);
                     }
                 }
-                advance(p, at, count, tiles);
             }
-        }
         }
     } else {  // ---- softmax: chain w, one thread per row
         if constexpr (kStreams == 2) {
@@ -530,13 +591,10 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
         const float c2 = 1.4426950408889634f / sqrtf(static_cast<float>(D));
         uint32_t s_phase = 0;
         uint32_t o_phase = 0;
-        while (at.left > 0) {
-            const ItemRange r = item_range(p, at.b, at.row_tile);
-            const int tiles = item_tiles<kKeys>(r);
-            const int count = static_cast<int>(tiles - at.tile < at.left ? tiles - at.tile : at.left);
-            const int chains = chains_of(r, count);
+        uint32_t n = 0;  // tiles of the chain before the current one
+        for (; segment(); advance(p, at, count, tiles)) {
             if (w >= chains) {
-                advance(p, at, count, tiles);
+                n += kPair ? static_cast<uint32_t>(count) : 0u;
                 continue;
             }
             const int token0 = r.first + (kPair ? w * p.tile_tokens : 0);
@@ -545,7 +603,6 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             const bool valid = inside && t < r.valid;
             const bool busy = __any_sync(0xffffffffu, inside);
             const int limit = valid ? r.len + t + 1 : 0;
-            const int lead = count < kAhead ? count : kAhead;
             const int part0 = r.full_end / kKeys * kKeys;  // first key of the first tile in which a key may be hidden
             const bool hides = (at.tile + count) * kKeys > r.full_end;  // the segment has such tiles
             const uint32_t* bits_row = nullptr;
@@ -581,73 +638,17 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             }
             float top = -INFINITY;  // the maximum that P is taken against, in units of S
             float sum = 0.0f;
-            for (int i = kPair ? 0 : w; i < count; i += kPair ? 1 : kStreams) {
+            for (int i = kPair ? 0 : w; i < count; i += L::kStep, ++n) {
                 const int key0 = (at.tile + i) * kKeys;
                 const bool partial = key0 + kKeys > r.full_end;
                 wait(bar_s + w, s_phase);
                 s_phase ^= 1u;
                 tc_fence_after();
-                if (busy) {
-                    float x[kKeys];
-                    tmem_load_row<kKeys>(t_s, x);
-                    if (partial) {
-#pragma unroll
-                        for (int c = 0; c < kKeys / 32; ++c) {
-                            const uint32_t see = visible_bits(bits_row, key0 + c * 32, r.len, limit);
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) {
-                                x[c * 32 + j] = (see >> j & 1u) != 0u ? x[c * 32 + j] : -INFINITY;
-                            }
-                        }
-                    }
-                    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int j = 0; j < kKeys / 2; ++j) {
-                        tops[j & 3] = max3(tops[j & 3], x[2 * j], x[2 * j + 1]);
-                    }
-                    const float tile_top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-                    const float new_top = fmaxf(top, tile_top);
-                    const bool first = i < kStreams && (!kPair || i == 0);
-                    const bool grown = first || (new_top - top) * c2 > 8.0f;
-                    if (!first && __any_sync(0xffffffffu, grown)) {
-                        const float f = grown ? exp2_approx((top - new_top) * c2) : 1.0f;
-                        sum *= f;
-#pragma unroll 1
-                        for (int c = 0; c < D / 16; ++c) {
-                            uint32_t o[16];
-                            tmem_load16(t_o + c * 16, o);
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) {
-                                o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-                            }
-                            tmem_store16(t_o + c * 16, o);
-                        }
-                    }
-                    top = grown ? new_top : top;
-                    const float shift = top == -INFINITY ? 0.0f : top * c2;
-                    const float2 factor = make_float2(c2, c2);
-                    const float2 offset = make_float2(-shift, -shift);
-                    float2 sums[2] = {};
-#pragma unroll
-                    for (int c = 0; c < kKeys / 32; ++c) {
-                        uint32_t packed[16];
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const int k = c * 32 + 2 * j;
-                            float2 e = __ffma2_rn(make_float2(x[k], x[k + 1]), factor, offset);
-                            e = make_float2(exp2_approx(e.x), exp2_approx(e.y));
-                            sums[j & 1] = __fadd2_rn(sums[j & 1], e);
-                            packed[j] = pack_bf16x2(e.x, e.y);
-                        }
-                        tmem_store16(t_s + c * 16, packed);
-                    }
-                    sum += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
-                    tmem_store_wait();
-                }
                 if (partial) {  // V rows that nobody sees become zeros, values that are not finite are set aside
-                    const uint32_t fill = fill_of_v(at.fills, i, lead, count);
-                    wait(bar_full + fill % L::kSlots, (fill / L::kSlots) & 1u);
-                    unsigned char* v = sm + L::kRing + fill % L::kSlots * L::kSlot;
+                    // S is complete, so the chain's product before is, and the slot's tile before this one has landed.
+                    const int slot = L::v_slot(kPair ? 0 : w, n);
+                    wait(bar_full + slot, L::parity(n));
+                    unsigned char* v = sm + L::kRing + slot * L::kSlot;
                     const int sharing = kPair ? chains : 1;  // chains that read this tile
                     for (int u = (sharing == 2 ? w * 128 : 0) + row; u < kKeys * L::kAtoms; u += 128 * sharing) {
                         const int key = u % kKeys;  // this thread's: 64 dims of a row
@@ -680,54 +681,109 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                         named_barrier(3, 256);
                     }
                 }
+                float2 factor = make_float2(c2, c2);
+                float2 offset = make_float2(0.0f, 0.0f);
+                float x0[kHalf];
+                float x1[kHalf];
+                if (busy) {
+                    tmem_load_begin<kHalf>(t_s, x0);
+                    tmem_load_end<kHalf>(x0);
+                    tmem_load_begin<kHalf>(t_s + kHalf, x1);
+                    if (partial) {
+                        hide(x0, bits_row, key0, r.len, limit);
+                    }
+                    float new_top = largest(x0, top);
+                    tmem_load_end<kHalf>(x1);
+                    if (partial) {
+                        hide(x1, bits_row, key0 + kHalf, r.len, limit);
+                    }
+                    new_top = largest(x1, new_top);
+                    const bool first = i < L::kStep;
+                    const bool grown = first || (new_top - top) * c2 > 8.0f;
+                    if (!first && __any_sync(0xffffffffu, grown)) {
+                        const float f = grown ? exp2_approx((top - new_top) * c2) : 1.0f;
+                        sum *= f;
+#pragma unroll 1
+                        for (int c = 0; c < D / 16; ++c) {
+                            uint32_t o[16];
+                            tmem_load16(t_o + c * 16, o);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                            }
+                            tmem_store16(t_o + c * 16, o);
+                        }
+                    }
+                    top = grown ? new_top : top;
+                    const float shift = top == -INFINITY ? 0.0f : top * c2;
+                    offset = make_float2(-shift, -shift);
+                    sum += probabilities(x0, factor, offset, t_s);
+                    tmem_store_wait();
+                }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(bar_p + w);
+                    mbar_arrive(bar_p + 2 * w);
+                }
+                if (busy) {
+                    sum += probabilities(x1, factor, offset, t_s + kHalf / 2);
+                    tmem_store_wait();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(bar_p + 2 * w + 1);
                 }
             }
             wait(bar_o + w, o_phase);
             o_phase ^= 1u;
             tc_fence_after();
-            // Values that are not finite, in rows that this row sees: added to O as they are.
-            uint32_t flagged = 0u;
             if (hides) {
                 named_barrier(1 + w, 128);  // the flags of all the chain's threads
-                for (int i = 0; i < 32; ++i) {
-                    flagged |= kPair || (i >> 4) == w ? s_flags[i] : 0u;
+                uint32_t flagged = 0u;
+                for (int i = 0; i < 16; ++i) {
+                    flagged |= s_flags[w * 16 + i] | (kPair && chains == 2 ? s_flags[(1 - w) * 16 + i] : 0u);
                 }
-            }
-            const auto add_set_aside = [&](float (&o)[32], int d0) {
-                for (int i = 0; i < 32; ++i) {
-                    uint32_t word = kPair ? (i < 16 ? s_flags[i] | (chains > 1 ? s_flags[16 + i] : 0u) : 0u)
-                                          : (i < 16 ? s_flags[w * 16 + i] : 0u);
-                    while (word != 0u) {
-                        const int key = part0 + i * 32 + __ffs(word) - 1;
-                        word &= word - 1u;
-                        const bool sees_it = valid && (visible_bits(bits_row, key, r.len, limit) & 1u) != 0u;
-                        const bf16* v = p.v + at.b * p.vs[0] + key * p.vs[1] + at.h * p.vs[2] + d0;
-                        for (int j = 0; j < 32; ++j) {
-                            const float x = __bfloat162float(v[j]);
-                            if (sees_it && !(fabsf(x) < INFINITY)) {
-                                o[j] += x;
+                if (flagged != 0u && busy) {  // values that are not finite, added to the O of the rows that see them
+#pragma unroll 1
+                    for (int c = 0; c < D / 16; ++c) {
+                        uint32_t o[16];
+                        tmem_load16(t_o + c * 16, o);
+                        for (int i = 0; i < 16; ++i) {
+                            uint32_t word = s_flags[w * 16 + i] | (kPair && chains == 2 ? s_flags[(1 - w) * 16 + i] : 0u);
+                            while (word != 0u) {
+                                const int key = part0 + i * 32 + __ffs(word) - 1;
+                                word &= word - 1u;
+                                const bool seen = valid && (visible_bits(bits_row, key, r.len, limit) & 1u) != 0u;
+                                const bf16* v = p.v + at.b * p.vs[0] + key * p.vs[1] + at.h * p.vs[2] + c * 16;
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) {
+                                    const float x = __bfloat162float(v[j]);
+                                    if (seen && !(fabsf(x) < INFINITY)) {
+                                        o[j] = __float_as_uint(__uint_as_float(o[j]) + x);
+                                    }
+                                }
                             }
                         }
+                        __syncwarp();
+                        tmem_store16(t_o + c * 16, o);
                     }
+                    tmem_store_wait();
                 }
-            };
+            }
             float scaled_top = top == -INFINITY ? -INFINITY : top * c2;
             const bool whole = at.tile == 0 && count == tiles;
-            const bool joins = !kPair && chains == 2;
-            const int64_t item_row = static_cast<int64_t>(kPair ? w * 128 : 0) + row;
-            const int64_t part = 2 * static_cast<int64_t>(blockIdx.x) + (at.index == 0 ? 0 : 1);
+            const bool joins = !kPair && chains == 2;  // the second chain's sums and O are the first's to add
             float f0 = 1.0f;
             float f1 = 0.0f;
-            if (joins) {  // the two chains' sums: the second hands its maximum, sum and O to the first
+            if (joins) {
                 if (w == 1) {
                     s_ml[row] = make_float2(scaled_top, sum);
+                    tc_fence_before();
                 }
                 named_barrier(3, 256);
                 if (w == 0) {
+                    tc_fence_after();
                     const float2 other = s_ml[row];
                     const float most = fmaxf(scaled_top, other.x);
                     f0 = scaled_top == -INFINITY ? 0.0f : exp2_approx(scaled_top - most);
@@ -736,88 +792,59 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                     scaled_top = most;
                 }
             }
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            uint4* stage = reinterpret_cast<uint4*>(sm + L::kStage) + (warp - 4) * 128;
-            // Where the four rows that this lane writes a piece of lie in ctx.
-            const int64_t place = inside ? ((at.b * p.tokens + t) * p.q_heads + at.h * p.group + g) * D : -1;
-            int64_t places[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                places[i] = __shfl_sync(0xffffffffu, place, i * 8 + (lane >> 2));
-            }
+            if (busy && !(joins && w == 1)) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const int64_t part_row = static_cast<int64_t>(kPair ? w * 128 : 0) + row;
+                const int64_t part = 2 * static_cast<int64_t>(blockIdx.x) + (at.index == 0 ? 0 : 1);
+                bf16* ctx = p.ctx + ((at.b * p.tokens + t) * p.q_heads + at.h * p.group + g) * D;
+                float* part_o = p.part_o + part * D * p.part_rows + part_row * 4;
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-                float o[32];
-                if (busy) {
-                    tmem_load32(t_o + c * 32, o);
-                    if (flagged != 0u) {
-                        add_set_aside(o, c * 32);
-                        __syncwarp();
+                for (int c = 0; c < D; c += 64) {
+                    float o[64];
+                    tmem_load_begin<64>(t_o + c, o);
+                    tmem_load_end<64>(o);
+                    if (joins) {
+                        float o1[64];
+                        tmem_load_begin<64>(t_o + D + c, o1);
+                        tmem_load_end<64>(o1);
+#pragma unroll
+                        for (int j = 0; j < 64; ++j) {
+                            o[j] = __fmaf_rn(o1[j], f1, o[j] * f0);
+                        }
                     }
+                    if (inside && whole) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            U8 x;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                x.r[e] = valid ? pack_bf16x2(o[16 * j + 2 * e] * inv, o[16 * j + 2 * e + 1] * inv) : 0u;
+                            }
+                            st_stream32(ctx + c + 16 * j, x);
+                        }
+                    } else if (inside) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            st_v4(part_o + (c + 4 * j) * static_cast<int64_t>(p.part_rows),
+                                  make_uint4(__float_as_uint(o[4 * j]), __float_as_uint(o[4 * j + 1]),
+                                             __float_as_uint(o[4 * j + 2]), __float_as_uint(o[4 * j + 3])));
+                        }
+                    }
+                    __syncwarp();  // the next tensor-memory load is warp-collective
                 }
-                if (joins) {
-                    if (w == 1 && busy) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            s_exchange[row * 33 + j] = o[j];
-                        }
-                    }
-                    named_barrier(3, 256);
-                    if (w == 0 && busy) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            o[j] = __fmaf_rn(s_exchange[row * 33 + j], f1, o[j] * f0);
-                        }
-                    }
-                    named_barrier(3, 256);
-                }
-                if (whole && !(joins && w == 1) && busy) {
-                    // The warp's 32 rows of 64 bytes change hands in shared memory, so that four lanes write a row.
-                    const float scale = valid ? inv : 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t x[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            x[e] = valid ? pack_bf16x2(o[8 * j + 2 * e] * scale, o[8 * j + 2 * e + 1] * scale) : 0u;
-                        }
-                        stage[lane * 4 + (j ^ (lane >> 1 & 3))] = make_uint4(x[0], x[1], x[2], x[3]);
-                    }
-                    __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int from = i * 8 + (lane >> 2);
-                        const uint4 x = stage[from * 4 + ((lane & 3) ^ (from >> 1 & 3))];
-                        if (places[i] >= 0) {
-                            st_v4(p.ctx + places[i] + c * 32 + (lane & 3) * 8, x);
-                        }
-                    }
-                } else if (!whole && inside && !(joins && w == 1)) {
-                    float* dst = p.part_o + (part * D + c * 32) * p.part_rows + item_row * 4;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        st_v4(dst + 4 * j * p.part_rows,
-                              make_uint4(__float_as_uint(o[4 * j]), __float_as_uint(o[4 * j + 1]),
-                                         __float_as_uint(o[4 * j + 2]), __float_as_uint(o[4 * j + 3])));
-                    }
-                }
-                __syncwarp();  // the next tensor-memory load is warp-collective
-            }
-            if (inside && !(joins && w == 1)) {
-                if (!whole) {
-                    p.part_ml[part * p.part_rows + item_row] = make_float2(scaled_top, sum);
-                } else if (p.stats != nullptr) {
+                if (inside && !whole) {
+                    p.part_ml[part * p.part_rows + part_row] = make_float2(scaled_top, sum);
+                } else if (inside && p.stats != nullptr) {
                     p.stats[((at.b * p.kv_heads + at.h) * p.tokens + t) * p.group + g] =
                         valid ? make_float2(scaled_top == -INFINITY ? 0.0f : scaled_top, inv) : make_float2(0.0f, 0.0f);
                 }
             }
             tc_fence_before();
-            if (kPair && chains == 2) {
-                named_barrier(3, 256);  // both chains are done with the flags
+            if (chains == 2 && (joins || (kPair && hides))) {
+                named_barrier(3, 256);  // the second chain's O has been read; both are done with the flags
             } else if (hides) {
                 named_barrier(1 + w, 128);
             }
-            advance(p, at, count, tiles);
         }
     }
     tc_fence_before();
@@ -838,16 +865,15 @@ __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAt
     __shared__ int64_t s_places[32];
     grid_dependency_begin();
     const int cut = static_cast<int>(blockIdx.x) + 1;
-    const int64_t total = *p.line;
     const int4 where = p.cuts[cut];
-    const Cuts cuts(total, static_cast<unsigned>(ctas));
-    const int64_t begin = cuts.begin(cut);
-    const int64_t first = begin - where.w;  // the item's first tile on the line
+    const Cuts cuts(*p.line, ctas);
+    const int first = cuts.begin(cut) - where.w;  // the item's first tile on the line
     if (cuts.empty(cut) || where.w == 0 || cuts.begin(cut - 1) > first) {
         return;
     }
-    const ItemRange r = item_range(p, where.x, where.y);
-    const int64_t last = cuts.of(first + item_tiles<kKeys>(r) - 1);  // parts before it are not empty
+    const ItemRange r = item_range(p, static_cast<int>(committed_rows(p, where.x)),
+                                   static_cast<int>(valid_queries(p, where.x)), where.y);
+    const int last = cuts.of(first + item_tiles<kKeys>(r) - 1);  // parts before it are not empty
     const int lane = threadIdx.x & 31;
     const int warp = threadIdx.x >> 5;
     const int row = static_cast<int>(blockIdx.y) * 32 + lane;
@@ -861,8 +887,8 @@ __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAt
     float o[kPieces][4] = {};
     if (inside) {
 #pragma unroll 2
-        for (int64_t c = cut - 1; c <= last; ++c) {
-            const int64_t slot = 2 * c + (cuts.begin(c) >= first ? 0 : 1);
+        for (int c = cut - 1; c <= last; ++c) {
+            const int64_t slot = 2 * static_cast<int64_t>(c) + (cuts.begin(c) >= first ? 0 : 1);
             const float2 ml = p.part_ml[slot * p.part_rows + row];
             float4 x[kPieces];
 #pragma unroll
@@ -954,13 +980,13 @@ __device__ __forceinline__ KeyRange key_range(const CacheAttentionParams& p, int
 }
 
 // Products of one head of a sequence: whole rows of query tiles for the key tiles that begin in committed rows.
-__device__ __forceinline__ int64_t head_products(const CacheAttentionParams& p, const KeyRange& r) {
+__device__ __forceinline__ int head_products(const CacheAttentionParams& p, const KeyRange& r) {
     if (r.valid == 0) {
         return 0;
     }
     int kt = r.len / 128 + 1;
     kt = kt < r.key_tiles ? kt : r.key_tiles;
-    int64_t sum = int64_t{kt} * r.q_tiles;
+    int sum = kt * r.q_tiles;
     for (; kt < r.key_tiles; ++kt) {
         sum += r.q_tiles - r.first(kt, p.tile_tokens);
     }
@@ -972,10 +998,10 @@ struct UnitWalk {
     int b;
     int kt;
     int h;
-    int q;          // first query tile of the current segment, counted from the unit's first
-    int64_t left;
-    int64_t begin;  // the current segment's place on the line
-    int64_t total;
+    int q;       // first query tile of the current segment, counted from the unit's first
+    int left;
+    int begin;   // the current segment's place on the line
+    int total;
     uint32_t products;  // before the current segment
     int index;
 };
@@ -1034,44 +1060,40 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
     fence_proxy_async_smem();
     grid_dependency_begin();
     if (warp == 0) {
-        int64_t total = 0;
+        const int heads = static_cast<int>(p.kv_heads);
+        int total = 0;
         for (int64_t b = lane; b < p.batch; b += 32) {
-            total += head_products(p, key_range(p, b)) * p.kv_heads;
+            total += head_products(p, key_range(p, b)) * heads;
         }
-        for (int offset = 16; offset > 0; offset >>= 1) {
-            total += __shfl_xor_sync(0xffffffffu, total, offset);
-        }
-        const Cuts cuts(total, gridDim.x);
-        const int64_t begin = cuts.begin(blockIdx.x);
-        const int64_t end = cuts.begin(blockIdx.x + 1);
+        total = __reduce_add_sync(0xffffffffu, total);
+        const Cuts cuts(total, static_cast<int>(gridDim.x));
+        const int begin = cuts.begin(static_cast<int>(blockIdx.x));
+        const int end = cuts.begin(static_cast<int>(blockIdx.x) + 1);
         if (lane == 0) {
             UnitWalk w{};
             w.total = total;
             s_walk = w;
         }
         __syncwarp();
-        int64_t before = 0;
+        int before = 0;
         for (int64_t b0 = 0; b0 < p.batch && begin < end; b0 += 32) {
             const KeyRange r = b0 + lane < p.batch ? key_range(p, b0 + lane) : KeyRange{};
-            const int64_t mine = head_products(p, r) * p.kv_heads;
-            int64_t sum = mine;
+            const int mine = head_products(p, r) * heads;
+            int sum = mine;
             for (int offset = 1; offset < 32; offset <<= 1) {
-                const int64_t other = __shfl_up_sync(0xffffffffu, sum, offset);
+                const int other = __shfl_up_sync(0xffffffffu, sum, offset);
                 sum += lane >= offset ? other : 0;
             }
-            const int64_t lo = before + sum - mine;
+            const int lo = before + sum - mine;
             if (begin >= lo && begin < lo + mine) {
                 // Order within a sequence: key tile, head, query tile.
-                int64_t rest = begin - lo;
-                int kt = 0;
-                const int64_t whole = int64_t{r.q_tiles} * p.kv_heads;
-                int64_t skip = rest / whole;
-                const int64_t most = r.len / 128 < r.key_tiles - 1 ? r.len / 128 : r.key_tiles - 1;
-                skip = skip < most ? skip : most;
-                kt = static_cast<int>(skip);
-                rest -= skip * whole;
+                int rest = begin - lo;
+                const int whole = r.q_tiles * heads;
+                const int most = r.len / 128 < r.key_tiles - 1 ? r.len / 128 : r.key_tiles - 1;
+                int kt = rest / whole < most ? rest / whole : most;
+                rest -= kt * whole;
                 for (;;) {
-                    const int64_t here = (r.q_tiles - r.first(kt, p.tile_tokens)) * p.kv_heads;
+                    const int here = (r.q_tiles - r.first(kt, p.tile_tokens)) * heads;
                     if (rest < here) {
                         break;
                     }
@@ -1082,8 +1104,8 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
                 UnitWalk w;
                 w.b = static_cast<int>(b0 + lane);
                 w.kt = kt;
-                w.h = static_cast<int>(rest / each);
-                w.q = static_cast<int>(rest % each);
+                w.h = rest / each;
+                w.q = rest % each;
                 w.left = end - begin;
                 w.begin = begin;
                 w.total = total;
@@ -1135,7 +1157,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
             while (at.left > 0) {
                 const int q0 = r.first(at.kt, p.tile_tokens);
                 const int tiles = r.q_tiles - q0;
-                const int count = static_cast<int>(tiles - at.q < at.left ? tiles - at.q : at.left);
+                const int count = tiles - at.q < at.left ? tiles - at.q : at.left;
                 const uint32_t ks = static_cast<uint32_t>(at.index) % L::kKeySlots;
                 const uint32_t kr = static_cast<uint32_t>(at.index) / L::kKeySlots;
                 if (kr > 0) {
@@ -1166,7 +1188,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
             const uint32_t idesc = idesc_bf16_f32(chunks * 32);
             while (at.left > 0) {
                 const int tiles = r.q_tiles - r.first(at.kt, p.tile_tokens);
-                const int count = static_cast<int>(tiles - at.q < at.left ? tiles - at.q : at.left);
+                const int count = tiles - at.q < at.left ? tiles - at.q : at.left;
                 const uint32_t ks = static_cast<uint32_t>(at.index) % L::kKeySlots;
                 wait(bar_k_full + ks, static_cast<uint32_t>(at.index) / L::kKeySlots & 1u);
                 for (int i = 0; i < count; ++i) {
@@ -1202,7 +1224,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
         while (at.left > 0) {
             const int q0 = r.first(at.kt, p.tile_tokens);
             const int tiles = r.q_tiles - q0;
-            const int count = static_cast<int>(tiles - at.q < at.left ? tiles - at.q : at.left);
+            const int count = tiles - at.q < at.left ? tiles - at.q : at.left;
             const int key = at.kt * 128 + row;
             float part[4] = {};
             bool mine = false;
@@ -1274,13 +1296,12 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
                     }
                 } else {
                     // A cut went through the unit: whoever leaves the last of its parts adds them up in their order.
-                    const int64_t first = at.begin - at.q;
-                    const int64_t end = first + tiles;
+                    const int first = at.begin - at.q;
                     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (at.index == 0 ? 0 : 1);
                     p.part_sums[slot * 128 + row] = sum;
-                    const Cuts cuts(at.total, gridDim.x);
-                    const int64_t c0 = cuts.of(first);
-                    const int64_t c1 = cuts.of(end - 1);  // parts between them are not empty
+                    const Cuts cuts(at.total, static_cast<int>(gridDim.x));
+                    const int c0 = cuts.of(first);
+                    const int c1 = cuts.of(first + tiles - 1);  // parts between them are not empty
                     __threadfence();
                     named_barrier(1 + w, 128);
                     if (row == 0) {
@@ -1290,8 +1311,8 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
                     if (s_last[w] != 0u) {
                         __threadfence();
                         float all = 0.0f;
-                        for (int64_t c = c0; c <= c1; ++c) {
-                            all += __ldcg(p.part_sums + (2 * c + (cuts.begin(c) >= first ? 0 : 1)) * 128 + row);
+                        for (int c = c0; c <= c1; ++c) {
+                            all += __ldcg(p.part_sums + (2 * int64_t{c} + (cuts.begin(c) >= first ? 0 : 1)) * 128 + row);
                         }
                         if (seen) {
                             *out += all;
@@ -1313,6 +1334,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
 
 // The tiling of a call, and where its scratch lies (offsets in bytes; `bytes` in all).
 struct Plan {
+    bool fits;         // the lines' lengths stay below 2^31
     bool pair;         // two row tiles on each K and V tile
     int ctas;
     int tile_tokens;
@@ -1340,6 +1362,8 @@ Plan plan(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads, int6
     pl.part_rows = pl.pair ? 2 * kBM : static_cast<int>((tokens < pl.tile_tokens ? tokens : pl.tile_tokens) * group);
     const int64_t most = batch * pl.row_tiles * kv_heads * runtime::ceil_div(capacity, keys);  // of the line's tiles
     pl.ctas = static_cast<int>(most < runtime::sm_count() ? most : runtime::sm_count());
+    const int64_t products = batch * kv_heads * runtime::ceil_div(capacity, 128) * runtime::ceil_div(tokens, pl.tile_tokens);
+    pl.fits = most < (int64_t{1} << 31) && products < (int64_t{1} << 31);
     const auto up = [](int64_t n) { return (n + 127) / 128 * 128; };
     pl.cuts = 128;  // after the line's length
     pl.ml = pl.cuts + up(pl.ctas * static_cast<int64_t>(sizeof(int4)));
@@ -1347,7 +1371,6 @@ Plan plan(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads, int6
     pl.stats = pl.o + 2 * pl.ctas * pl.part_rows * head_dim * static_cast<int64_t>(sizeof(float));
     pl.bytes = pl.stats;
     if (with_stats) {
-        const int64_t products = batch * kv_heads * runtime::ceil_div(capacity, 128) * runtime::ceil_div(tokens, pl.tile_tokens);
         pl.weight_ctas = static_cast<int>(products < runtime::sm_count() ? products : runtime::sm_count());
         pl.sums = pl.stats + up(batch * tokens * q_heads * static_cast<int64_t>(sizeof(float2)));
         // The parts of the units, then the tickets.
@@ -1462,6 +1485,7 @@ int run_attention(const char* op, CacheAttentionParams& p, int64_t head_dim, voi
                   cudaStream_t s) {
     const std::string name(op);
     const Plan pl = plan(p.batch, p.tokens, p.q_heads, p.kv_heads, head_dim, p.capacity, p.weights != nullptr);
+    CPPINF_REQUIRE(pl.fits, CPPINF_ERR_OVERFLOW, name + " sizes exceed the kernels' index range.");
     CPPINF_REQUIRE(scratch && scratch_bytes >= pl.bytes, CPPINF_ERR_INVALID_ARGUMENT,
                    name + " requires a scratch of cppinf_cache_attention_scratch_bytes.");
     CPPINF_REQUIRE(runtime::aligned16(scratch), CPPINF_ERR_UNSUPPORTED, name + " requires a 16-byte aligned scratch.");
@@ -1472,7 +1496,7 @@ int run_attention(const char* op, CacheAttentionParams& p, int64_t head_dim, voi
     p.row_tiles = pl.row_tiles;
     p.q_box_tokens = static_cast<int>(p.tokens < pl.tile_tokens ? p.tokens : pl.tile_tokens);
     p.part_rows = pl.part_rows;
-    p.line = reinterpret_cast<int64_t*>(base);
+    p.line = reinterpret_cast<int*>(base);
     p.cuts = reinterpret_cast<int4*>(base + pl.cuts);
     p.part_ml = reinterpret_cast<float2*>(base + pl.ml);
     p.part_o = reinterpret_cast<float*>(base + pl.o);
@@ -1523,7 +1547,8 @@ int64_t cppinf_cache_attention_scratch_bytes(int64_t batch, int64_t tokens, int6
     if (batch == 0 || tokens == 0) {
         return 0;
     }
-    return plan(batch, tokens, q_heads, kv_heads, head_dim, capacity, with_weights != 0).bytes;
+    const Plan pl = plan(batch, tokens, q_heads, kv_heads, head_dim, capacity, with_weights != 0);
+    return pl.fits ? pl.bytes : -1;
 }
 
 int cppinf_tree_attention(const void* q, const void* k_cache, const int64_t* k_strides, const void* v_cache,
@@ -1549,8 +1574,8 @@ int cppinf_tree_attention(const void* q, const void* k_cache, const int64_t* k_s
     if (const int st = check_cache(kOp, v_cache, v_strides); st != CPPINF_OK) {
         return st;
     }
-    CPPINF_REQUIRE(rt::aligned16(q) && rt::aligned16(ctx), CPPINF_ERR_UNSUPPORTED,
-                   "tree_attention requires 16-byte aligned queries and contexts.");
+    CPPINF_REQUIRE(rt::aligned16(q) && (reinterpret_cast<std::uintptr_t>(ctx) & 31u) == 0, CPPINF_ERR_UNSUPPORTED,
+                   "tree_attention requires 16-byte aligned queries and 32-byte aligned contexts.");
     CacheAttentionParams p{};
     p.q = static_cast<const bf16*>(q);
     p.k = static_cast<const bf16*>(k_cache);
@@ -1593,8 +1618,8 @@ int cppinf_decoder_attention_weights(const void* q, const void* k_cache, const i
     if (const int st = check_cache(kOp, v_cache, v_strides); st != CPPINF_OK) {
         return st;
     }
-    CPPINF_REQUIRE(rt::aligned16(q) && rt::aligned16(ctx), CPPINF_ERR_UNSUPPORTED,
-                   "decoder_attention_weights requires 16-byte aligned queries and contexts.");
+    CPPINF_REQUIRE(rt::aligned16(q) && (reinterpret_cast<std::uintptr_t>(ctx) & 31u) == 0, CPPINF_ERR_UNSUPPORTED,
+                   "decoder_attention_weights requires 16-byte aligned queries and 32-byte aligned contexts.");
     CacheAttentionParams p{};
     p.q = static_cast<const bf16*>(q);
     p.k = static_cast<const bf16*>(k_cache);

@@ -273,8 +273,8 @@ CPPINF_API int cppinf_decoder_attention_tc(const void* q, const void* k_cache, c
  *
  * A cache is a K and a V tensor of [batch, capacity, kv_heads, head_dim] whose rows of head_dim elements are dense;
  * `k_strides` / `v_strides` are HOST arrays of 3 element strides {batch, row, head}, so views of a larger cache (one
- * layer of many, K and V interleaved) are read and written in place. Strides must be multiples of 16 bytes and the
- * base addresses 16-byte aligned. `lengths` (DEVICE int64, one per sequence) are the committed rows; the new tokens of
+ * layer of many, K and V interleaved) are read and written in place. Strides must be positive multiples of 16 bytes,
+ * the base addresses 16-byte aligned, `ctx` 32-byte aligned. `lengths` (DEVICE int64, one per sequence) are the committed rows; the new tokens of
  * a call occupy the rows after them. They are read on the device, so a captured call follows them from replay to
  * replay; they cannot be refused there, so a length is taken as 0 below 0 and as the capacity above it, and a new token
  * whose row would lie past the capacity counts as padding. Query head h reads key-value head
