@@ -150,9 +150,11 @@ struct Tiling {
     static constexpr uint32_t kFlags = kMl + 128 * 8;               // [2][16]
     static constexpr uint32_t kBars = kFlags + 2 * 16 * 4;
     static constexpr std::size_t kBytes = 1024 + kBars + 256;
-    // Tensor memory columns: the chains' S (P over it), then their O.
-    static constexpr uint32_t kTmemO = kStreams * kKeys;
-    static_assert(kDepth >= 1 && kStreams * (kKeys + D) <= 512, "tensor memory has 512 columns");
+    // A chain goes in steps of 64 keys with an S for each of two steps (P over it): while one step's softmax runs, the
+    // step before it is multiplied with V and the step after it with Q. Tensor memory: the chains' S, then their O.
+    static constexpr int kSteps = kKeys / 64;  // of a key tile
+    static constexpr uint32_t kTmemO = kStreams * 128;
+    static_assert(kDepth >= 1 && kStreams * (128 + D) <= 512, "tensor memory has 512 columns");
 
     // The slot of a ring's n-th K or V tile, and the parity of its barriers' phase.
     __device__ static __forceinline__ int k_slot(int ring, uint32_t n) { return ring * 2 * kDepth + static_cast<int>(n % kDepth); }
@@ -279,12 +281,11 @@ __device__ __forceinline__ float largest(const float (&x)[N], float top) {
     return fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
 }
 
-// P of N keys, 2^(x factor + offset), stored as bf16 pairs at `taddr`; returns their sum in f32.
-template <int N>
-__device__ __forceinline__ float probabilities(const float (&x)[N], float2 factor, float2 offset, uint32_t taddr) {
+// P of 64 keys, 2^(x factor + offset), stored as bf16 pairs at `taddr`; returns their sum in f32.
+__device__ __forceinline__ float probabilities(const float (&x)[64], float2 factor, float2 offset, uint32_t taddr) {
     float2 sums[2] = {};
 #pragma unroll
-    for (int c = 0; c < N / 32; ++c) {
+    for (int c = 0; c < 2; ++c) {
         uint32_t packed[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
@@ -319,7 +320,6 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
     using L = Tiling<D, kPair>;
     constexpr int kStreams = L::kStreams;
     constexpr int kKeys = L::kKeys;
-    constexpr int kHalf = kKeys / 2;
     extern __shared__ __align__(16) unsigned char raw[];
     unsigned char* sm = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
     uint32_t* s_mask = reinterpret_cast<uint32_t*>(sm + L::kMask);
@@ -330,9 +330,9 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
     uint64_t* bar_empty = bars + L::kSlots;       // [slots] its products are done
     uint64_t* bar_q_full = bars + 2 * L::kSlots;
     uint64_t* bar_q_empty = bar_q_full + 1;
-    uint64_t* bar_s = bar_q_empty + 1;            // [chains] S is complete
-    uint64_t* bar_p = bar_s + kStreams;           // [chains][2] half of P is written
-    uint64_t* bar_o = bar_p + 2 * kStreams;       // [chains] the segment's O is complete
+    uint64_t* bar_s = bar_q_empty + 1;            // [chains][2] S is complete
+    uint64_t* bar_p = bar_s + 2 * kStreams;       // [chains][2] P is written
+    uint64_t* bar_pv = bar_p + 2 * kStreams;      // [chains][2] its product with V is complete
     __shared__ uint32_t s_tmem;
     __shared__ uint32_t s_stop;
     __shared__ Walk s_walk;
@@ -349,10 +349,12 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
         mbar_init(bar_q_full, 1);
         mbar_init(bar_q_empty, kStreams);
         for (int w = 0; w < kStreams; ++w) {
-            mbar_init(bar_s + w, 1);
+            mbar_init(bar_s + 2 * w, 1);
+            mbar_init(bar_s + 2 * w + 1, 1);
             mbar_init(bar_p + 2 * w, 4);
             mbar_init(bar_p + 2 * w + 1, 4);
-            mbar_init(bar_o + w, 1);
+            mbar_init(bar_pv + 2 * w, 1);
+            mbar_init(bar_pv + 2 * w + 1, 1);
         }
     }
     if (warp == 2) {
@@ -444,12 +446,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
         chains = kStreams == 1 ? 1 : kPair ? (r.first + p.tile_tokens < p.tokens ? 2 : 1) : (count < 2 ? count : 2);
         return true;
     };
-    // A row of S takes 128 registers: with two chains the control warps give up what they do not need of the 168
-    // registers a thread that 384 threads start with (128 * 88 + 256 * 208 = 384 * 168).
     if (warp < 4) {
-        if constexpr (kStreams == 2) {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        }
         if (warp == 0 && lane == 0) {  // ---- loads
             uint32_t k_tiles[L::kRings] = {};  // loaded so far
             uint32_t v_tiles[L::kRings] = {};
@@ -510,7 +507,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             }
         } else if ((warp == 1 || (warp == 3 && kStreams == 2)) && lane == 0) {  // ---- matrix products of chain w
             const int w = warp >> 1;
-            constexpr uint32_t s_idesc = idesc_bf16_f32(kKeys);
+            constexpr uint32_t s_idesc = idesc_bf16_f32(64);
             constexpr uint32_t o_idesc = idesc_bf16_f32_bmn(D);
             const unsigned char* q = sm + L::kQ + (kPair ? w * L::kAtoms * L::kQAtom : 0);
             const int ring = kPair ? 0 : w;
@@ -519,20 +516,27 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 wait(bar_full + slot, L::parity(tile));
                 tc_fence_after();
             };
-            const auto scores = [&](uint32_t tile) {
+            // S of the chain's `step`-th 64 keys of the segment.
+            const auto scores = [&](int step) {
+                const uint32_t tile = n + static_cast<uint32_t>(step / L::kSteps);
+                const int part = step % L::kSteps;
                 const int slot = L::k_slot(ring, tile);
-                const unsigned char* k = sm + L::kRing + slot * L::kSlot;
-                landed(slot, tile);
+                const unsigned char* k = sm + L::kRing + slot * L::kSlot + part * (64 * 128);
+                if (part == 0) {
+                    landed(slot, tile);
+                }
 #pragma unroll
                 for (int i = 0; i < D / kUmmaK; ++i) {
                     const uint32_t in = static_cast<uint32_t>(i & 3) * 32u;
-                    umma_bf16(tmem + w * kKeys, smem_desc_sw128(q, (i >> 2) * L::kQAtom + in),
+                    umma_bf16(tmem + w * 128 + (step & 1) * 64, smem_desc_sw128(q, (i >> 2) * L::kQAtom + in),
                               smem_desc_sw128(k, (i >> 2) * L::kKvAtom + in), s_idesc, i > 0 ? 1u : 0u);
                 }
-                umma_commit(bar_s + w);
-                umma_commit(bar_empty + slot);
+                umma_commit(bar_s + 2 * w + (step & 1));
+                if (part == L::kSteps - 1) {
+                    umma_commit(bar_empty + slot);
+                }
             };
-            uint32_t p_phase = 0;
+            uint32_t p_phase = 0;  // a bit for each of the chain's two S
             for (; segment(); advance(p, at, count, tiles)) {
                 wait(bar_q_full, static_cast<uint32_t>(at.index) & 1u);
                 tc_fence_after();
@@ -546,52 +550,63 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                     umma_commit(bar_q_empty);
                     continue;
                 }
-                const int first = kPair ? 0 : w;
-                scores(n);
-                for (int i = first; i < count; i += L::kStep, ++n) {
-                    const bool more = i + L::kStep < count;
-                    if (!more) {
-                        umma_commit(bar_q_empty);
-                    }
-                    const int slot = L::v_slot(ring, n);
+                const int mine = kPair ? count : (count - w + kStreams - 1) / kStreams;  // the chain's key tiles
+                const int steps = mine * L::kSteps;
+                scores(0);
+                if (steps > 1) {
+                    scores(1);
+                }
+                if (steps <= 2) {
+                    umma_commit(bar_q_empty);
+                }
+                for (int step = 0; step < steps; ++step) {
+                    const uint32_t tile = n + static_cast<uint32_t>(step / L::kSteps);
+                    const int part = step % L::kSteps;
+                    const int slot = L::v_slot(ring, tile);
                     const unsigned char* v = sm + L::kRing + slot * L::kSlot;
-                    landed(slot, n);
+                    if (part == 0) {
+                        landed(slot, tile);
+                    }
+                    wait(bar_p + 2 * w + (step & 1), p_phase >> (step & 1) & 1u);
+                    p_phase ^= 1u << (step & 1);
+                    tc_fence_after();
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        wait(bar_p + 2 * w + half, p_phase);
-                        tc_fence_after();
-#pragma unroll
-                        for (int j = half * (kHalf / kUmmaK); j < (half + 1) * (kHalf / kUmmaK); ++j) {
-                            umma_bf16_ta(tmem + L::kTmemO + w * D, tmem + w * kKeys + j * 8,
-                                         smem_desc_sw128_mn(v, j * 2048u, L::kKvAtom), o_idesc,
-                                         (i > first || j > 0) ? 1u : 0u);
+                    for (int j = 0; j < 4; ++j) {
+                        umma_bf16_ta(tmem + L::kTmemO + w * D, tmem + w * 128 + (step & 1) * 64 + j * 8,
+                                     smem_desc_sw128_mn(v, (part * 4 + j) * 2048u, L::kKvAtom), o_idesc,
+                                     (step > 0 || j > 0) ? 1u : 0u);
+                    }
+                    umma_commit(bar_pv + 2 * w + (step & 1));
+                    if (part == L::kSteps - 1) {
+                        umma_commit(bar_empty + slot);
+                    }
+                    if (step + 2 < steps) {
+                        scores(step + 2);
+                        if (step + 3 == steps) {
+                            umma_commit(bar_q_empty);
                         }
                     }
-                    p_phase ^= 1u;
-                    umma_commit(bar_empty + slot);
-                    if (more) {
-                        scores(n + 1);
-                    } else {
-                        umma_commit(bar_o + w);
-                    }
                 }
+                n += static_cast<uint32_t>(mine);
             }
         }
     } else {  // ---- softmax: chain w, one thread per row
-        if constexpr (kStreams == 2) {
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        }
         const int w = (warp - 4) >> 2;
         const int row = tid & 127;
         const int g = row % p.group;
         const int token_in_tile = row / p.group;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t t_s = tmem + lanes + w * kKeys;
+        const uint32_t t_s = tmem + lanes + w * 128;
         const uint32_t t_o = tmem + lanes + L::kTmemO + w * D;
         const float c2 = 1.4426950408889634f / sqrtf(static_cast<float>(D));
-        uint32_t s_phase = 0;
-        uint32_t o_phase = 0;
-        uint32_t n = 0;  // tiles of the chain before the current one
+        uint32_t s_phase = 0;  // a bit for each of the chain's two S
+        uint32_t n = 0;        // tiles of the chain before the segment
+        // Waits until a step, the last one whose S has been taken or the one before it, has reached O. Each S of the two
+        // has a barrier for this: its last phase but one is over, since S was complete after it.
+        const auto settled = [&](int step) {
+            wait(bar_pv + 2 * w + (step & 1), (s_phase >> (step & 1) & 1u) ^ 1u);
+            tc_fence_after();
+        };
         for (; segment(); advance(p, at, count, tiles)) {
             if (w >= chains) {
                 n += kPair ? static_cast<uint32_t>(count) : 0u;
@@ -638,22 +653,27 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             }
             float top = -INFINITY;  // the maximum that P is taken against, in units of S
             float sum = 0.0f;
-            for (int i = kPair ? 0 : w; i < count; i += L::kStep, ++n) {
-                const int key0 = (at.tile + i) * kKeys;
-                const bool partial = key0 + kKeys > r.full_end;
-                wait(bar_s + w, s_phase);
-                s_phase ^= 1u;
+            const int mine = kPair ? count : (count - w + kStreams - 1) / kStreams;  // the chain's key tiles
+            for (int step = 0; step < mine * L::kSteps; ++step) {
+                const uint32_t tile = n + static_cast<uint32_t>(step / L::kSteps);
+                const int tile0 = (at.tile + (kPair ? 0 : w) + step / L::kSteps * L::kStep) * kKeys;
+                const int key0 = tile0 + step % L::kSteps * 64;
+                const bool partial = tile0 + kKeys > r.full_end;
+                const uint32_t t_x = t_s + (step & 1) * 64;
+                wait(bar_s + 2 * w + (step & 1), s_phase >> (step & 1) & 1u);
+                s_phase ^= 1u << (step & 1);
                 tc_fence_after();
-                if (partial) {  // V rows that nobody sees become zeros, values that are not finite are set aside
-                    // S is complete, so the chain's product before is, and the slot's tile before this one has landed.
-                    const int slot = L::v_slot(kPair ? 0 : w, n);
-                    wait(bar_full + slot, L::parity(n));
+                if (partial && step % L::kSteps == 0) {
+                    // V rows that nobody sees become zeros, values that are not finite are set aside. S is complete, so
+                    // the chain's product two steps before is, and the slot's tile before this one has landed.
+                    const int slot = L::v_slot(kPair ? 0 : w, tile);
+                    wait(bar_full + slot, L::parity(tile));
                     unsigned char* v = sm + L::kRing + slot * L::kSlot;
                     const int sharing = kPair ? chains : 1;  // chains that read this tile
                     for (int u = (sharing == 2 ? w * 128 : 0) + row; u < kKeys * L::kAtoms; u += 128 * sharing) {
                         const int key = u % kKeys;  // this thread's: 64 dims of a row
                         uint4* at16 = reinterpret_cast<uint4*>(v + u / kKeys * L::kKvAtom + key * 128);
-                        if (key0 + key >= r.kv_end) {
+                        if (tile0 + key >= r.kv_end) {
 #pragma unroll
                             for (int ch = 0; ch < 8; ++ch) {
                                 at16[ch ^ (key & 7)] = make_uint4(0u, 0u, 0u, 0u);
@@ -672,7 +692,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                                 at16[ch] = make_uint4(finite_pair(x.x), finite_pair(x.y), finite_pair(x.z),
                                                       finite_pair(x.w));
                             }
-                            const int bit = key0 + key - part0;
+                            const int bit = tile0 + key - part0;
                             atomicOr(&s_flags[w * 16 + (bit >> 5)], 1u << (bit & 31));
                         }
                     }
@@ -681,26 +701,17 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                         named_barrier(3, 256);
                     }
                 }
-                float2 factor = make_float2(c2, c2);
-                float2 offset = make_float2(0.0f, 0.0f);
-                float x0[kHalf];
-                float x1[kHalf];
                 if (busy) {
-                    tmem_load_begin<kHalf>(t_s, x0);
-                    tmem_load_end<kHalf>(x0);
-                    tmem_load_begin<kHalf>(t_s + kHalf, x1);
+                    float x[64];
+                    tmem_load_begin<64>(t_x, x);
+                    tmem_load_end<64>(x);
                     if (partial) {
-                        hide(x0, bits_row, key0, r.len, limit);
+                        hide(x, bits_row, key0, r.len, limit);
                     }
-                    float new_top = largest(x0, top);
-                    tmem_load_end<kHalf>(x1);
-                    if (partial) {
-                        hide(x1, bits_row, key0 + kHalf, r.len, limit);
-                    }
-                    new_top = largest(x1, new_top);
-                    const bool first = i < L::kStep;
-                    const bool grown = first || (new_top - top) * c2 > 8.0f;
-                    if (!first && __any_sync(0xffffffffu, grown)) {
+                    const float new_top = largest(x, top);
+                    const bool grown = step == 0 || (new_top - top) * c2 > 8.0f;
+                    if (step > 0 && __any_sync(0xffffffffu, grown)) {
+                        settled(step - 1);
                         const float f = grown ? exp2_approx((top - new_top) * c2) : 1.0f;
                         sum *= f;
 #pragma unroll 1
@@ -716,28 +727,17 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                     }
                     top = grown ? new_top : top;
                     const float shift = top == -INFINITY ? 0.0f : top * c2;
-                    offset = make_float2(-shift, -shift);
-                    sum += probabilities(x0, factor, offset, t_s);
+                    sum += probabilities(x, make_float2(c2, c2), make_float2(-shift, -shift), t_x);
                     tmem_store_wait();
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(bar_p + 2 * w);
-                }
-                if (busy) {
-                    sum += probabilities(x1, factor, offset, t_s + kHalf / 2);
-                    tmem_store_wait();
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(bar_p + 2 * w + 1);
+                    mbar_arrive(bar_p + 2 * w + (step & 1));
                 }
             }
-            wait(bar_o + w, o_phase);
-            o_phase ^= 1u;
-            tc_fence_after();
+            n += static_cast<uint32_t>(mine);
+            settled(mine * L::kSteps - 1);
             if (hides) {
                 named_barrier(1 + w, 128);  // the flags of all the chain's threads
                 uint32_t flagged = 0u;
