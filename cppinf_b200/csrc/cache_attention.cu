@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
     __shared__ Walk s_walk;
 
     const int tid = threadIdx.x;
-    const int warp = tid >> 5;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int lane = tid & 31;
     if (tid == 0) {
         s_stop = 0u;
@@ -447,19 +447,22 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
         return true;
     };
     if (warp < 4) {
-        if (warp == 0 && lane == 0) {  // ---- loads
+        if (warp == 0) {  // ---- loads
             uint32_t k_tiles[L::kRings] = {};  // loaded so far
             uint32_t v_tiles[L::kRings] = {};
             const auto load = [&](const CUtensorMap* map, int slot, uint32_t n, int tile) {
                 if (n >= static_cast<uint32_t>(L::kDepth)) {
                     wait(bar_empty + slot, L::parity(n) ^ 1u);
                 }
-                mbar_arrive_expect_tx(bar_full + slot, L::kSlot);
-                unsigned char* dst = sm + L::kRing + slot * L::kSlot;
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(bar_full + slot, L::kSlot);
+                    unsigned char* dst = sm + L::kRing + slot * L::kSlot;
 #pragma unroll
-                for (int a = 0; a < L::kAtoms; ++a) {
-                    tma_load_4d(dst + a * L::kKvAtom, map, a * 64, at.h, tile * kKeys, at.b, bar_full + slot);
+                    for (int a = 0; a < L::kAtoms; ++a) {
+                        tma_load_4d(dst + a * L::kKvAtom, map, a * 64, at.h, tile * kKeys, at.b, bar_full + slot);
+                    }
                 }
+                __syncwarp();
             };
             // Tile i of the segment; a tile that does not exist is left out.
             const auto load_k = [&](int i) {
@@ -482,14 +485,17 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 }
                 const int q_tiles = kPair ? chains : 1;
                 const uint32_t box = static_cast<uint32_t>(p.q_box_tokens * p.group) * 128u;
-                mbar_arrive_expect_tx(bar_q_full, box * L::kAtoms * q_tiles);
-                for (int i = 0; i < q_tiles; ++i) {
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(bar_q_full, box * L::kAtoms * q_tiles);
+                    for (int i = 0; i < q_tiles; ++i) {
 #pragma unroll
-                    for (int a = 0; a < L::kAtoms; ++a) {
-                        tma_load_4d(sm + L::kQ + (i * L::kAtoms + a) * L::kQAtom, &map_q, a * 64, at.h * p.group,
-                                    r.first + i * p.tile_tokens, at.b, bar_q_full);
+                        for (int a = 0; a < L::kAtoms; ++a) {
+                            tma_load_4d(sm + L::kQ + (i * L::kAtoms + a) * L::kQAtom, &map_q, a * 64, at.h * p.group,
+                                        r.first + i * p.tile_tokens, at.b, bar_q_full);
+                        }
                     }
                 }
+                __syncwarp();
                 // In the order in which slots come free: a chain's S lets go of its K tile, its O a step later of its V tile.
                 for (int i = 0; i < L::kStep; ++i) {
                     load_k(i);
@@ -505,7 +511,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                     load_k(i + L::kStep);
                 }
             }
-        } else if ((warp == 1 || (warp == 3 && kStreams == 2)) && lane == 0) {  // ---- matrix products of chain w
+        } else if (warp == 1 || (warp == 3 && kStreams == 2)) {  // ---- matrix products of chain w
             const int w = warp >> 1;
             constexpr uint32_t s_idesc = idesc_bf16_f32(64);
             constexpr uint32_t o_idesc = idesc_bf16_f32_bmn(D);
@@ -516,8 +522,8 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 wait(bar_full + slot, L::parity(tile));
                 tc_fence_after();
             };
-            // S of the chain's `step`-th 64 keys of the segment.
-            const auto scores = [&](int step) {
+            // S of the chain's `step`-th 64 keys of the segment; `last`: its last step.
+            const auto scores = [&](int step, int last) {
                 const uint32_t tile = n + static_cast<uint32_t>(step / L::kSteps);
                 const int part = step % L::kSteps;
                 const int slot = L::k_slot(ring, tile);
@@ -525,16 +531,22 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 if (part == 0) {
                     landed(slot, tile);
                 }
+                if (elect_one()) {
 #pragma unroll
-                for (int i = 0; i < D / kUmmaK; ++i) {
-                    const uint32_t in = static_cast<uint32_t>(i & 3) * 32u;
-                    umma_bf16(tmem + w * 128 + (step & 1) * 64, smem_desc_sw128(q, (i >> 2) * L::kQAtom + in),
-                              smem_desc_sw128(k, (i >> 2) * L::kKvAtom + in), s_idesc, i > 0 ? 1u : 0u);
+                    for (int i = 0; i < D / kUmmaK; ++i) {
+                        const uint32_t in = static_cast<uint32_t>(i & 3) * 32u;
+                        umma_bf16(tmem + w * 128 + (step & 1) * 64, smem_desc_sw128(q, (i >> 2) * L::kQAtom + in),
+                                  smem_desc_sw128(k, (i >> 2) * L::kKvAtom + in), s_idesc, i > 0 ? 1u : 0u);
+                    }
+                    umma_commit(bar_s + 2 * w + (step & 1));
+                    if (part == L::kSteps - 1) {
+                        umma_commit(bar_empty + slot);
+                    }
+                    if (step == last) {
+                        umma_commit(bar_q_empty);
+                    }
                 }
-                umma_commit(bar_s + 2 * w + (step & 1));
-                if (part == L::kSteps - 1) {
-                    umma_commit(bar_empty + slot);
-                }
+                __syncwarp();
             };
             uint32_t p_phase = 0;  // a bit for each of the chain's two S
             for (; segment(); advance(p, at, count, tiles)) {
@@ -543,21 +555,24 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 if (w >= chains) {  // this segment has nothing for the chain
                     for (int i = 0; kPair && i < count; ++i, ++n) {
                         landed(L::k_slot(ring, n), n);
-                        umma_commit(bar_empty + L::k_slot(ring, n));
                         landed(L::v_slot(ring, n), n);
-                        umma_commit(bar_empty + L::v_slot(ring, n));
+                        if (elect_one()) {
+                            umma_commit(bar_empty + L::k_slot(ring, n));
+                            umma_commit(bar_empty + L::v_slot(ring, n));
+                        }
+                        __syncwarp();
                     }
-                    umma_commit(bar_q_empty);
+                    if (elect_one()) {
+                        umma_commit(bar_q_empty);
+                    }
+                    __syncwarp();
                     continue;
                 }
                 const int mine = kPair ? count : (count - w + kStreams - 1) / kStreams;  // the chain's key tiles
                 const int steps = mine * L::kSteps;
-                scores(0);
+                scores(0, steps - 1);
                 if (steps > 1) {
-                    scores(1);
-                }
-                if (steps <= 2) {
-                    umma_commit(bar_q_empty);
+                    scores(1, steps - 1);
                 }
                 for (int step = 0; step < steps; ++step) {
                     const uint32_t tile = n + static_cast<uint32_t>(step / L::kSteps);
@@ -570,21 +585,21 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                     wait(bar_p + 2 * w + (step & 1), p_phase >> (step & 1) & 1u);
                     p_phase ^= 1u << (step & 1);
                     tc_fence_after();
+                    if (elect_one()) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        umma_bf16_ta(tmem + L::kTmemO + w * D, tmem + w * 128 + (step & 1) * 64 + j * 8,
-                                     smem_desc_sw128_mn(v, (part * 4 + j) * 2048u, L::kKvAtom), o_idesc,
-                                     (step > 0 || j > 0) ? 1u : 0u);
-                    }
-                    umma_commit(bar_pv + 2 * w + (step & 1));
-                    if (part == L::kSteps - 1) {
-                        umma_commit(bar_empty + slot);
-                    }
-                    if (step + 2 < steps) {
-                        scores(step + 2);
-                        if (step + 3 == steps) {
-                            umma_commit(bar_q_empty);
+                        for (int j = 0; j < 4; ++j) {
+                            umma_bf16_ta(tmem + L::kTmemO + w * D, tmem + w * 128 + (step & 1) * 64 + j * 8,
+                                         smem_desc_sw128_mn(v, (part * 4 + j) * 2048u, L::kKvAtom), o_idesc,
+                                         (step > 0 || j > 0) ? 1u : 0u);
                         }
+                        umma_commit(bar_pv + 2 * w + (step & 1));
+                        if (part == L::kSteps - 1) {
+                            umma_commit(bar_empty + slot);
+                        }
+                    }
+                    __syncwarp();
+                    if (step + 2 < steps) {
+                        scores(step + 2, steps - 1);
                     }
                 }
                 n += static_cast<uint32_t>(mine);
@@ -701,6 +716,9 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                         named_barrier(3, 256);
                     }
                 }
+                if (w == 1 && step == 0) {
+                    named_barrier(4, 256);  // half a step behind the first chain: see below
+                }
                 if (busy) {
                     float x[64];
                     tmem_load_begin<64>(t_x, x);
@@ -734,6 +752,11 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 __syncwarp();
                 if (lane == 0) {
                     mbar_arrive(bar_p + 2 * w + (step & 1));
+                }
+                if (w == 0 && step == 0 && chains == 2) {
+                    // The exponentials of both chains share one unit; a chain that starts when the other's first are
+                    // done finds it free when its own come, in all steps that follow.
+                    named_barrier_arrive(4, 256);
                 }
             }
             n += static_cast<uint32_t>(mine);
@@ -1028,7 +1051,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
     __shared__ UnitWalk s_walk;
 
     const int tid = threadIdx.x;
-    const int warp = tid >> 5;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int lane = tid & 31;
     const int columns = p.q_box_tokens * p.group;       // rows of a query tile, columns of the product
     const int chunks = (columns + 31) / 32;
@@ -1153,7 +1176,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
     };
 
     if (warp == 0) {
-        if (lane == 0) {  // ---- loads
+        {  // ---- loads
             while (at.left > 0) {
                 const int q0 = r.first(at.kt, p.tile_tokens);
                 const int tiles = r.q_tiles - q0;
@@ -1163,28 +1186,36 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
                 if (kr > 0) {
                     wait(bar_k_empty + ks, (kr - 1) & 1u);
                 }
-                mbar_arrive_expect_tx(bar_k_full + ks, L::kTile);
-                for (int a = 0; a < L::kAtoms; ++a) {
-                    tma_load_4d(sm + L::kK + ks * L::kTile + a * L::kAtom, &map_k, a * 64, at.h, at.kt * 128, at.b,
-                                bar_k_full + ks);
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(bar_k_full + ks, L::kTile);
+#pragma unroll
+                    for (int a = 0; a < L::kAtoms; ++a) {
+                        tma_load_4d(sm + L::kK + ks * L::kTile + a * L::kAtom, &map_k, a * 64, at.h, at.kt * 128, at.b,
+                                    bar_k_full + ks);
+                    }
                 }
+                __syncwarp();
                 for (int i = 0; i < count; ++i) {
                     const uint32_t fill = at.products + static_cast<uint32_t>(i);
                     const uint32_t slot = fill % L::kSlots;
                     if (fill >= static_cast<uint32_t>(L::kSlots)) {
                         wait(bar_empty + slot, (fill / L::kSlots - 1) & 1u);
                     }
-                    mbar_arrive_expect_tx(bar_full + slot, static_cast<uint32_t>(columns) * 128u * L::kAtoms);
-                    for (int a = 0; a < L::kAtoms; ++a) {
-                        tma_load_4d(sm + L::kRing + slot * L::kTile + a * L::kAtom, &map_q, a * 64, at.h * p.group,
-                                    (q0 + at.q + i) * p.tile_tokens, at.b, bar_full + slot);
+                    if (elect_one()) {
+                        mbar_arrive_expect_tx(bar_full + slot, static_cast<uint32_t>(columns) * 128u * L::kAtoms);
+#pragma unroll
+                        for (int a = 0; a < L::kAtoms; ++a) {
+                            tma_load_4d(sm + L::kRing + slot * L::kTile + a * L::kAtom, &map_q, a * 64, at.h * p.group,
+                                        (q0 + at.q + i) * p.tile_tokens, at.b, bar_full + slot);
+                        }
                     }
+                    __syncwarp();
                 }
                 step(count, tiles);
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {  // ---- matrix products
+        {  // ---- matrix products
             const uint32_t idesc = idesc_bf16_f32(chunks * 32);
             while (at.left > 0) {
                 const int tiles = r.q_tiles - r.first(at.kt, p.tile_tokens);
@@ -1202,16 +1233,21 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
                     tc_fence_after();
                     const unsigned char* k = sm + L::kK + ks * L::kTile;
                     const unsigned char* q = sm + L::kRing + slot * L::kTile;
+                    if (elect_one()) {
 #pragma unroll
-                    for (int j = 0; j < D / kUmmaK; ++j) {
-                        const uint32_t off = (j >> 2) * L::kAtom + static_cast<uint32_t>(j & 3) * 32u;
-                        umma_bf16(tmem + buffer * 128, smem_desc_sw128(k, off), smem_desc_sw128(q, off), idesc,
-                                  j > 0 ? 1u : 0u);
+                        for (int j = 0; j < D / kUmmaK; ++j) {
+                            const uint32_t off = (j >> 2) * L::kAtom + static_cast<uint32_t>(j & 3) * 32u;
+                            umma_bf16(tmem + buffer * 128, smem_desc_sw128(k, off), smem_desc_sw128(q, off), idesc,
+                                      j > 0 ? 1u : 0u);
+                        }
+                        umma_commit(bar_s + buffer);
+                        umma_commit(bar_empty + slot);
+                        if (i == count - 1) {
+                            umma_commit(bar_k_empty + ks);
+                        }
                     }
-                    umma_commit(bar_s + buffer);
-                    umma_commit(bar_empty + slot);
+                    __syncwarp();
                 }
-                umma_commit(bar_k_empty + ks);
                 step(count, tiles);
             }
         }

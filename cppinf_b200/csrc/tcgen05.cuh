@@ -260,6 +260,26 @@ __device__ __forceinline__ void named_barrier(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
+// True in one lane of a converged warp. Code that issues tcgen05 and TMA instructions goes in warps that stay together
+// and has one lane picked for the instructions alone: their descriptors then stay in the warp's uniform registers, where
+// the instructions take them from, instead of being moved there for each of them.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t picked;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "elect.sync _|p, 0xffffffff;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(picked));
+    return picked != 0u;
+}
+
+// Arrives at barrier `id` without waiting for it.
+__device__ __forceinline__ void named_barrier_arrive(int id, int threads) {
+    asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 // 2^x of the hardware, within 2 ulp.
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
