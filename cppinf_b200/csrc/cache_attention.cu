@@ -149,10 +149,10 @@ struct Tiling {
     static constexpr uint32_t kMl = kMask + kStreams * 128 * 9 * 4;  // [128] the second chain's (M, l)
     static constexpr uint32_t kFlags = kMl + 128 * 8;               // [2][16]
     static constexpr uint32_t kBars = kFlags + 2 * 16 * 4;
-    static constexpr std::size_t kBytes = 1024 + kBars + 256;
-    // A chain goes in steps of 64 keys with an S for each of two steps (P over it): while one step's softmax runs, the
-    // step before it is multiplied with V and the step after it with Q. Tensor memory: the chains' S, then their O.
-    static constexpr int kSteps = kKeys / 64;  // of a key tile
+    static constexpr std::size_t kBytes = 1024 + kBars + 384;
+    // Tensor memory columns: the chains' S (P over it), one each or two for a lone chain, then their O.
+    static constexpr int kAhead = 128 / kKeys;
+    static constexpr int kHalf = kKeys / 2;  // P is handed over in halves
     static constexpr uint32_t kTmemO = kStreams * 128;
     static_assert(kDepth >= 1 && kStreams * (128 + D) <= 512, "tensor memory has 512 columns");
 
@@ -223,10 +223,13 @@ struct Waiter {
     volatile uint32_t* stop;
 
     __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t phase) const {
-        if (mbar_wait_bounded(bar, phase, limit < 64u ? limit : 64u) || *stop != 0u) {
-            return;
+        if (limit == 0u || !mbar_try_wait(bar, phase)) {
+            slow(bar, phase);
         }
-        if (mbar_wait_bounded(bar, phase, limit)) {
+    }
+
+    __device__ __forceinline__ void slow(uint64_t* bar, uint32_t phase) const {
+        if (*stop != 0u || mbar_wait_bounded(bar, phase, limit)) {
             return;
         }
         if (error != nullptr) {
@@ -281,11 +284,12 @@ __device__ __forceinline__ float largest(const float (&x)[N], float top) {
     return fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
 }
 
-// P of 64 keys, 2^(x factor + offset), stored as bf16 pairs at `taddr`; returns their sum in f32.
-__device__ __forceinline__ float probabilities(const float (&x)[64], float2 factor, float2 offset, uint32_t taddr) {
+// P of N keys, 2^(x factor + offset), stored as bf16 pairs at `taddr`; returns their sum in f32.
+template <int N>
+__device__ __forceinline__ float probabilities(const float (&x)[N], float2 factor, float2 offset, uint32_t taddr) {
     float2 sums[2] = {};
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < N / 32; ++c) {
         uint32_t packed[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
@@ -331,8 +335,8 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
     uint64_t* bar_q_full = bars + 2 * L::kSlots;
     uint64_t* bar_q_empty = bar_q_full + 1;
     uint64_t* bar_s = bar_q_empty + 1;            // [chains][2] S is complete
-    uint64_t* bar_p = bar_s + 2 * kStreams;       // [chains][2] P is written
-    uint64_t* bar_pv = bar_p + 2 * kStreams;      // [chains][2] its product with V is complete
+    uint64_t* bar_pv = bar_s + 2 * kStreams;      // [chains][2] the product of its P with V is complete
+    uint64_t* bar_p = bar_pv + 2 * kStreams;      // [chains][2][2] half of P is written
     __shared__ uint32_t s_tmem;
     __shared__ uint32_t s_stop;
     __shared__ Walk s_walk;
@@ -344,15 +348,16 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
         s_stop = 0u;
         for (int i = 0; i < L::kSlots; ++i) {
             mbar_init(bar_full + i, 1);
-            mbar_init(bar_empty + i, kPair ? 2 : 1);
+            mbar_init(bar_empty + i, 1);
         }
         mbar_init(bar_q_full, 1);
-        mbar_init(bar_q_empty, kStreams);
+        mbar_init(bar_q_empty, 1);
         for (int w = 0; w < kStreams; ++w) {
             mbar_init(bar_s + 2 * w, 1);
             mbar_init(bar_s + 2 * w + 1, 1);
-            mbar_init(bar_p + 2 * w, 4);
-            mbar_init(bar_p + 2 * w + 1, 4);
+            for (int i = 0; i < 4; ++i) {
+                mbar_init(bar_p + 4 * w + i, 4);
+            }
             mbar_init(bar_pv + 2 * w, 1);
             mbar_init(bar_pv + 2 * w + 1, 1);
         }
@@ -428,7 +433,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = uniform(s_tmem);
     const Waiter wait{p.error, p.poll_limit, &s_stop};
     Walk at = s_walk;
     // The current segment: its item, the item's key tiles, the key tiles of them that it takes, the chains at work.
@@ -511,98 +516,104 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                     load_k(i + L::kStep);
                 }
             }
-        } else if (warp == 1 || (warp == 3 && kStreams == 2)) {  // ---- matrix products of chain w
-            const int w = warp >> 1;
-            constexpr uint32_t s_idesc = idesc_bf16_f32(64);
+        } else if (warp == 1) {  // ---- matrix products, the chains in turn
+            constexpr uint32_t s_idesc = idesc_bf16_f32(kKeys);
             constexpr uint32_t o_idesc = idesc_bf16_f32_bmn(D);
-            const unsigned char* q = sm + L::kQ + (kPair ? w * L::kAtoms * L::kQAtom : 0);
-            const int ring = kPair ? 0 : w;
-            uint32_t n = 0;  // tiles of the chain before the current one
-            const auto landed = [&](int slot, uint32_t tile) {
-                wait(bar_full + slot, L::parity(tile));
-                tc_fence_after();
-            };
-            // S of the chain's `step`-th 64 keys of the segment; `last`: its last step.
-            const auto scores = [&](int step, int last) {
-                const uint32_t tile = n + static_cast<uint32_t>(step / L::kSteps);
-                const int part = step % L::kSteps;
-                const int slot = L::k_slot(ring, tile);
-                const unsigned char* k = sm + L::kRing + slot * L::kSlot + part * (64 * 128);
-                if (part == 0) {
-                    landed(slot, tile);
-                }
-                if (elect_one()) {
-#pragma unroll
-                    for (int i = 0; i < D / kUmmaK; ++i) {
-                        const uint32_t in = static_cast<uint32_t>(i & 3) * 32u;
-                        umma_bf16(tmem + w * 128 + (step & 1) * 64, smem_desc_sw128(q, (i >> 2) * L::kQAtom + in),
-                                  smem_desc_sw128(k, (i >> 2) * L::kKvAtom + in), s_idesc, i > 0 ? 1u : 0u);
-                    }
-                    umma_commit(bar_s + 2 * w + (step & 1));
-                    if (part == L::kSteps - 1) {
-                        umma_commit(bar_empty + slot);
-                    }
-                    if (step == last) {
-                        umma_commit(bar_q_empty);
-                    }
-                }
-                __syncwarp();
-            };
-            uint32_t p_phase = 0;  // a bit for each of the chain's two S
+            uint32_t n[kStreams] = {};  // tiles of the chains before the segment
+            uint32_t p_phase = 0;       // a bit for each S
+            const uint64_t q_desc = uniform(smem_desc_sw128(sm + L::kQ, 0));
+            const uint64_t k_desc = uniform(smem_desc_sw128(sm + L::kRing, 0));
+            const uint64_t v_desc = uniform(smem_desc_sw128_mn(sm + L::kRing, 0, L::kKvAtom));
+            const auto landed = [&](int slot, uint32_t tile) { wait(bar_full + slot, L::parity(tile)); };
             for (; segment(); advance(p, at, count, tiles)) {
-                wait(bar_q_full, static_cast<uint32_t>(at.index) & 1u);
-                tc_fence_after();
-                if (w >= chains) {  // this segment has nothing for the chain
-                    for (int i = 0; kPair && i < count; ++i, ++n) {
-                        landed(L::k_slot(ring, n), n);
-                        landed(L::v_slot(ring, n), n);
-                        if (elect_one()) {
-                            umma_commit(bar_empty + L::k_slot(ring, n));
-                            umma_commit(bar_empty + L::v_slot(ring, n));
-                        }
-                        __syncwarp();
-                    }
-                    if (elect_one()) {
-                        umma_commit(bar_q_empty);
-                    }
-                    __syncwarp();
-                    continue;
+                int mine[kStreams];  // the chains' key tiles
+#pragma unroll
+                for (int w = 0; w < kStreams; ++w) {
+                    mine[w] = w >= chains ? 0 : kPair ? count : (count - w + kStreams - 1) / kStreams;
                 }
-                const int mine = kPair ? count : (count - w + kStreams - 1) / kStreams;  // the chain's key tiles
-                const int steps = mine * L::kSteps;
-                scores(0, steps - 1);
-                if (steps > 1) {
-                    scores(1, steps - 1);
-                }
-                for (int step = 0; step < steps; ++step) {
-                    const uint32_t tile = n + static_cast<uint32_t>(step / L::kSteps);
-                    const int part = step % L::kSteps;
-                    const int slot = L::v_slot(ring, tile);
-                    const unsigned char* v = sm + L::kRing + slot * L::kSlot;
-                    if (part == 0) {
-                        landed(slot, tile);
-                    }
-                    wait(bar_p + 2 * w + (step & 1), p_phase >> (step & 1) & 1u);
-                    p_phase ^= 1u << (step & 1);
-                    tc_fence_after();
+                int left = kStreams == 1 ? mine[0] : mine[0] + mine[kStreams - 1];  // S still to come
+                // S of chain w's i-th key tile of the segment.
+                const auto scores = [&](int w, int i) {
+                    const uint32_t tile = n[w] + static_cast<uint32_t>(i);
+                    const int slot = L::k_slot(kPair ? 0 : w, tile);
+                    const int buffer = i % L::kAhead;
+                    const uint64_t q = smem_desc_at(q_desc, kPair ? w * L::kAtoms * L::kQAtom : 0);
+                    const uint64_t k = smem_desc_at(k_desc, uniform(slot * L::kSlot));
+                    --left;
                     if (elect_one()) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            umma_bf16_ta(tmem + L::kTmemO + w * D, tmem + w * 128 + (step & 1) * 64 + j * 8,
-                                         smem_desc_sw128_mn(v, (part * 4 + j) * 2048u, L::kKvAtom), o_idesc,
-                                         (step > 0 || j > 0) ? 1u : 0u);
+                        for (int j = 0; j < D / kUmmaK; ++j) {
+                            const uint32_t in = static_cast<uint32_t>(j & 3) * 32u;
+                            umma_bf16(tmem + w * 128 + buffer * kKeys, smem_desc_at(q, (j >> 2) * L::kQAtom + in),
+                                      smem_desc_at(k, (j >> 2) * L::kKvAtom + in), s_idesc, j > 0 ? 1u : 0u);
                         }
-                        umma_commit(bar_pv + 2 * w + (step & 1));
-                        if (part == L::kSteps - 1) {
+                        umma_commit(bar_s + 2 * w + buffer);
+                        if (!kPair || w == chains - 1) {
                             umma_commit(bar_empty + slot);
                         }
+                        if (left == 0) {
+                            umma_commit(bar_q_empty);
+                        }
                     }
                     __syncwarp();
-                    if (step + 2 < steps) {
-                        scores(step + 2, steps - 1);
+                };
+                wait(bar_q_full, static_cast<uint32_t>(at.index) & 1u);
+                tc_fence_after();
+#pragma unroll
+                for (int i = 0; i < L::kAhead; ++i) {
+#pragma unroll
+                    for (int w = 0; w < kStreams; ++w) {
+                        if (i < mine[w]) {
+                            landed(L::k_slot(kPair ? 0 : w, n[w] + i), n[w] + i);
+                            scores(w, i);
+                        }
                     }
                 }
-                n += static_cast<uint32_t>(mine);
+                for (int i = 0; i < mine[0]; ++i) {
+#pragma unroll
+                    for (int w = 0; w < kStreams; ++w) {
+                        if (i >= mine[w]) {
+                            continue;
+                        }
+                        const uint32_t tile = n[w] + static_cast<uint32_t>(i);
+                        const int slot = L::v_slot(kPair ? 0 : w, tile);
+                        const int buffer = i % L::kAhead;
+                        const uint64_t v = smem_desc_at(v_desc, uniform(slot * L::kSlot));
+                        const bool more = i + L::kAhead < mine[w];
+                        landed(slot, tile);
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            if (half == 1 && more) {
+                                landed(L::k_slot(kPair ? 0 : w, tile + L::kAhead), tile + L::kAhead);
+                            }
+                            wait(bar_p + 4 * w + 2 * buffer + half, p_phase >> (2 * w + buffer) & 1u);
+                            tc_fence_after();
+                            if (elect_one()) {
+#pragma unroll
+                                for (int j = half * (L::kHalf / kUmmaK); j < (half + 1) * (L::kHalf / kUmmaK); ++j) {
+                                    umma_bf16_ta(tmem + L::kTmemO + w * D, tmem + w * 128 + buffer * kKeys + j * 8,
+                                                 smem_desc_at(v, j * 2048u), o_idesc,
+                                                 (i > 0 || j > 0) ? 1u : 0u);
+                                }
+                                if (half == 1) {
+                                    umma_commit(bar_pv + 2 * w + buffer);
+                                    if (!kPair || w == chains - 1) {
+                                        umma_commit(bar_empty + slot);
+                                    }
+                                }
+                            }
+                            __syncwarp();
+                        }
+                        p_phase ^= 1u << (2 * w + buffer);
+                        if (more) {
+                            scores(w, i + L::kAhead);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < kStreams; ++w) {
+                    n[w] += static_cast<uint32_t>(kPair ? count : mine[w]);
+                }
             }
         }
     } else {  // ---- softmax: chain w, one thread per row
@@ -616,10 +627,17 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
         const float c2 = 1.4426950408889634f / sqrtf(static_cast<float>(D));
         uint32_t s_phase = 0;  // a bit for each of the chain's two S
         uint32_t n = 0;        // tiles of the chain before the segment
-        // Waits until a step, the last one whose S has been taken or the one before it, has reached O. Each S of the two
-        // has a barrier for this: its last phase but one is over, since S was complete after it.
-        const auto settled = [&](int step) {
-            wait(bar_pv + 2 * w + (step & 1), (s_phase >> (step & 1) & 1u) ^ 1u);
+        // Waits until the product of a tile, the last one whose S has been taken or the one before it, has reached O.
+        // With two S each has a barrier for this: its last phase but one is over, since its S was complete after that.
+        const auto hand_over = [&](uint64_t* bar) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(bar);
+            }
+        };
+        const auto settled = [&](int i) {
+            wait(bar_pv + 2 * w + i % L::kAhead, (s_phase >> (i % L::kAhead) & 1u) ^ 1u);
             tc_fence_after();
         };
         for (; segment(); advance(p, at, count, tiles)) {
@@ -669,18 +687,18 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             float top = -INFINITY;  // the maximum that P is taken against, in units of S
             float sum = 0.0f;
             const int mine = kPair ? count : (count - w + kStreams - 1) / kStreams;  // the chain's key tiles
-            for (int step = 0; step < mine * L::kSteps; ++step) {
-                const uint32_t tile = n + static_cast<uint32_t>(step / L::kSteps);
-                const int tile0 = (at.tile + (kPair ? 0 : w) + step / L::kSteps * L::kStep) * kKeys;
-                const int key0 = tile0 + step % L::kSteps * 64;
-                const bool partial = tile0 + kKeys > r.full_end;
-                const uint32_t t_x = t_s + (step & 1) * 64;
-                wait(bar_s + 2 * w + (step & 1), s_phase >> (step & 1) & 1u);
-                s_phase ^= 1u << (step & 1);
+            for (int i = 0; i < mine; ++i) {
+                const uint32_t tile = n + static_cast<uint32_t>(i);
+                const int buffer = i % L::kAhead;
+                const int key0 = (at.tile + (kPair ? 0 : w) + i * L::kStep) * kKeys;
+                const bool partial = key0 + kKeys > r.full_end;
+                const uint32_t t_x = t_s + buffer * kKeys;
+                wait(bar_s + 2 * w + buffer, s_phase >> buffer & 1u);
+                s_phase ^= 1u << buffer;
                 tc_fence_after();
-                if (partial && step % L::kSteps == 0) {
+                if (partial) {
                     // V rows that nobody sees become zeros, values that are not finite are set aside. S is complete, so
-                    // the chain's product two steps before is, and the slot's tile before this one has landed.
+                    // the tile before the last of the chain has been multiplied and the slot's tile before has landed.
                     const int slot = L::v_slot(kPair ? 0 : w, tile);
                     wait(bar_full + slot, L::parity(tile));
                     unsigned char* v = sm + L::kRing + slot * L::kSlot;
@@ -688,7 +706,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                     for (int u = (sharing == 2 ? w * 128 : 0) + row; u < kKeys * L::kAtoms; u += 128 * sharing) {
                         const int key = u % kKeys;  // this thread's: 64 dims of a row
                         uint4* at16 = reinterpret_cast<uint4*>(v + u / kKeys * L::kKvAtom + key * 128);
-                        if (tile0 + key >= r.kv_end) {
+                        if (key0 + key >= r.kv_end) {
 #pragma unroll
                             for (int ch = 0; ch < 8; ++ch) {
                                 at16[ch ^ (key & 7)] = make_uint4(0u, 0u, 0u, 0u);
@@ -707,7 +725,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                                 at16[ch] = make_uint4(finite_pair(x.x), finite_pair(x.y), finite_pair(x.z),
                                                       finite_pair(x.w));
                             }
-                            const int bit = tile0 + key - part0;
+                            const int bit = key0 + key - part0;
                             atomicOr(&s_flags[w * 16 + (bit >> 5)], 1u << (bit & 31));
                         }
                     }
@@ -716,20 +734,28 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                         named_barrier(3, 256);
                     }
                 }
-                if (w == 1 && step == 0) {
-                    named_barrier(4, 256);  // half a step behind the first chain: see below
-                }
+                float2 offset = make_float2(0.0f, 0.0f);
+                float x[L::kHalf];
+                // The second half first, for its maximum alone: it is read again for its exponentials, which costs less
+                // than a row of registers.
                 if (busy) {
-                    float x[64];
-                    tmem_load_begin<64>(t_x, x);
-                    tmem_load_end<64>(x);
+                    tmem_load_begin<L::kHalf>(t_x + L::kHalf, x);
+                    tmem_load_end<L::kHalf>(x);
+                    if (partial) {
+                        hide(x, bits_row, key0 + L::kHalf, r.len, limit);
+                    }
+                    float new_top = largest(x, top);
+                    tmem_load_begin<L::kHalf>(t_x, x);
+                    tmem_load_end<L::kHalf>(x);
                     if (partial) {
                         hide(x, bits_row, key0, r.len, limit);
                     }
-                    const float new_top = largest(x, top);
-                    const bool grown = step == 0 || (new_top - top) * c2 > 8.0f;
-                    if (step > 0 && __any_sync(0xffffffffu, grown)) {
-                        settled(step - 1);
+                    new_top = largest(x, new_top);
+                    const bool grown = i == 0 || (new_top - top) * c2 > 8.0f;
+                    if (i > 0 && __any_sync(0xffffffffu, grown)) {
+                        if constexpr (L::kAhead > 1) {
+                            settled(i - 1);
+                        }
                         const float f = grown ? exp2_approx((top - new_top) * c2) : 1.0f;
                         sum *= f;
 #pragma unroll 1
@@ -745,22 +771,24 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                     }
                     top = grown ? new_top : top;
                     const float shift = top == -INFINITY ? 0.0f : top * c2;
-                    sum += probabilities(x, make_float2(c2, c2), make_float2(-shift, -shift), t_x);
+                    offset = make_float2(-shift, -shift);
+                    sum += probabilities(x, make_float2(c2, c2), offset, t_x);
                     tmem_store_wait();
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(bar_p + 2 * w + (step & 1));
+                hand_over(bar_p + 4 * w + 2 * buffer);
+                if (busy) {
+                    tmem_load_begin<L::kHalf>(t_x + L::kHalf, x);
+                    tmem_load_end<L::kHalf>(x);
+                    if (partial) {
+                        hide(x, bits_row, key0 + L::kHalf, r.len, limit);
+                    }
+                    sum += probabilities(x, make_float2(c2, c2), offset, t_x + L::kHalf / 2);
+                    tmem_store_wait();
                 }
-                if (w == 0 && step == 0 && chains == 2) {
-                    // The exponentials of both chains share one unit; a chain that starts when the other's first are
-                    // done finds it free when its own come, in all steps that follow.
-                    named_barrier_arrive(4, 256);
-                }
+                hand_over(bar_p + 4 * w + 2 * buffer + 1);
             }
             n += static_cast<uint32_t>(mine);
-            settled(mine * L::kSteps - 1);
+            settled(mine - 1);
             if (hides) {
                 named_barrier(1 + w, 128);  // the flags of all the chain's threads
                 uint32_t flagged = 0u;

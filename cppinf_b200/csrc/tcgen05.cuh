@@ -95,6 +95,22 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(const void* tile, uint32_t k
     return d;
 }
 
+// A descriptor `bytes` (a multiple of 16) further on: the start address lies below 2^18 and leaves its field's upper bits
+// free, so only the lower word changes.
+__device__ __forceinline__ uint64_t smem_desc_at(uint64_t desc, uint32_t bytes) {
+    return (desc & 0xffffffff00000000ull) | (static_cast<uint32_t>(desc) + (bytes >> 4));
+}
+
+// A value that is the same in all lanes of a converged warp, said so that the compiler knows it: it can then live in a
+// uniform register, where the tcgen05 instructions take their operands from.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) {
+    return __shfl_sync(0xffffffffu, x, 0);
+}
+
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+    return static_cast<uint64_t>(uniform(static_cast<uint32_t>(x >> 32))) << 32 | uniform(static_cast<uint32_t>(x));
+}
+
 // Instruction descriptor of kind::f16 with bf16 A and B, f32 D, both K-major, M = 128, N = n:
 // D format bits 4-5 (1 = f32), A format bits 7-9 and B format bits 10-12 (1 = bf16), N >> 3 in bits 17-22,
 // M >> 4 in bits 24-28.
