@@ -67,8 +67,8 @@ struct CacheAttentionParams {
     int row_tiles;        // items along the tokens
     int q_box_tokens;     // tokens of one TMA box of q
     int part_rows;        // rows of a part in the scratch
-    int4* cuts;           // [CTAs] where each CTA's part of the line begins: sequence, row tile, head, key tile
-    int* line;            // length of the line
+    int4* cuts;           // [CTAs] where each CTA's part of the line begins: sequence, row tile, head, piece
+    int* line;            // length of the line, pieces of an item before its tiles
     float2* part_ml;      // [2 CTAs][part_rows] (M in base 2, l)
     float* part_o;        // [2 CTAs][D / 4][part_rows][4]
     unsigned int* tickets;  // [weight CTAs] parts of a unit that have been left, zeroed by the attention kernel
@@ -166,27 +166,30 @@ struct Tiling {
 
 constexpr uint32_t kTmemAll = 512;
 
+// An item's share of the line: its key tiles, and before them `kSetUp` pieces without any for what an item costs besides
+// its tiles (loading Q, the first S, writing the rows: 9000 to 12000 cycles, where a tile takes about 3000). Left out
+// where CTAs have few tiles each and a set-up's place would be better taken by a tile.
+constexpr int kSetUp = 3;
+constexpr int kSetUpFrom = 8;  // tiles per CTA
+
 // Where a CTA's part of the line is, item by item; every role of the CTA walks it for itself.
 struct Walk {
     int b;
     int row_tile;
     int h;
-    int tile;        // first key tile of the current segment
-    int left;        // key tiles of the part still to come, the current segment's included
+    int piece;       // first piece of the current item that the part has
+    int left;        // pieces of the part still to come, those of the current item included
+    int set_up;      // pieces of each item before its tiles
     int len;         // of sequence b
     int valid;
     int index;       // segments before the current one
 };
 
-__device__ __forceinline__ void advance(const CacheAttentionParams& p, Walk& w, int count, int tiles) {
-    w.left -= count;
-    ++w.index;
-    w.tile += count;
-    if (w.tile < tiles) {
-        return;
-    }
-    w.tile = 0;
-    if (++w.h < static_cast<int>(p.kv_heads)) {
+__device__ __forceinline__ void advance(const CacheAttentionParams& p, Walk& w, int tiles) {
+    const int pieces = tiles + w.set_up - w.piece;
+    w.left -= pieces;
+    w.piece = 0;
+    if (w.left <= 0 || ++w.h < static_cast<int>(p.kv_heads)) {
         return;
     }
     w.h = 0;
@@ -195,10 +198,8 @@ __device__ __forceinline__ void advance(const CacheAttentionParams& p, Walk& w, 
     }
     w.row_tile = 0;
     ++w.b;
-    if (w.left > 0) {
-        w.len = static_cast<int>(committed_rows(p, w.b));
-        w.valid = static_cast<int>(valid_queries(p, w.b));
-    }
+    w.len = static_cast<int>(committed_rows(p, w.b));
+    w.valid = static_cast<int>(valid_queries(p, w.b));
 }
 
 // A line of `total` pieces cut into `parts` that differ by one piece at most.
@@ -260,18 +261,37 @@ __device__ __forceinline__ uint32_t visible_bits(const uint32_t* row, int key, i
 }
 
 // Scores of keys that the row does not see become -inf; words of 32 keys that every row of the warp sees are left alone.
+// Returns whether the warp has other words.
 template <int N>
-__device__ __forceinline__ void hide(float (&x)[N], const uint32_t* row, int key, int len, int limit) {
+__device__ __forceinline__ bool hide(float (&x)[N], const uint32_t* row, int key, int len, int limit) {
+    bool hidden = false;
 #pragma unroll
     for (int c = 0; c < N / 32; ++c) {
         const uint32_t see = visible_bits(row, key + c * 32, len, limit);
         if (!__all_sync(0xffffffffu, see == 0xffffffffu)) {
+            hidden = true;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
                 x[c * 32 + j] = (see >> j & 1u) != 0u ? x[c * 32 + j] : -INFINITY;
             }
         }
     }
+    return hidden;
+}
+
+// Stores N consecutive f32 columns of this thread's tensor-memory lane and waits for the stores.
+template <int N>
+__device__ __forceinline__ void tmem_store(uint32_t taddr, const float (&x)[N]) {
+#pragma unroll
+    for (int c = 0; c < N / 16; ++c) {
+        uint32_t r[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            r[j] = __float_as_uint(x[c * 16 + j]);
+        }
+        tmem_store16(taddr + c * 16, r);
+    }
+    tmem_store_wait();
 }
 
 template <int N>
@@ -389,6 +409,8 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             total += tiles_of(e, entry(e));
         }
         total = __reduce_add_sync(0xffffffffu, total);
+        const int set_up = total / kSetUpFrom >= static_cast<int>(gridDim.x) ? kSetUp : 0;
+        total += set_up * heads * entries;
         const Cuts cuts(total, static_cast<int>(gridDim.x));
         const int begin = cuts.begin(static_cast<int>(blockIdx.x));
         const int end = cuts.begin(static_cast<int>(blockIdx.x) + 1);
@@ -402,6 +424,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 w = entry(e0 + lane);
                 mine = tiles_of(e0 + lane, w);
             }
+            mine += e0 + lane < entries ? set_up * heads : 0;
             int sum = mine;
             for (int offset = 1; offset < 32; offset <<= 1) {
                 const int other = __shfl_up_sync(0xffffffffu, sum, offset);
@@ -411,10 +434,11 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             if (begin >= lo && begin < lo + mine) {
                 const int each = mine / heads;
                 w.h = (begin - lo) / each;
-                w.tile = (begin - lo) - w.h * each;
+                w.piece = (begin - lo) - w.h * each;
                 w.left = end - begin;
+                w.set_up = set_up;
                 s_walk = w;
-                p.cuts[blockIdx.x] = make_int4(w.b, w.row_tile, w.h, w.tile);
+                p.cuts[blockIdx.x] = make_int4(w.b, w.row_tile, w.h, w.piece);
             }
             before += __shfl_sync(0xffffffffu, sum, 31);
             if (before > begin) {
@@ -423,7 +447,8 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
         }
         if (blockIdx.x == 0) {
             if (lane == 0) {
-                *p.line = total;
+                p.line[0] = total;
+                p.line[1] = set_up;
             }
             for (int i = lane; i < p.weight_ctas; i += 32) {
                 p.tickets[i] = 0u;
@@ -436,20 +461,33 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
     const uint32_t tmem = uniform(s_tmem);
     const Waiter wait{p.error, p.poll_limit, &s_stop};
     Walk at = s_walk;
-    // The current segment: its item, the item's key tiles, the key tiles of them that it takes, the chains at work.
+    // The current segment: its item, the item's key tiles, the first and the number of those that it takes, the chains at
+    // work (a row tile without valid queries has none).
     ItemRange r{};
     int tiles = 0;
+    int tile0 = 0;
     int count = 0;
     int chains = 0;
     const auto segment = [&]() {
-        if (at.left <= 0) {
-            return false;
+        for (;; advance(p, at, tiles)) {
+            if (at.left <= 0) {
+                return false;
+            }
+            r = item_range(p, at.len, at.valid, at.row_tile);
+            tiles = item_tiles<kKeys>(r);
+            tile0 = at.piece > at.set_up ? at.piece - at.set_up : 0;
+            const int end = at.piece + at.left - at.set_up;
+            count = (end < tiles ? end : tiles) - tile0;
+            if (count > 0) {
+                break;
+            }
         }
-        r = item_range(p, at.len, at.valid, at.row_tile);
-        tiles = item_tiles<kKeys>(r);
-        count = tiles - at.tile < at.left ? tiles - at.tile : at.left;
-        chains = kStreams == 1 ? 1 : kPair ? (r.first + p.tile_tokens < p.tokens ? 2 : 1) : (count < 2 ? count : 2);
+        chains = kStreams == 1 ? 1 : kPair ? (r.first + p.tile_tokens < r.valid ? 2 : 1) : (count < 2 ? count : 2);
         return true;
+    };
+    const auto next = [&]() {
+        ++at.index;
+        advance(p, at, tiles);
     };
     if (warp < 4) {
         if (warp == 0) {  // ---- loads
@@ -473,18 +511,18 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             const auto load_k = [&](int i) {
                 const int ring = i % L::kRings;
                 if (i < count) {
-                    load(&map_k, L::k_slot(ring, k_tiles[ring]), k_tiles[ring], at.tile + i);
+                    load(&map_k, L::k_slot(ring, k_tiles[ring]), k_tiles[ring], tile0 + i);
                     ++k_tiles[ring];
                 }
             };
             const auto load_v = [&](int i) {
                 const int ring = i % L::kRings;
                 if (i < count) {
-                    load(&map_v, L::v_slot(ring, v_tiles[ring]), v_tiles[ring], at.tile + i);
+                    load(&map_v, L::v_slot(ring, v_tiles[ring]), v_tiles[ring], tile0 + i);
                     ++v_tiles[ring];
                 }
             };
-            for (; segment(); advance(p, at, count, tiles)) {
+            for (; segment(); next()) {
                 if (at.index > 0) {
                     wait(bar_q_empty, static_cast<uint32_t>(at.index - 1) & 1u);
                 }
@@ -519,101 +557,82 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
         } else if (warp == 1) {  // ---- matrix products, the chains in turn
             constexpr uint32_t s_idesc = idesc_bf16_f32(kKeys);
             constexpr uint32_t o_idesc = idesc_bf16_f32_bmn(D);
-            uint32_t n[kStreams] = {};  // tiles of the chains before the segment
-            uint32_t p_phase = 0;       // a bit for each S
+            uint32_t n0 = 0;  // tiles of the chains before the segment
+            uint32_t n1 = 0;
+            uint32_t p_phase = 0;  // a bit for each S
             const uint64_t q_desc = uniform(smem_desc_sw128(sm + L::kQ, 0));
             const uint64_t k_desc = uniform(smem_desc_sw128(sm + L::kRing, 0));
             const uint64_t v_desc = uniform(smem_desc_sw128_mn(sm + L::kRing, 0, L::kKvAtom));
-            const auto landed = [&](int slot, uint32_t tile) { wait(bar_full + slot, L::parity(tile)); };
-            for (; segment(); advance(p, at, count, tiles)) {
-                int mine[kStreams];  // the chains' key tiles
-#pragma unroll
-                for (int w = 0; w < kStreams; ++w) {
-                    mine[w] = w >= chains ? 0 : kPair ? count : (count - w + kStreams - 1) / kStreams;
-                }
-                int left = kStreams == 1 ? mine[0] : mine[0] + mine[kStreams - 1];  // S still to come
-                // S of chain w's i-th key tile of the segment.
-                const auto scores = [&](int w, int i) {
-                    const uint32_t tile = n[w] + static_cast<uint32_t>(i);
-                    const int slot = L::k_slot(kPair ? 0 : w, tile);
-                    const int buffer = i % L::kAhead;
-                    const uint64_t q = smem_desc_at(q_desc, kPair ? w * L::kAtoms * L::kQAtom : 0);
-                    const uint64_t k = smem_desc_at(k_desc, uniform(slot * L::kSlot));
-                    --left;
-                    if (elect_one()) {
-#pragma unroll
-                        for (int j = 0; j < D / kUmmaK; ++j) {
-                            const uint32_t in = static_cast<uint32_t>(j & 3) * 32u;
-                            umma_bf16(tmem + w * 128 + buffer * kKeys, smem_desc_at(q, (j >> 2) * L::kQAtom + in),
-                                      smem_desc_at(k, (j >> 2) * L::kKvAtom + in), s_idesc, j > 0 ? 1u : 0u);
-                        }
-                        umma_commit(bar_s + 2 * w + buffer);
-                        if (!kPair || w == chains - 1) {
-                            umma_commit(bar_empty + slot);
-                        }
-                        if (left == 0) {
-                            umma_commit(bar_q_empty);
-                        }
-                    }
-                    __syncwarp();
-                };
+            for (; segment(); next()) {
+                const int mine0 = kPair ? count : (count + kStreams - 1) / kStreams;  // the chains' key tiles
+                const int mine1 = chains < 2 ? 0 : kPair ? count : count / 2;
                 wait(bar_q_full, static_cast<uint32_t>(at.index) & 1u);
-                tc_fence_after();
+                // Turn i of a chain: O += P V of its i-th key tile, then S of its tile kAhead further on. The loops stay
+                // rolled: the code is run once a tile, and what it takes in the instruction cache the softmax misses.
+#pragma unroll 1
+                for (int i = -L::kAhead; i < mine0; ++i) {
+#pragma unroll 1
+                    for (int w = 0; w < chains; ++w) {
+                        const int mine = w == 0 ? mine0 : mine1;
+                        const int ring = kPair ? 0 : w;
+                        const int buffer = (i + L::kAhead) % L::kAhead;
+                        const uint32_t tile = (w == 0 ? n0 : n1) + static_cast<uint32_t>(i);
+                        const uint32_t t_s = uniform(tmem + w * 128 + buffer * kKeys);
+                        const uint32_t t_o = uniform(tmem + L::kTmemO + w * D);
+                        if (i >= 0 && i < mine) {
+                            const int slot = L::v_slot(ring, tile);
+                            const uint64_t v = smem_desc_at(v_desc, uniform(slot * L::kSlot));
+                            wait(bar_full + slot, L::parity(tile));
 #pragma unroll
-                for (int i = 0; i < L::kAhead; ++i) {
+                            for (int half = 0; half < 2; ++half) {
+                                wait(bar_p + 4 * w + 2 * buffer + half, p_phase >> (2 * w + buffer) & 1u);
+                                tc_fence_after();
+                                if (elect_one()) {
 #pragma unroll
-                    for (int w = 0; w < kStreams; ++w) {
-                        if (i < mine[w]) {
-                            landed(L::k_slot(kPair ? 0 : w, n[w] + i), n[w] + i);
-                            scores(w, i);
-                        }
-                    }
-                }
-                for (int i = 0; i < mine[0]; ++i) {
-#pragma unroll
-                    for (int w = 0; w < kStreams; ++w) {
-                        if (i >= mine[w]) {
-                            continue;
-                        }
-                        const uint32_t tile = n[w] + static_cast<uint32_t>(i);
-                        const int slot = L::v_slot(kPair ? 0 : w, tile);
-                        const int buffer = i % L::kAhead;
-                        const uint64_t v = smem_desc_at(v_desc, uniform(slot * L::kSlot));
-                        const bool more = i + L::kAhead < mine[w];
-                        landed(slot, tile);
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            if (half == 1 && more) {
-                                landed(L::k_slot(kPair ? 0 : w, tile + L::kAhead), tile + L::kAhead);
+                                    for (int j = half * (L::kHalf / kUmmaK); j < (half + 1) * (L::kHalf / kUmmaK); ++j) {
+                                        umma_bf16_ta(t_o, t_s + j * 8, smem_desc_at(v, j * 2048u), o_idesc,
+                                                     (i > 0 || j > 0) ? 1u : 0u);
+                                    }
+                                    if (half == 1) {
+                                        umma_commit(bar_pv + 2 * w + buffer);
+                                        if (!kPair || w == chains - 1) {
+                                            umma_commit(bar_empty + slot);
+                                        }
+                                    }
+                                }
+                                __syncwarp();
                             }
-                            wait(bar_p + 4 * w + 2 * buffer + half, p_phase >> (2 * w + buffer) & 1u);
+                            p_phase ^= 1u << (2 * w + buffer);
+                        }
+                        if (i + L::kAhead < mine) {
+                            const uint32_t ahead = tile + L::kAhead;
+                            const int slot = L::k_slot(ring, ahead);
+                            const uint64_t q = smem_desc_at(q_desc, uniform(kPair ? w * L::kAtoms * L::kQAtom : 0u));
+                            const uint64_t k = smem_desc_at(k_desc, uniform(slot * L::kSlot));
+                            wait(bar_full + slot, L::parity(ahead));
                             tc_fence_after();
                             if (elect_one()) {
 #pragma unroll
-                                for (int j = half * (L::kHalf / kUmmaK); j < (half + 1) * (L::kHalf / kUmmaK); ++j) {
-                                    umma_bf16_ta(tmem + L::kTmemO + w * D, tmem + w * 128 + buffer * kKeys + j * 8,
-                                                 smem_desc_at(v, j * 2048u), o_idesc,
-                                                 (i > 0 || j > 0) ? 1u : 0u);
+                                for (int j = 0; j < D / kUmmaK; ++j) {
+                                    const uint32_t in = static_cast<uint32_t>(j & 3) * 32u;
+                                    umma_bf16(t_s, smem_desc_at(q, (j >> 2) * L::kQAtom + in),
+                                              smem_desc_at(k, (j >> 2) * L::kKvAtom + in), s_idesc, j > 0 ? 1u : 0u);
                                 }
-                                if (half == 1) {
-                                    umma_commit(bar_pv + 2 * w + buffer);
-                                    if (!kPair || w == chains - 1) {
-                                        umma_commit(bar_empty + slot);
-                                    }
+                                umma_commit(bar_s + 2 * w + buffer);
+                                if (!kPair || w == chains - 1) {
+                                    umma_commit(bar_empty + slot);
+                                }
+                                // The segment's last S: no chain has another tile.
+                                if (w == 0 ? i + L::kAhead >= mine1 && i + L::kAhead == mine0 - 1 : i + L::kAhead == mine0 - 1) {
+                                    umma_commit(bar_q_empty);
                                 }
                             }
                             __syncwarp();
                         }
-                        p_phase ^= 1u << (2 * w + buffer);
-                        if (more) {
-                            scores(w, i + L::kAhead);
-                        }
                     }
                 }
-#pragma unroll
-                for (int w = 0; w < kStreams; ++w) {
-                    n[w] += static_cast<uint32_t>(kPair ? count : mine[w]);
-                }
+                n0 += static_cast<uint32_t>(mine0);
+                n1 += static_cast<uint32_t>(kPair ? count : mine1);
             }
         }
     } else {  // ---- softmax: chain w, one thread per row
@@ -640,19 +659,29 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             wait(bar_pv + 2 * w + i % L::kAhead, (s_phase >> (i % L::kAhead) & 1u) ^ 1u);
             tc_fence_after();
         };
-        for (; segment(); advance(p, at, count, tiles)) {
-            if (w >= chains) {
-                n += kPair ? static_cast<uint32_t>(count) : 0u;
-                continue;
-            }
+        for (; segment(); next()) {
             const int token0 = r.first + (kPair ? w * p.tile_tokens : 0);
             const int t = token0 + token_in_tile;
             const bool inside = token_in_tile < p.tile_tokens && t < p.tokens;  // a row of ctx
+            bf16* ctx = p.ctx + ((at.b * p.tokens + t) * p.q_heads + at.h * p.group + g) * D;
+            float2* stats = p.stats + ((at.b * p.kv_heads + at.h) * p.tokens + t) * p.group + g;
+            if (w >= chains) {  // nothing to do in this segment, but for rows of padding
+                if (kPair && inside && tile0 == 0) {
+                    for (int c = 0; c < D; c += 16) {
+                        st_stream32(ctx + c, U8{});
+                    }
+                    if (p.stats != nullptr) {
+                        *stats = make_float2(0.0f, 0.0f);
+                    }
+                }
+                n += kPair ? static_cast<uint32_t>(count) : 0u;
+                continue;
+            }
             const bool valid = inside && t < r.valid;
             const bool busy = __any_sync(0xffffffffu, inside);
             const int limit = valid ? r.len + t + 1 : 0;
             const int part0 = r.full_end / kKeys * kKeys;  // first key of the first tile in which a key may be hidden
-            const bool hides = (at.tile + count) * kKeys > r.full_end;  // the segment has such tiles
+            const bool hides = (tile0 + count) * kKeys > r.full_end;  // the segment has such tiles
             const uint32_t* bits_row = nullptr;
             if (hides) {
                 if (row < 16) {
@@ -690,7 +719,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             for (int i = 0; i < mine; ++i) {
                 const uint32_t tile = n + static_cast<uint32_t>(i);
                 const int buffer = i % L::kAhead;
-                const int key0 = (at.tile + (kPair ? 0 : w) + i * L::kStep) * kKeys;
+                const int key0 = (tile0 + (kPair ? 0 : w) + i * L::kStep) * kKeys;
                 const bool partial = key0 + kKeys > r.full_end;
                 const uint32_t t_x = t_s + buffer * kKeys;
                 wait(bar_s + 2 * w + buffer, s_phase >> buffer & 1u);
@@ -736,13 +765,13 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 }
                 float2 offset = make_float2(0.0f, 0.0f);
                 float x[L::kHalf];
-                // The second half first, for its maximum alone: it is read again for its exponentials, which costs less
-                // than a row of registers.
                 if (busy) {
+                    // The second half first, for its maximum alone: it is read again for its exponentials, which costs
+                    // less than a row of registers. Scores that the row does not see are written back as -inf.
                     tmem_load_begin<L::kHalf>(t_x + L::kHalf, x);
                     tmem_load_end<L::kHalf>(x);
-                    if (partial) {
-                        hide(x, bits_row, key0 + L::kHalf, r.len, limit);
+                    if (partial && hide(x, bits_row, key0 + L::kHalf, r.len, limit)) {
+                        tmem_store(t_x + L::kHalf, x);
                     }
                     float new_top = largest(x, top);
                     tmem_load_begin<L::kHalf>(t_x, x);
@@ -779,9 +808,6 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 if (busy) {
                     tmem_load_begin<L::kHalf>(t_x + L::kHalf, x);
                     tmem_load_end<L::kHalf>(x);
-                    if (partial) {
-                        hide(x, bits_row, key0 + L::kHalf, r.len, limit);
-                    }
                     sum += probabilities(x, make_float2(c2, c2), offset, t_x + L::kHalf / 2);
                     tmem_store_wait();
                 }
@@ -823,7 +849,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 }
             }
             float scaled_top = top == -INFINITY ? -INFINITY : top * c2;
-            const bool whole = at.tile == 0 && count == tiles;
+            const bool whole = count == tiles;
             const bool joins = !kPair && chains == 2;  // the second chain's sums and O are the first's to add
             float f0 = 1.0f;
             float f1 = 0.0f;
@@ -847,7 +873,6 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 const int64_t part_row = static_cast<int64_t>(kPair ? w * 128 : 0) + row;
                 const int64_t part = 2 * static_cast<int64_t>(blockIdx.x) + (at.index == 0 ? 0 : 1);
-                bf16* ctx = p.ctx + ((at.b * p.tokens + t) * p.q_heads + at.h * p.group + g) * D;
                 float* part_o = p.part_o + part * D * p.part_rows + part_row * 4;
 #pragma unroll 1
                 for (int c = 0; c < D; c += 64) {
@@ -886,8 +911,8 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 if (inside && !whole) {
                     p.part_ml[part * p.part_rows + part_row] = make_float2(scaled_top, sum);
                 } else if (inside && p.stats != nullptr) {
-                    p.stats[((at.b * p.kv_heads + at.h) * p.tokens + t) * p.group + g] =
-                        valid ? make_float2(scaled_top == -INFINITY ? 0.0f : scaled_top, inv) : make_float2(0.0f, 0.0f);
+                    *stats = valid ? make_float2(scaled_top == -INFINITY ? 0.0f : scaled_top, inv)
+                                   : make_float2(0.0f, 0.0f);
                 }
             }
             tc_fence_before();
@@ -917,14 +942,15 @@ __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAt
     grid_dependency_begin();
     const int cut = static_cast<int>(blockIdx.x) + 1;
     const int4 where = p.cuts[cut];
-    const Cuts cuts(*p.line, ctas);
-    const int first = cuts.begin(cut) - where.w;  // the item's first tile on the line
-    if (cuts.empty(cut) || where.w == 0 || cuts.begin(cut - 1) > first) {
+    const int set_up = p.line[1];
+    const Cuts cuts(p.line[0], ctas);
+    const int first = cuts.begin(cut) - where.w;  // the item's first piece on the line
+    if (cuts.empty(cut) || where.w <= set_up || cuts.begin(cut - 1) > first + set_up) {
         return;
     }
     const ItemRange r = item_range(p, static_cast<int>(committed_rows(p, where.x)),
                                    static_cast<int>(valid_queries(p, where.x)), where.y);
-    const int last = cuts.of(first + item_tiles<kKeys>(r) - 1);  // parts before it are not empty
+    const int last = cuts.of(first + set_up + item_tiles<kKeys>(r) - 1);  // parts before it are not empty
     const int lane = threadIdx.x & 31;
     const int warp = threadIdx.x >> 5;
     const int row = static_cast<int>(blockIdx.y) * 32 + lane;
@@ -1424,10 +1450,10 @@ Plan plan(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads, int6
     pl.item_tokens = pl.tile_tokens * (pl.pair ? 2 : 1);
     pl.row_tiles = static_cast<int>(runtime::ceil_div(tokens, pl.item_tokens));
     pl.part_rows = pl.pair ? 2 * kBM : static_cast<int>((tokens < pl.tile_tokens ? tokens : pl.tile_tokens) * group);
-    const int64_t most = batch * pl.row_tiles * kv_heads * runtime::ceil_div(capacity, keys);  // of the line's tiles
+    const int64_t most = batch * pl.row_tiles * kv_heads * runtime::ceil_div(capacity, keys);  // tiles of the line
     pl.ctas = static_cast<int>(most < runtime::sm_count() ? most : runtime::sm_count());
     const int64_t products = batch * kv_heads * runtime::ceil_div(capacity, 128) * runtime::ceil_div(tokens, pl.tile_tokens);
-    pl.fits = most < (int64_t{1} << 31) && products < (int64_t{1} << 31);
+    pl.fits = most < (int64_t{1} << 29) && products < (int64_t{1} << 31);
     const auto up = [](int64_t n) { return (n + 127) / 128 * 128; };
     pl.cuts = 128;  // after the line's length
     pl.ml = pl.cuts + up(pl.ctas * static_cast<int64_t>(sizeof(int4)));
