@@ -30,6 +30,8 @@
 // before the softmax, and V tiles in which some row is hidden from some query are cleared of such values in shared
 // memory before the product (0 * NaN would be NaN); values that are not finite in a row that a query does see are added
 // to its O afterwards.
+#include <cmath>
+
 #include "common.cuh"
 #include "runtime.h"
 #include "tcgen05.cuh"
@@ -41,6 +43,7 @@ using namespace tc;
 
 constexpr int kMaxNodes = 256;  // drafted tokens of a sequence
 constexpr int kMaxGroup = 128;  // query heads of a key-value head
+constexpr int kMaxKeptRows = 16;  // rows of a head whose scores are kept for the weights
 
 struct CacheAttentionParams {
     const bf16* q;  // [B, T, Hq, D]
@@ -71,6 +74,8 @@ struct CacheAttentionParams {
     int* line;            // length of the line, pieces of an item before its tiles
     float2* part_ml;      // [2 CTAs][part_rows] (M in base 2, l)
     float* part_o;        // [2 CTAs][D / 4][part_rows][4]
+    float* scores;          // [B, Hkv][rows][score_stride] S of few rows, kept for the weights, or null
+    int64_t score_stride;
     unsigned int* tickets;  // [weight CTAs] parts of a unit that have been left, zeroed by the attention kernel
     float* part_sums;       // [2 weight CTAs][128]
     int weight_ctas;
@@ -292,6 +297,14 @@ __device__ __forceinline__ void tmem_store(uint32_t taddr, const float (&x)[N]) 
         tmem_store16(taddr + c * 16, r);
     }
     tmem_store_wait();
+}
+
+template <int N>
+__device__ __forceinline__ void keep(const float (&x)[N], float* to) {
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) {
+        *reinterpret_cast<float4*>(to + 4 * j) = make_float4(x[4 * j], x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+    }
 }
 
 template <int N>
@@ -678,6 +691,8 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 continue;
             }
             const bool valid = inside && t < r.valid;
+            // This row's scores, where they are kept.
+            float* scores = p.scores + ((at.b * p.kv_heads + at.h) * p.part_rows + row) * p.score_stride;
             const bool busy = __any_sync(0xffffffffu, inside);
             const int limit = valid ? r.len + t + 1 : 0;
             const int part0 = r.full_end / kKeys * kKeys;  // first key of the first tile in which a key may be hidden
@@ -773,11 +788,23 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                     if (partial && hide(x, bits_row, key0 + L::kHalf, r.len, limit)) {
                         tmem_store(t_x + L::kHalf, x);
                     }
+                    if (!kPair && p.scores != nullptr) {
+                        if (valid) {
+                            keep(x, scores + key0 + L::kHalf);
+                        }
+                        __syncwarp();
+                    }
                     float new_top = largest(x, top);
                     tmem_load_begin<L::kHalf>(t_x, x);
                     tmem_load_end<L::kHalf>(x);
                     if (partial) {
                         hide(x, bits_row, key0, r.len, limit);
+                    }
+                    if (!kPair && p.scores != nullptr) {
+                        if (valid) {
+                            keep(x, scores + key0);
+                        }
+                        __syncwarp();
                     }
                     new_top = largest(x, new_top);
                     const bool grown = i == 0 || (new_top - top) * c2 > 8.0f;
@@ -1422,6 +1449,48 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
     }
 }
 
+// The weights from kept scores: a thread takes four keys of a head and adds their probabilities over the head's rows.
+// Scores that a row does not see were kept as -inf.
+__global__ void __launch_bounds__(256) cache_weights_kept_kernel(const CacheAttentionParams p, float c2) {
+    __shared__ float2 s_stats[kMaxKeptRows];
+    grid_dependency_begin();
+    const unsigned blocks = static_cast<unsigned>((p.capacity + 1023) / 1024);  // of a head
+    const int64_t head = blockIdx.x / blocks;                                     // of all sequences
+    const int block = static_cast<int>(blockIdx.x % blocks);
+    const int64_t b = head / p.kv_heads;
+    const int valid = static_cast<int>(valid_queries(p, b));
+    const int end = valid > 0 ? static_cast<int>(committed_rows(p, b)) + valid : 0;
+    const int key = (block * 256 + static_cast<int>(threadIdx.x)) * 4;
+    const int rows = valid * p.group;
+    if (block * 1024 >= end) {
+        return;
+    }
+    if (static_cast<int>(threadIdx.x) < rows) {
+        s_stats[threadIdx.x] = p.stats[head * p.tokens * p.group + threadIdx.x];
+    }
+    __syncthreads();
+    float sum[4] = {};
+    if (key < end) {
+        const float* scores = p.scores + head * p.part_rows * p.score_stride + key;
+#pragma unroll 4
+        for (int i = 0; i < rows; ++i) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(scores + i * p.score_stride));
+            const float2 st = s_stats[i];
+            sum[0] = __fmaf_rn(exp2_approx(__fmaf_rn(x.x, c2, -st.x)), st.y, sum[0]);
+            sum[1] = __fmaf_rn(exp2_approx(__fmaf_rn(x.y, c2, -st.x)), st.y, sum[1]);
+            sum[2] = __fmaf_rn(exp2_approx(__fmaf_rn(x.z, c2, -st.x)), st.y, sum[2]);
+            sum[3] = __fmaf_rn(exp2_approx(__fmaf_rn(x.w, c2, -st.x)), st.y, sum[3]);
+        }
+    }
+    float* out = p.weights + head * p.capacity + key;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (key + j < end) {
+            out[j] += sum[j];
+        }
+    }
+}
+
 // The tiling of a call, and where its scratch lies (offsets in bytes; `bytes` in all).
 struct Plan {
     bool fits;         // the lines' lengths stay below 2^31
@@ -1436,6 +1505,8 @@ struct Plan {
     int64_t o;
     int64_t stats;
     int64_t sums;
+    int64_t scores;
+    int64_t score_stride;  // 0: K Q^T is formed again for the weights
     int64_t bytes;
     int weight_ctas;
 };
@@ -1461,8 +1532,16 @@ Plan plan(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads, int6
     pl.stats = pl.o + 2 * pl.ctas * pl.part_rows * head_dim * static_cast<int64_t>(sizeof(float));
     pl.bytes = pl.stats;
     if (with_stats) {
-        pl.weight_ctas = static_cast<int>(products < runtime::sm_count() ? products : runtime::sm_count());
         pl.sums = pl.stats + up(batch * tokens * q_heads * static_cast<int64_t>(sizeof(float2)));
+        // Keeping a key's scores for the weights moves 8 bytes for each row, mostly within L2; forming them again reads
+        // the key's 2 * head_dim bytes of K from memory and takes a tile's products.
+        if (tokens * group <= kMaxKeptRows) {
+            pl.score_stride = runtime::ceil_div(capacity, 128) * 128;
+            pl.scores = pl.sums;
+            pl.bytes = pl.scores + batch * kv_heads * pl.part_rows * pl.score_stride * static_cast<int64_t>(sizeof(float));
+            return pl;
+        }
+        pl.weight_ctas = static_cast<int>(products < runtime::sm_count() ? products : runtime::sm_count());
         // The parts of the units, then the tickets.
         pl.bytes = pl.sums + up(pl.weight_ctas * static_cast<int64_t>(2 * 128 * sizeof(float) + sizeof(unsigned int)));
     }
@@ -1592,6 +1671,8 @@ int run_attention(const char* op, CacheAttentionParams& p, int64_t head_dim, voi
     p.part_o = reinterpret_cast<float*>(base + pl.o);
     if (p.weights != nullptr) {
         p.stats = reinterpret_cast<float2*>(base + pl.stats);
+        p.scores = pl.score_stride > 0 ? reinterpret_cast<float*>(base + pl.scores) : nullptr;
+        p.score_stride = pl.score_stride;
         p.weight_ctas = pl.weight_ctas;
         p.part_sums = reinterpret_cast<float*>(base + pl.sums);
         p.tickets = reinterpret_cast<unsigned int*>(p.part_sums + pl.weight_ctas * 2 * 128);
@@ -1614,6 +1695,14 @@ int run_attention(const char* op, CacheAttentionParams& p, int64_t head_dim, voi
 }
 
 int run_weights(const char* op, const CacheAttentionParams& p, int64_t head_dim, cudaStream_t s) {
+    if (p.scores != nullptr) {
+        const float c2 = 1.4426950408889634f / std::sqrt(static_cast<float>(head_dim));
+        return runtime::launched(runtime::launch(cache_weights_kept_kernel,
+                                                 dim3(static_cast<unsigned>(runtime::ceil_div(p.capacity, 1024) *
+                                                                            p.batch * p.kv_heads)),
+                                                 dim3(256), s, 1u, p, c2),
+                                 op);
+    }
     const cudaError_t err = head_dim == 64    ? launch_cache_weights<64>(p, s)
                             : head_dim == 128 ? launch_cache_weights<128>(p, s)
                                               : launch_cache_weights<256>(p, s);
