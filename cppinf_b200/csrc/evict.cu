@@ -1,10 +1,13 @@
 // Eviction of cached rows by accumulated attention weight: of each sequence's rows, per key-value head, the first
 // `sinks`, the last `recent` and the heaviest of the others stay, `keep` in all, in their order.
 //
-// Two kernels. The first finds the kept rows: weights map to unsigned keys of the same order (NaN lowest, -0 as +0),
-// a radix select of four 8-bit digits finds the key of the last row that stays and how many rows of that very key do
-// (the lowest rows first), and one pass in row order writes the kept rows' indices and weights. The second copies the
-// kept K and V rows, one 16-byte vector per thread, and is bound by their bytes.
+// Two kernels. The first finds the kept rows, one CTA per sequence and head: weights map to unsigned keys of the same
+// order (NaN lowest, -0 as +0) that are read once into shared memory; a radix select of four 8-bit digits finds the key
+// of the last row that stays and how many rows of that very key do (the lowest rows first); then each thread counts the
+// kept rows of its own stretch of keys, one scan over the block places them, and their indices and weights are written.
+// Stretches are of odd length, so that the threads' reads fall on different banks. Its time is a chain of a few dozen
+// shared-memory round trips and barriers. The second copies the kept K and V rows, one 16-byte vector per thread and
+// step, the source rows of a CTA's share looked up once, and is bound by their bytes.
 #include "common.cuh"
 #include "runtime.h"
 
@@ -27,7 +30,6 @@ struct EvictParams {
     int64_t* index;           // [B, Hkv, keep]
     int64_t batch;
     int64_t kv_heads;
-    int64_t columns;          // 16-byte columns of a row
     int64_t capacity;
     int64_t keep;
     int64_t recent;
@@ -49,49 +51,37 @@ __device__ __forceinline__ uint32_t order_key(float w) {
     return (bits & 0x80000000u) != 0 ? ~bits : bits | 0x80000000u;
 }
 
-// Sum over the block of each thread's flag before the thread (exclusive prefix), with the total.
-__device__ __forceinline__ int block_rank(bool flag, int* warp_sums, int* total) {
-    const int lane = threadIdx.x & 31;
-    const int warp = threadIdx.x >> 5;
-    const unsigned who = __ballot_sync(0xffffffffu, flag);
-    if (lane == 0) {
-        warp_sums[warp] = __popc(who);
-    }
-    __syncthreads();
-    int before = 0;
-    int all = 0;
-    for (int w = 0; w < kSelectThreads / 32; ++w) {
-        const int n = warp_sums[w];
-        before += w < warp ? n : 0;
-        all += n;
-    }
-    __syncthreads();
-    *total = all;
-    return before + __popc(who & ((1u << lane) - 1u));
-}
+constexpr int kSharedKeys = 49152;  // keys of a head that fit into shared memory beside the rest
 
+// The kept rows of one head. Keys lie in shared memory, or, where the cache is too long for that, are formed again from
+// the weights each time.
+template <bool kShared>
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictParams p) {
+    extern __shared__ uint32_t s_keys[];
     __shared__ int histogram[256];
-    __shared__ int warp_sums[kSelectThreads / 32];
+    __shared__ unsigned long long warp_sums[kSelectThreads / 32];
     __shared__ uint32_t s_prefix;
     __shared__ int s_need;
     grid_dependency_begin();
     const int tid = threadIdx.x;
-    const int64_t h = blockIdx.x % p.kv_heads;
-    const int64_t b = blockIdx.x / p.kv_heads;
-    const int64_t len = cached_rows(p, b);
-    const float* w = p.weights + (b * p.kv_heads + h) * p.capacity;
-    float* w_out = p.weights_out + (b * p.kv_heads + h) * p.out_capacity;
-    int64_t* index = p.index + (b * p.kv_heads + h) * p.keep;
-    const int64_t left = len < p.keep ? len : p.keep;
-    if (h == 0 && tid == 0) {
+    const int lane = tid & 31;
+    const int warp = tid >> 5;
+    const int64_t head = blockIdx.x;  // of all sequences
+    const int64_t b = head / p.kv_heads;
+    const int len = static_cast<int>(cached_rows(p, b));
+    const float* w = p.weights + head * p.capacity;
+    float* w_out = p.weights_out + head * p.out_capacity;
+    int64_t* index = p.index + head * p.keep;
+    const int keep = static_cast<int>(p.keep);
+    const int left = len < keep ? len : keep;
+    if (head == b * p.kv_heads && tid == 0) {
         p.lengths_out[b] = left;
     }
-    for (int64_t i = left + tid; i < p.out_capacity; i += kSelectThreads) {
+    for (int i = left + tid; i < p.out_capacity; i += kSelectThreads) {
         w_out[i] = 0.0f;
     }
-    if (len <= p.keep) {
-        for (int64_t i = tid; i < p.keep; i += kSelectThreads) {
+    if (len <= keep) {
+        for (int i = tid; i < keep; i += kSelectThreads) {
             index[i] = i < len ? i : -1;
             if (i < len) {
                 w_out[i] = w[i];
@@ -99,87 +89,141 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
         }
         return;
     }
-    const int64_t lo = p.sinks;
-    const int64_t hi = len - p.recent;
+    const int sinks = static_cast<int>(p.sinks);
+    const int recent = static_cast<int>(p.recent);
+    const int n = len - sinks - recent;  // rows [sinks, sinks + n) are ranked
+    const float* ranked = w + sinks;
+    if (kShared) {
+#pragma unroll 8
+        for (int i = tid; i < n; i += kSelectThreads) {
+            s_keys[i] = order_key(ranked[i]);
+        }
+    }
+    const auto key_of = [&](int i) { return kShared ? s_keys[i] : order_key(ranked[i]); };
+    for (int i = tid; i < sinks; i += kSelectThreads) {
+        index[i] = i;
+        w_out[i] = w[i];
+    }
+    for (int i = tid; i < recent; i += kSelectThreads) {
+        index[keep - recent + i] = len - recent + i;
+        w_out[keep - recent + i] = w[len - recent + i];
+    }
     uint32_t prefix = 0;
     uint32_t known = 0;
-    int need = static_cast<int>(p.keep - p.sinks - p.recent);  // of the rows [lo, hi)
+    int need = keep - sinks - recent;
     for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += kSelectThreads) {
-            histogram[i] = 0;
+        if (tid < 256) {
+            histogram[tid] = 0;
         }
         __syncthreads();
-        for (int64_t i = lo + tid; i < hi; i += kSelectThreads) {
-            const uint32_t key = order_key(w[i]);
+#pragma unroll 4
+        for (int i = tid; i < n; i += kSelectThreads) {
+            const uint32_t key = key_of(i);
             if ((key & known) == prefix) {
                 atomicAdd(&histogram[(key >> shift) & 255u], 1);
             }
         }
         __syncthreads();
-        if (tid == 0) {
-            int above = 0;
-            int digit = 255;
-            while (digit > 0 && above + histogram[digit] < need) {
-                above += histogram[digit];
-                --digit;
+        if (warp == 0) {  // the digit at which the keys from the highest down reach `need`; eight digits a lane
+            int mine = 0;
+            for (int j = 0; j < 8; ++j) {
+                mine += histogram[255 - lane * 8 - j];
             }
-            s_prefix = prefix | (static_cast<uint32_t>(digit) << shift);
-            s_need = need - above;
+            int sum = mine;
+            for (int offset = 1; offset < 32; offset <<= 1) {
+                const int other = __shfl_up_sync(0xffffffffu, sum, offset);
+                sum += lane >= offset ? other : 0;
+            }
+            const unsigned reached = __ballot_sync(0xffffffffu, sum >= need);
+            if (reached != 0u && lane == __ffs(reached) - 1) {
+                int above = sum - mine;
+                int digit = 255 - lane * 8;
+                while (above + histogram[digit] < need) {
+                    above += histogram[digit];
+                    --digit;
+                }
+                s_prefix = prefix | (static_cast<uint32_t>(digit) << shift);
+                s_need = need - above;
+            }
         }
         __syncthreads();
         prefix = s_prefix;
         need = s_need;
         known |= 255u << shift;
     }
-    // Rows in order: those that stay are the fixed ones, keys above the last kept key, and the first `need` equal to it.
-    int64_t out = 0;
-    int equal = 0;
-    for (int64_t i0 = 0; i0 < len; i0 += kSelectThreads) {
-        const int64_t i = i0 + tid;
-        const bool inside = i < len;
-        const float value = inside ? w[i] : 0.0f;
-        const uint32_t key = order_key(value);
-        const bool ranked = inside && i >= lo && i < hi;
-        const bool tie = ranked && key == prefix;
-        int ties = 0;
-        const int tie_rank = equal + block_rank(tie, warp_sums, &ties);
-        const bool stays = inside && (!ranked || key > prefix || (tie && tie_rank < need));
-        int kept = 0;
-        const int64_t at = out + block_rank(stays, warp_sums, &kept);
-        if (stays) {
-            index[at] = i;
-            w_out[at] = value;
+    // Of the rows of key `prefix` the first `need` stay (none where no ranked row does), and all of higher keys.
+    const int stretch = ((n + kSelectThreads - 1) / kSelectThreads) | 1;
+    const int i0 = tid * stretch;
+    const int i1 = i0 + stretch < n ? i0 + stretch : n;
+    unsigned long long mine = 0;  // higher keys, and from bit 32 on equal ones
+    for (int i = i0; i < i1; ++i) {
+        const uint32_t key = key_of(i);
+        mine += key > prefix ? 1ull : (key == prefix ? 1ull << 32 : 0ull);
+    }
+    unsigned long long sum = mine;
+    for (int offset = 1; offset < 32; offset <<= 1) {
+        const unsigned long long other = __shfl_up_sync(0xffffffffu, sum, offset);
+        sum += lane >= offset ? other : 0ull;
+    }
+    if (lane == 31) {
+        warp_sums[warp] = sum;
+    }
+    __syncthreads();
+    sum -= mine;
+    for (int i = 0; i < warp; ++i) {
+        sum += warp_sums[i];
+    }
+    int equal = static_cast<int>(sum >> 32);
+    int out = sinks + static_cast<int>(sum & 0xffffffffull) + (equal < need ? equal : need);
+    for (int i = i0; i < i1; ++i) {
+        const uint32_t key = key_of(i);
+        const bool tie = key == prefix;
+        if (key > prefix || (tie && equal < need)) {
+            index[out] = sinks + i;
+            w_out[out] = ranked[i];
+            ++out;
         }
-        equal += ties;
-        out += kept;
+        equal += tie ? 1 : 0;
     }
 }
 
-__global__ void __launch_bounds__(256) evict_copy_kernel(const EvictParams p) {
+constexpr int kCopyThreads = 256;
+constexpr int kCopyRows = 32;  // kept rows of one head that a CTA copies
+
+__global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const EvictParams p, FastDiv columns, unsigned blocks) {
+    __shared__ int s_from[kCopyRows];
     grid_dependency_begin();
-    int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    const int64_t each = p.batch * p.out_capacity * p.kv_heads * p.columns;
-    if (i >= 2 * each) {
-        return;
-    }
-    const bool value = i >= each;
-    i -= value ? each : 0;
-    uint4* out = reinterpret_cast<uint4*>(value ? p.v_out : p.k_out) + i;
-    const int64_t column = i % p.columns;
-    i /= p.columns;
-    const int64_t h = i % p.kv_heads;
-    i /= p.kv_heads;
-    const int64_t row = i % p.out_capacity;
-    const int64_t b = i / p.out_capacity;
+    const unsigned head = blockIdx.x / blocks;  // of all sequences
+    const int row0 = static_cast<int>(blockIdx.x % blocks) * kCopyRows;
+    const int64_t b = head / static_cast<unsigned>(p.kv_heads);
+    const int64_t h = head % static_cast<unsigned>(p.kv_heads);
     const int64_t len = cached_rows(p, b);
-    uint4 data = make_uint4(0u, 0u, 0u, 0u);
-    if (row < (len < p.keep ? len : p.keep)) {
-        const int64_t from = p.index[(b * p.kv_heads + h) * p.keep + row];
-        const char* base = value ? p.v + b * p.vs[0] + from * p.vs[1] + h * p.vs[2]
-                                 : p.k + b * p.ks[0] + from * p.ks[1] + h * p.ks[2];
-        data = *reinterpret_cast<const uint4*>(base + column * 16);
+    const int left = static_cast<int>(len < p.keep ? len : p.keep);
+    if (threadIdx.x < kCopyRows) {
+        const int row = row0 + static_cast<int>(threadIdx.x);
+        s_from[threadIdx.x] = row < left ? static_cast<int>(p.index[head * p.keep + row]) : -1;
     }
-    *out = data;
+    __syncthreads();
+    const int rows = p.out_capacity - row0 < kCopyRows ? static_cast<int>(p.out_capacity - row0) : kCopyRows;
+    const unsigned vectors = static_cast<unsigned>(rows) * columns.d;
+    const char* k = p.k + b * p.ks[0] + h * p.ks[2];
+    const char* v = p.v + b * p.vs[0] + h * p.vs[2];
+    const int64_t out0 = ((b * p.out_capacity + row0) * p.kv_heads + h) * columns.d;
+#pragma unroll 4
+    for (unsigned i = threadIdx.x; i < vectors; i += kCopyThreads) {
+        const unsigned row = columns.quot(i);
+        const int64_t column = i - row * columns.d;
+        const int64_t from = s_from[row];
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        uint4 y = x;
+        if (from >= 0) {
+            x = ld_stream(k + from * p.ks[1] + column * 16);
+            y = ld_stream(v + from * p.vs[1] + column * 16);
+        }
+        const int64_t to = out0 + row * p.kv_heads * columns.d + column;
+        st_v4(reinterpret_cast<uint4*>(p.k_out) + to, x);
+        st_v4(reinterpret_cast<uint4*>(p.v_out) + to, y);
+    }
 }
 
 }  // namespace
@@ -209,8 +253,7 @@ int cppinf_cache_evict(cppinf_dtype dtype, const void* k_cache, const int64_t* k
     constexpr int64_t kMost = int64_t{1} << 31;
     CPPINF_REQUIRE(capacity < kMost && out_capacity < kMost && batch < (1 << 24) && kv_heads < (1 << 16) &&
                        head_dim < (1 << 16) && batch * kv_heads < kMost &&
-                       (batch * kv_heads == 0 || head_dim == 0 ||
-                        out_capacity < (int64_t{1} << 38) / (batch * kv_heads * head_dim)),
+                       (batch * kv_heads == 0 || rt::ceil_div(out_capacity, kCopyRows) < kMost / (batch * kv_heads)),
                    CPPINF_ERR_OVERFLOW, "cache_evict sizes exceed the launch range.");
     if (batch == 0 || kv_heads == 0 || head_dim == 0) {
         return rt::ok();
@@ -240,22 +283,31 @@ int cppinf_cache_evict(cppinf_dtype dtype, const void* k_cache, const int64_t* k
     p.index = index;
     p.batch = batch;
     p.kv_heads = kv_heads;
-    p.columns = head_dim * size / 16;
     p.capacity = capacity;
     p.keep = keep;
     p.recent = recent;
     p.sinks = sinks;
     p.out_capacity = out_capacity;
     const cudaStream_t s = rt::as_stream(stream);
-    if (const int st = rt::launched(rt::launch(evict_select_kernel, dim3(static_cast<unsigned>(batch * kv_heads)),
-                                               dim3(kSelectThreads), s, 1u, p),
-                                    "cache_evict selection");
-        st != CPPINF_OK) {
+    const unsigned heads = static_cast<unsigned>(batch * kv_heads);
+    cudaError_t err = cudaSuccess;
+    if (capacity <= kSharedKeys) {
+        const std::size_t bytes = static_cast<std::size_t>(capacity) * sizeof(uint32_t);
+        if (bytes > 40960) {  // beside the kernel's own arrays, more than a CTA has without asking
+            CPPINF_CUDA_TRY(cudaFuncSetAttribute(evict_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 static_cast<int>(kSharedKeys * sizeof(uint32_t))));
+        }
+        err = rt::launch_smem(evict_select_kernel<true>, dim3(heads), dim3(kSelectThreads), bytes, s, 1u, p);
+    } else {
+        err = rt::launch(evict_select_kernel<false>, dim3(heads), dim3(kSelectThreads), s, 1u, p);
+    }
+    if (const int st = rt::launched(err, "cache_evict selection"); st != CPPINF_OK) {
         return st;
     }
-    const int64_t vectors = 2 * batch * out_capacity * kv_heads * p.columns;
-    return rt::launched(rt::launch(evict_copy_kernel, dim3(static_cast<unsigned>(rt::ceil_div(vectors, 256))), dim3(256),
-                                   s, 1u, p),
+    const int64_t blocks = rt::ceil_div(out_capacity, kCopyRows);
+    return rt::launched(rt::launch(evict_copy_kernel, dim3(static_cast<unsigned>(blocks * heads)), dim3(kCopyThreads), s,
+                                   1u, p, FastDiv(static_cast<uint32_t>(head_dim * size / 16)),
+                                   static_cast<unsigned>(blocks)),
                         "cache_evict copy");
 }
 
