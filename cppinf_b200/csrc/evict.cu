@@ -2,8 +2,9 @@
 // `sinks`, the last `recent` and the heaviest of the others stay, `keep` in all, in their order.
 //
 // Two kernels. The first finds the kept rows, one CTA per sequence and head: weights map to unsigned keys of the same
-// order (NaN lowest, -0 as +0) that are read once into shared memory; a radix select of four 8-bit digits finds the key
-// of the last row that stays and how many rows of that very key do (the lowest rows first); then each thread counts the
+// order (NaN lowest, -0 as +0) that are read once into shared memory; a radix select of three digits finds the key of the
+// last row that stays and how many rows of that very key do (the lowest rows first; digits of 11 bits, since weights
+// have few exponents and the counters of a shorter digit are hit by many threads at once); then each thread counts the
 // kept rows of its own stretch of keys, one scan over the block places them, and their indices and weights are written.
 // Stretches are of odd length, so that the threads' reads fall on different banks. Its time is a chain of a few dozen
 // shared-memory round trips and barriers. The second copies the kept K and V rows, one 16-byte vector per thread and
@@ -51,6 +52,7 @@ __device__ __forceinline__ uint32_t order_key(float w) {
     return (bits & 0x80000000u) != 0 ? ~bits : bits | 0x80000000u;
 }
 
+constexpr int kDigits = 2048;       // values of a digit
 constexpr int kSharedKeys = 49152;  // keys of a head that fit into shared memory beside the rest
 
 // The kept rows of one head. Keys lie in shared memory, or, where the cache is too long for that, are formed again from
@@ -58,7 +60,7 @@ constexpr int kSharedKeys = 49152;  // keys of a head that fit into shared memor
 template <bool kShared>
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictParams p) {
     extern __shared__ uint32_t s_keys[];
-    __shared__ int histogram[256];
+    __shared__ int histogram[kDigits];
     __shared__ unsigned long long warp_sums[kSelectThreads / 32];
     __shared__ uint32_t s_prefix;
     __shared__ int s_need;
@@ -111,45 +113,49 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     uint32_t prefix = 0;
     uint32_t known = 0;
     int need = keep - sinks - recent;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) {
-            histogram[tid] = 0;
-        }
+    if (need == 0) {
+        return;
+    }
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t digits = pass == 2 ? 1023u : 2047u;
+        histogram[tid] = 0;
+        histogram[tid + kSelectThreads] = 0;
         __syncthreads();
 #pragma unroll 4
         for (int i = tid; i < n; i += kSelectThreads) {
             const uint32_t key = key_of(i);
             if ((key & known) == prefix) {
-                atomicAdd(&histogram[(key >> shift) & 255u], 1);
+                atomicAdd(&histogram[(key >> shift) & digits], 1);
             }
         }
         __syncthreads();
-        if (warp == 0) {  // the digit at which the keys from the highest down reach `need`; eight digits a lane
-            int mine = 0;
-            for (int j = 0; j < 8; ++j) {
-                mine += histogram[255 - lane * 8 - j];
-            }
-            int sum = mine;
-            for (int offset = 1; offset < 32; offset <<= 1) {
-                const int other = __shfl_up_sync(0xffffffffu, sum, offset);
-                sum += lane >= offset ? other : 0;
-            }
-            const unsigned reached = __ballot_sync(0xffffffffu, sum >= need);
-            if (reached != 0u && lane == __ffs(reached) - 1) {
-                int above = sum - mine;
-                int digit = 255 - lane * 8;
-                while (above + histogram[digit] < need) {
-                    above += histogram[digit];
-                    --digit;
-                }
-                s_prefix = prefix | (static_cast<uint32_t>(digit) << shift);
-                s_need = need - above;
-            }
+        // The digit at which the keys from the highest down reach `need`; a thread has two digits.
+        const int digit = kDigits - 1 - 2 * tid;
+        const int upper = histogram[digit];
+        const int mine = upper + histogram[digit - 1];
+        int sum = mine;
+        for (int offset = 1; offset < 32; offset <<= 1) {
+            const int other = __shfl_up_sync(0xffffffffu, sum, offset);
+            sum += lane >= offset ? other : 0;
+        }
+        if (lane == 31) {
+            warp_sums[warp] = static_cast<unsigned long long>(sum);
+        }
+        __syncthreads();
+        int above = sum - mine;
+        for (int i = 0; i < warp; ++i) {
+            above += static_cast<int>(warp_sums[i]);
+        }
+        if (above < need && above + mine >= need) {
+            const bool first = above + upper >= need;
+            s_prefix = prefix | (static_cast<uint32_t>(first ? digit : digit - 1) << shift);
+            s_need = need - above - (first ? 0 : upper);
         }
         __syncthreads();
         prefix = s_prefix;
         need = s_need;
-        known |= 255u << shift;
+        known |= digits << shift;
     }
     // Of the rows of key `prefix` the first `need` stay (none where no ranked row does), and all of higher keys.
     const int stretch = ((n + kSelectThreads - 1) / kSelectThreads) | 1;

@@ -3,13 +3,13 @@
 //
 // tree_accept: node 0 is the token the model produced last; from an accepted node p the walk goes to the child c of p
 // with token[c] == predicted[p] (the lowest index where drafts repeat), and ends where there is none; the model's own
-// token after the last accepted node is the next one. The walk is a chain of dependent steps, so it is bound by the
-// latency of one step: a warp per sequence holds its nodes in shared memory, and each step is one ballot per 32 nodes
-// above the current one.
+// token after the last accepted node is the next one. Whether a node would follow its parent depends on the two alone, so
+// one warp per sequence first gives every node its following child, the minimum over its children in shared memory; the
+// walk is then one shared-memory load per step. Bound by the latency of two dependent global loads.
 //
 // tree_commit: cache row len + i takes row len + path[i]. A path ascends from path[i] >= i, so going through it in
-// order never overwrites a row that is still to be read; every 16-byte column of a head's rows is one thread's, and the
-// columns of all sequences, heads and both caches run side by side.
+// order never overwrites a row that is still to be read; every 16-byte column of a head's rows is one thread's, which
+// loads eight rows before it stores them, and the columns of all sequences, heads and both caches run side by side.
 #include "common.cuh"
 #include "runtime.h"
 
@@ -21,6 +21,8 @@ constexpr int kMaxNodes = 256;
 __global__ void __launch_bounds__(32)
     tree_accept_kernel(const int64_t* tokens, const int64_t* parents, const int64_t* predicted, const int64_t* nodes,
                        int64_t* path, int64_t* counts, int64_t* next, int t) {
+    __shared__ int64_t s_predicted[kMaxNodes];
+    __shared__ int s_following[kMaxNodes];
     grid_dependency_begin();
     const int lane = threadIdx.x;
     const int64_t b = blockIdx.x;
@@ -30,30 +32,35 @@ __global__ void __launch_bounds__(32)
     path += b * t;
     int64_t n = nodes == nullptr ? t : nodes[b];
     n = n < 0 ? 0 : (n > t ? t : n);
-    int at = n > 0 ? 0 : -1;
-    int count = 0;
-    int64_t following = -1;
-    while (at >= 0) {
-        if (lane == 0) {
-            path[count] = at;
+    int64_t token[kMaxNodes / 32];
+    int64_t parent[kMaxNodes / 32];
+#pragma unroll
+    for (int i = 0; i < kMaxNodes / 32; ++i) {
+        const int c = i * 32 + lane;
+        if (c < t) {
+            token[i] = tokens[c];
+            parent[i] = parents[c];
+            s_predicted[c] = predicted[c];
+            s_following[c] = kMaxNodes;
+            path[c] = -1;
         }
-        ++count;
-        following = predicted[at];
-        int found = -1;
-        for (int c0 = at + 1; c0 < n && found < 0; c0 += 32) {
-            const int c = c0 + lane;
-            const bool fits = c < n && parents[c] == at && tokens[c] == following;
-            const unsigned who = __ballot_sync(0xffffffffu, fits);
-            if (who != 0) {
-                found = c0 + __ffs(who) - 1;
-            }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < kMaxNodes / 32; ++i) {
+        const int c = i * 32 + lane;
+        if (c < n && parent[i] >= 0 && parent[i] < c && token[i] == s_predicted[parent[i]]) {
+            atomicMin(&s_following[parent[i]], c);
         }
-        at = found;
     }
-    for (int i = count + lane; i < t; i += 32) {
-        path[i] = -1;
-    }
+    __syncwarp();
     if (lane == 0) {
+        int count = 0;
+        int64_t following = -1;
+        for (int at = n > 0 ? 0 : kMaxNodes; at < kMaxNodes; at = s_following[at]) {
+            path[count++] = at;
+            following = s_predicted[at];
+        }
         counts[b] = count;
         next[b] = following;
     }
@@ -86,18 +93,32 @@ __global__ void __launch_bounds__(128) tree_commit_kernel(const CommitParams p) 
     i /= p.kv_heads;
     const bool value = (i & 1) != 0;
     const int64_t b = i >> 1;
+    const int64_t* path = p.path + b * p.tokens;
     int64_t len = p.lengths[b];
+    int64_t n = p.counts[b];
     len = len < 0 ? 0 : (len > p.capacity ? p.capacity : len);
     const int64_t drafted = p.tokens < p.capacity - len ? p.tokens : p.capacity - len;  // rows inside the cache
-    int64_t n = p.counts[b];
     n = n < 0 ? 0 : (n > drafted ? drafted : n);
     const int64_t stride = value ? p.vs[1] : p.ks[1];
     char* rows = value ? p.v + b * p.vs[0] + h * p.vs[2] : p.k + b * p.ks[0] + h * p.ks[2];
     rows += len * stride + column * 16;
-    for (int64_t to = 0; to < n; ++to) {
-        const int64_t from = p.path[b * p.tokens + to];
-        if (from > to && from < drafted) {
-            *reinterpret_cast<uint4*>(rows + to * stride) = *reinterpret_cast<const uint4*>(rows + from * stride);
+    constexpr int kBatch = 8;
+    for (int64_t to = 0; to < n; to += kBatch) {
+        uint4 x[kBatch];
+        bool moves[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int64_t from = to + j < n ? path[to + j] : 0;
+            moves[j] = from > to + j && from < drafted;
+            if (moves[j]) {
+                x[j] = *reinterpret_cast<const uint4*>(rows + from * stride);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            if (moves[j]) {
+                *reinterpret_cast<uint4*>(rows + (to + j) * stride) = x[j];
+            }
         }
     }
 }
