@@ -2,7 +2,7 @@
 // `sinks`, the last `recent` and the heaviest of the others stay, `keep` in all, in their order.
 //
 // Two kernels. The first finds the kept rows, one CTA per sequence and head: weights map to unsigned keys of the same
-// order (NaN lowest, -0 as +0) that are read once into shared memory; a radix select of three digits finds the key of the
+// order (NaN lowest, -0 as +0), the weights read once into shared memory; a radix select of three digits finds the key of the
 // last row that stays and how many rows of that very key do (the lowest rows first; digits of 11 bits, since weights
 // have few exponents and the counters of a shorter digit are hit by many threads at once); then each thread counts the
 // kept rows of its own stretch of keys, one scan over the block places them, and their indices and weights are written.
@@ -53,15 +53,16 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 }
 
 constexpr int kDigits = 2048;       // values of a digit
-constexpr int kSharedKeys = 49152;  // keys of a head that fit into shared memory beside the rest
+constexpr int kSharedKeys = 49152;  // weights of a head that fit into shared memory beside the rest
 
-// The kept rows of one head. Keys lie in shared memory, or, where the cache is too long for that, are formed again from
-// the weights each time.
+// The kept rows of one head. The weights lie in shared memory, or, where the cache is too long for that, are read again
+// each time; their keys cost a few instructions.
 template <bool kShared>
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictParams p) {
-    extern __shared__ uint32_t s_keys[];
+    extern __shared__ float s_weights[];
     __shared__ int histogram[kDigits];
-    __shared__ unsigned long long warp_sums[kSelectThreads / 32];
+    __shared__ int warp_sums[kSelectThreads / 32];
+    __shared__ int warp_ties[kSelectThreads / 32];
     __shared__ uint32_t s_prefix;
     __shared__ int s_need;
     grid_dependency_begin();
@@ -98,10 +99,11 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     if (kShared) {
 #pragma unroll 8
         for (int i = tid; i < n; i += kSelectThreads) {
-            s_keys[i] = order_key(ranked[i]);
+            s_weights[i] = ranked[i];
         }
     }
-    const auto key_of = [&](int i) { return kShared ? s_keys[i] : order_key(ranked[i]); };
+    const auto weight_of = [&](int i) { return kShared ? s_weights[i] : ranked[i]; };
+    const auto key_of = [&](int i) { return order_key(weight_of(i)); };
     for (int i = tid; i < sinks; i += kSelectThreads) {
         index[i] = i;
         w_out[i] = w[i];
@@ -140,13 +142,10 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
             sum += lane >= offset ? other : 0;
         }
         if (lane == 31) {
-            warp_sums[warp] = static_cast<unsigned long long>(sum);
+            warp_sums[warp] = sum;
         }
         __syncthreads();
-        int above = sum - mine;
-        for (int i = 0; i < warp; ++i) {
-            above += static_cast<int>(warp_sums[i]);
-        }
+        const int above = sum - mine + __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[lane] : 0);
         if (above < need && above + mine >= need) {
             const bool first = above + upper >= need;
             s_prefix = prefix | (static_cast<uint32_t>(first ? digit : digit - 1) << shift);
@@ -161,32 +160,36 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     const int stretch = ((n + kSelectThreads - 1) / kSelectThreads) | 1;
     const int i0 = tid * stretch;
     const int i1 = i0 + stretch < n ? i0 + stretch : n;
-    unsigned long long mine = 0;  // higher keys, and from bit 32 on equal ones
+    int higher = 0;
+    int ties = 0;
     for (int i = i0; i < i1; ++i) {
         const uint32_t key = key_of(i);
-        mine += key > prefix ? 1ull : (key == prefix ? 1ull << 32 : 0ull);
+        higher += key > prefix ? 1 : 0;
+        ties += key == prefix ? 1 : 0;
     }
-    unsigned long long sum = mine;
+    int out = higher;  // becomes the number before the thread's stretch, as `equal` does of the ties
+    int equal = ties;
     for (int offset = 1; offset < 32; offset <<= 1) {
-        const unsigned long long other = __shfl_up_sync(0xffffffffu, sum, offset);
-        sum += lane >= offset ? other : 0ull;
+        const int a = __shfl_up_sync(0xffffffffu, out, offset);
+        const int b = __shfl_up_sync(0xffffffffu, equal, offset);
+        out += lane >= offset ? a : 0;
+        equal += lane >= offset ? b : 0;
     }
     if (lane == 31) {
-        warp_sums[warp] = sum;
+        warp_sums[warp] = out;
+        warp_ties[warp] = equal;
     }
     __syncthreads();
-    sum -= mine;
-    for (int i = 0; i < warp; ++i) {
-        sum += warp_sums[i];
-    }
-    int equal = static_cast<int>(sum >> 32);
-    int out = sinks + static_cast<int>(sum & 0xffffffffull) + (equal < need ? equal : need);
+    out += __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[lane] : 0) - higher;
+    equal += __reduce_add_sync(0xffffffffu, lane < warp ? warp_ties[lane] : 0) - ties;
+    out += sinks + (equal < need ? equal : need);
     for (int i = i0; i < i1; ++i) {
-        const uint32_t key = key_of(i);
+        const float weight = weight_of(i);
+        const uint32_t key = order_key(weight);
         const bool tie = key == prefix;
         if (key > prefix || (tie && equal < need)) {
             index[out] = sinks + i;
-            w_out[out] = ranked[i];
+            w_out[out] = weight;
             ++out;
         }
         equal += tie ? 1 : 0;
