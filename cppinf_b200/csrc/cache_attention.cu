@@ -30,6 +30,7 @@
 // before the softmax, and V tiles in which some row is hidden from some query are cleared of such values in shared
 // memory before the product (0 * NaN would be NaN); values that are not finite in a row that a query does see are added
 // to its O afterwards.
+#include <atomic>
 #include <cmath>
 
 #include "common.cuh"
@@ -69,6 +70,7 @@ struct CacheAttentionParams {
     int item_tokens;      // tokens of an item: one or two tiles
     int row_tiles;        // items along the tokens
     int q_box_tokens;     // tokens of one TMA box of q
+    bool whole_items;     // the line is cut between items only
     int part_rows;        // rows of a part in the scratch
     int4* cuts;           // [CTAs] where each CTA's part of the line begins: sequence, row tile, head, piece
     int* line;            // length of the line, pieces of an item before its tiles
@@ -176,6 +178,8 @@ constexpr uint32_t kTmemAll = 512;
 // where CTAs have few tiles each and a set-up's place would be better taken by a tile.
 constexpr int kSetUp = 3;
 constexpr int kSetUpFrom = 8;  // tiles per CTA
+// Items of up to so many key tiles are not cut at all (a piece is then an item): nothing is left to join.
+constexpr int kWholeTiles = 8;
 
 // Where a CTA's part of the line is, item by item; every role of the CTA walks it for itself.
 struct Walk {
@@ -191,8 +195,7 @@ struct Walk {
 };
 
 __device__ __forceinline__ void advance(const CacheAttentionParams& p, Walk& w, int tiles) {
-    const int pieces = tiles + w.set_up - w.piece;
-    w.left -= pieces;
+    w.left -= p.whole_items ? 1 : tiles + w.set_up - w.piece;
     w.piece = 0;
     if (w.left <= 0 || ++w.h < static_cast<int>(p.kv_heads)) {
         return;
@@ -413,7 +416,8 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             return w;
         };
         const auto tiles_of = [&](int e, const Walk& w) {
-            return e < entries ? item_tiles<kKeys>(item_range(p, w.len, w.valid, w.row_tile)) * heads : 0;
+            const int each = p.whole_items ? 1 : item_tiles<kKeys>(item_range(p, w.len, w.valid, w.row_tile));
+            return e < entries ? each * heads : 0;
         };
         Walk w = entry(lane);
         int mine = tiles_of(lane, w);
@@ -422,7 +426,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             total += tiles_of(e, entry(e));
         }
         total = __reduce_add_sync(0xffffffffu, total);
-        const int set_up = total / kSetUpFrom >= static_cast<int>(gridDim.x) ? kSetUp : 0;
+        const int set_up = !p.whole_items && total / kSetUpFrom >= static_cast<int>(gridDim.x) ? kSetUp : 0;
         total += set_up * heads * entries;
         const Cuts cuts(total, static_cast<int>(gridDim.x));
         const int begin = cuts.begin(static_cast<int>(blockIdx.x));
@@ -489,7 +493,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             r = item_range(p, at.len, at.valid, at.row_tile);
             tiles = item_tiles<kKeys>(r);
             tile0 = at.piece > at.set_up ? at.piece - at.set_up : 0;
-            const int end = at.piece + at.left - at.set_up;
+            const int end = p.whole_items ? tiles : at.piece + at.left - at.set_up;
             count = (end < tiles ? end : tiles) - tile0;
             if (count > 0) {
                 break;
@@ -1495,6 +1499,7 @@ __global__ void __launch_bounds__(256) cache_weights_kept_kernel(const CacheAtte
 struct Plan {
     bool fits;         // the lines' lengths stay below 2^31
     bool pair;         // two row tiles on each K and V tile
+    bool whole_items;  // no item has enough key tiles to be cut
     int ctas;
     int tile_tokens;
     int item_tokens;
@@ -1522,14 +1527,17 @@ Plan plan(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads, int6
     pl.row_tiles = static_cast<int>(runtime::ceil_div(tokens, pl.item_tokens));
     pl.part_rows = pl.pair ? 2 * kBM : static_cast<int>((tokens < pl.tile_tokens ? tokens : pl.tile_tokens) * group);
     const int64_t most = batch * pl.row_tiles * kv_heads * runtime::ceil_div(capacity, keys);  // tiles of the line
-    pl.ctas = static_cast<int>(most < runtime::sm_count() ? most : runtime::sm_count());
+    pl.whole_items = runtime::ceil_div(capacity, keys) <= kWholeTiles;
+    const int64_t pieces = pl.whole_items ? batch * pl.row_tiles * kv_heads : most;
+    pl.ctas = static_cast<int>(pieces < runtime::sm_count() ? pieces : runtime::sm_count());
     const int64_t products = batch * kv_heads * runtime::ceil_div(capacity, 128) * runtime::ceil_div(tokens, pl.tile_tokens);
     pl.fits = most < (int64_t{1} << 29) && products < (int64_t{1} << 31);
     const auto up = [](int64_t n) { return (n + 127) / 128 * 128; };
     pl.cuts = 128;  // after the line's length
+    const int64_t parts = pl.whole_items ? 0 : 2 * pl.ctas;
     pl.ml = pl.cuts + up(pl.ctas * static_cast<int64_t>(sizeof(int4)));
-    pl.o = pl.ml + up(2 * pl.ctas * pl.part_rows * static_cast<int64_t>(sizeof(float2)));
-    pl.stats = pl.o + 2 * pl.ctas * pl.part_rows * head_dim * static_cast<int64_t>(sizeof(float));
+    pl.o = pl.ml + up(parts * pl.part_rows * static_cast<int64_t>(sizeof(float2)));
+    pl.stats = pl.o + parts * pl.part_rows * head_dim * static_cast<int64_t>(sizeof(float));
     pl.bytes = pl.stats;
     if (with_stats) {
         pl.sums = pl.stats + up(batch * tokens * q_heads * static_cast<int64_t>(sizeof(float2)));
@@ -1570,6 +1578,25 @@ bool encode_4d(CUtensorMap* map, const void* base, const int64_t (&dims)[4], con
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// A kernel's limit of dynamic shared memory, raised once on each device (the call costs a microsecond).
+struct SharedMemoryLimit {
+    std::atomic<uint64_t> raised{0};  // a bit for each of the first 64 devices
+
+    template <typename Kernel>
+    cudaError_t raise(Kernel kernel, std::size_t bytes) {
+        int device = 0;
+        cudaError_t err = cudaGetDevice(&device);
+        const uint64_t bit = device < 64 ? uint64_t{1} << device : 0;
+        if (err == cudaSuccess && (raised.load(std::memory_order_acquire) & bit) == 0) {
+            err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+            if (err == cudaSuccess) {
+                raised.fetch_or(bit, std::memory_order_release);
+            }
+        }
+        return err;
+    }
+};
+
 template <int D, bool kPair>
 cudaError_t launch_cache_attention(const CacheAttentionParams& p, const Plan& pl, cudaStream_t s) {
     using L = Tiling<D, kPair>;
@@ -1582,14 +1609,14 @@ cudaError_t launch_cache_attention(const CacheAttentionParams& p, const Plan& pl
         !encode_4d(&mv, p.v, {D, p.kv_heads, p.capacity, p.batch}, {p.vs[2], p.vs[1], p.vs[0]}, {64, 1, L::kKeys, 1})) {
         return cudaErrorInvalidValue;
     }
-    cudaError_t err = cudaFuncSetAttribute(cache_attention_kernel<D, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           static_cast<int>(L::kBytes));
+    static SharedMemoryLimit limit;
+    cudaError_t err = limit.raise(cache_attention_kernel<D, kPair>, L::kBytes);
     if (err != cudaSuccess) {
         return err;
     }
     err = runtime::launch_smem(cache_attention_kernel<D, kPair>, dim3(static_cast<unsigned>(pl.ctas)),
                                dim3(L::kThreads), L::kBytes, s, 1u, mq, mk, mv, p);
-    if (err != cudaSuccess || pl.ctas == 1) {
+    if (err != cudaSuccess || pl.ctas == 1 || pl.whole_items) {
         return err;
     }
     runtime::count_launches(1);
@@ -1608,8 +1635,8 @@ cudaError_t launch_cache_weights(const CacheAttentionParams& p, cudaStream_t s) 
         !encode_4d(&mk, p.k, {D, p.kv_heads, p.capacity, p.batch}, {p.ks[2], p.ks[1], p.ks[0]}, {64, 1, 128, 1})) {
         return cudaErrorInvalidValue;
     }
-    const cudaError_t err = cudaFuncSetAttribute(cache_weights_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 static_cast<int>(L::kBytes));
+    static SharedMemoryLimit limit;
+    const cudaError_t err = limit.raise(cache_weights_kernel<D>, L::kBytes);
     if (err != cudaSuccess) {
         return err;
     }
@@ -1664,6 +1691,7 @@ int run_attention(const char* op, CacheAttentionParams& p, int64_t head_dim, voi
     p.item_tokens = pl.item_tokens;
     p.row_tiles = pl.row_tiles;
     p.q_box_tokens = static_cast<int>(p.tokens < pl.tile_tokens ? p.tokens : pl.tile_tokens);
+    p.whole_items = pl.whole_items;
     p.part_rows = pl.part_rows;
     p.line = reinterpret_cast<int*>(base);
     p.cuts = reinterpret_cast<int4*>(base + pl.cuts);

@@ -11,6 +11,8 @@ RMSNorm + RoPE), the row argmax of the greedy sampler, and the position-aware ca
 
 from __future__ import annotations
 
+import ctypes
+import functools
 import math
 import threading
 
@@ -456,20 +458,42 @@ def decoder_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
 # ---- batches of cached sequences: drafted trees, attention weights, eviction -------------------------------------
 
 
-def _same_device(op: str, *tensors: torch.Tensor | None) -> torch.device:
-    first = tensors[0]
+class _On:
+    """The tensors' device as the current one, for calls made while another is (entering torch.cuda.device always costs
+    more than the comparison)."""
+
+    __slots__ = ("index", "other")
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self) -> int:
+        self.other = None
+        if torch.cuda.current_device() != self.index:
+            self.other = torch.cuda.device(self.index)
+            self.other.__enter__()
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc) -> None:
+        if self.other is not None:
+            self.other.__exit__(*exc)
+
+
+def _same_device(op: str, *tensors: torch.Tensor | None) -> int:
+    first = tensors[0].get_device()
     for t in tensors:
-        if t is not None:
-            _require_cuda(t)
-            if t.device != first.device:
-                raise ValueError(f"{op} requires all tensors on one device.")
-    return first.device
+        if t is not None and t.get_device() != first:
+            _require_cuda(t, tensors[0])
+            raise ValueError(f"{op} requires all tensors on one device.")
+    if first < 0 or not tensors[0].is_cuda:
+        _require_cuda(*(t for t in tensors if t is not None))
+    return first
 
 
 def _row_counts(t: torch.Tensor | None, batch: int, op: str, name: str) -> torch.Tensor | None:
     if t is None:
         return None
-    if t.dtype != torch.int64 or t.shape != (batch,):
+    if t.dtype != torch.int64 or t.dim() != 1 or t.shape[0] != batch:
         raise ValueError(f"{op} requires int64 {name} of one per sequence.")
     return t.contiguous()
 
@@ -478,14 +502,17 @@ def _cache_strides(t: torch.Tensor) -> tuple[int, int, int] | None:
     """Element strides {batch, row, head} of a cache that the kernels can read and write in place, else None. The
     stride of a dimension of one entry is never followed and is given as if the tensor were dense."""
     b, n, h, d = t.shape
-    if t.stride(3) != 1 and d != 1:
+    sb, sn, sh, sd = t.stride()
+    if sd != 1 and d != 1:
         return None
-    sb, sn, sh = t.stride()[:3]
-    sh = sh if h > 1 else d
-    sn = sn if n > 1 else h * sh
-    sb = sb if b > 1 else n * sn
+    if h <= 1:
+        sh = d
+    if n <= 1:
+        sn = h * sh
+    if b <= 1:
+        sb = n * sn
     vec = 16 // t.element_size()
-    if sh < d or min(sb, sn) < d or (sb | sn | sh) % vec or t.data_ptr() % 16:
+    if sh < d or sb < d or sn < d or (sb | sn | sh) % vec or t.data_ptr() % 16:
         return None
     return sb, sn, sh
 
@@ -497,12 +524,15 @@ def _validate_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, op: str) -> N
         raise ValueError(f"{op} requires matching tensor dtypes.")
 
 
-def _readable_cache(t: torch.Tensor) -> tuple[torch.Tensor, tuple[int, int, int]]:
+_Strides = ctypes.c_int64 * 3
+
+
+def _readable_cache(t: torch.Tensor) -> tuple[torch.Tensor, ctypes.Array]:
     strides = _cache_strides(t)
     if strides is None:
         t = materialize(t) if not t.is_contiguous() else t.clone()
-        strides = (t.stride(0), t.stride(1), t.stride(2))
-    return t, strides
+        strides = t.stride()[:3]
+    return t, _Strides(*strides)
 
 
 def _cache_attention(op: str, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
@@ -513,22 +543,25 @@ def _cache_attention(op: str, q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
         raise ValueError(f"{op} requires queries of [batch, tokens, heads, head size].")
     if q.dtype != torch.bfloat16 or k_cache.dtype != torch.bfloat16:
         raise ValueError(f"{op} requires bf16 queries and caches.")
-    if q.shape[0] != k_cache.shape[0]:
+    batch, _, _, d = q.shape
+    if k_cache.shape[0] != batch:
         raise ValueError(f"{op} requires as many cached sequences as queries have.")
-    if q.shape[3] != k_cache.shape[3]:
+    if k_cache.shape[3] != d:
         raise ValueError(f"{op} requires matching query/key/value head sizes.")
-    if lengths is None:
-        raise ValueError(f"{op} requires int64 lengths of one per sequence.")
     if error is not None and (error.dtype != torch.int32 or error.numel() != 1):
         raise ValueError(f"{op} requires an int32 error word.")
-    device = _same_device(op, q, k_cache, v_cache, lengths, counts, extra, error)
-    lengths = _row_counts(lengths, q.shape[0], op, "lengths")
-    counts = _row_counts(counts, q.shape[0], op, "counts")
-    return device, lengths, counts
+    device = _same_device(op, q, k_cache, v_cache, lengths, extra, counts, error)
+    return device, _row_counts(lengths, batch, op, "lengths"), _row_counts(counts, batch, op, "counts")
 
 
 def _address(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_scratch(device: int, *sizes: int) -> int:
+    """cppinf_cache_attention_scratch_bytes of the current device; sizes that the call will refuse need none."""
+    return max(int(capi.load().cppinf_cache_attention_scratch_bytes(*sizes)), 0)
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
@@ -545,18 +578,17 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         raise ValueError("tree_attention requires a bool mask of [tokens, tokens], shared or one per sequence.")
     device, lengths, nodes = _cache_attention(op, q, k_cache, v_cache, lengths, nodes, mask, error)
     batch, tokens, q_heads, d = q.shape
-    capacity, kv_heads = k_cache.shape[1:3]
-    with torch.cuda.device(device):
+    _, capacity, kv_heads, _ = k_cache.shape
+    with _On(device) as stream:
         q, mask = materialize(q), mask.contiguous()
         k, ks = _readable_cache(k_cache)
         v, vs = _readable_cache(v_cache)
         ctx = torch.empty_like(q)
-        nbytes = int(capi.load().cppinf_cache_attention_scratch_bytes(batch, tokens, q_heads, kv_heads, d, capacity, 0))
-        scratch = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=device)
-        capi.call("cppinf_tree_attention", q.data_ptr(), k.data_ptr(), capi.i64_array(ks), v.data_ptr(),
-                  capi.i64_array(vs), lengths.data_ptr(), mask.data_ptr(),
-                  tokens * tokens if mask.dim() == 3 else 0, _address(nodes), ctx.data_ptr(), batch, tokens, q_heads,
-                  kv_heads, d, capacity, scratch.data_ptr(), nbytes, _address(error), _stream())
+        nbytes = _attention_scratch(device, batch, tokens, q_heads, kv_heads, d, capacity, 0)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        capi.call("cppinf_tree_attention", q.data_ptr(), k.data_ptr(), ks, v.data_ptr(), vs, lengths.data_ptr(),
+                  mask.data_ptr(), tokens * tokens if mask.dim() == 3 else 0, _address(nodes), ctx.data_ptr(), batch,
+                  tokens, q_heads, kv_heads, d, capacity, scratch.data_ptr(), nbytes, _address(error), stream)
     return ctx
 
 
@@ -573,12 +605,12 @@ def tree_accept(token_ids: torch.Tensor, parents: torch.Tensor, predicted: torch
     device = _same_device(op, token_ids, parents, predicted, nodes)
     batch, tokens = token_ids.shape
     nodes = _row_counts(nodes, batch, op, "nodes")
-    with torch.cuda.device(device):
+    with _On(device) as stream:
         token_ids, parents, predicted = token_ids.contiguous(), parents.contiguous(), predicted.contiguous()
-        path = torch.empty((batch, tokens), dtype=torch.int64, device=device)
-        counts, following = torch.empty((2, batch), dtype=torch.int64, device=device).unbind(0)
+        path = torch.empty_like(token_ids)
+        counts, following = token_ids.new_empty(batch), token_ids.new_empty(batch)
         capi.call("cppinf_tree_accept", token_ids.data_ptr(), parents.data_ptr(), predicted.data_ptr(), _address(nodes),
-                  path.data_ptr(), counts.data_ptr(), following.data_ptr(), batch, tokens, _stream())
+                  path.data_ptr(), counts.data_ptr(), following.data_ptr(), batch, tokens, stream)
     return path, counts, following
 
 
@@ -599,11 +631,11 @@ def tree_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Ten
     ks, vs = _cache_strides(k_cache), _cache_strides(v_cache)
     if ks is None or vs is None:
         raise ValueError("tree_commit requires caches with dense 16-byte aligned rows.")
-    with torch.cuda.device(device):
+    with _On(device) as stream:
         path = path.contiguous()
-        capi.call("cppinf_tree_commit", code, k_cache.data_ptr(), capi.i64_array(ks), v_cache.data_ptr(),
-                  capi.i64_array(vs), lengths.data_ptr(), path.data_ptr(), counts.data_ptr(), batch, path.shape[1],
-                  heads, d, capacity, _stream())
+        capi.call("cppinf_tree_commit", code, k_cache.data_ptr(), _Strides(*ks), v_cache.data_ptr(), _Strides(*vs),
+                  lengths.data_ptr(), path.data_ptr(), counts.data_ptr(), batch, path.shape[1], heads, d, capacity,
+                  stream)
 
 
 def decoder_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
@@ -617,19 +649,19 @@ def decoder_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     op = "decoder_attention_weights"
     device, lengths, counts = _cache_attention(op, q, k_cache, v_cache, lengths, counts, weights, error)
     batch, tokens, q_heads, d = q.shape
-    capacity, kv_heads = k_cache.shape[1:3]
+    _, capacity, kv_heads, _ = k_cache.shape
     if weights.dtype != torch.float32 or weights.shape != (batch, kv_heads, capacity) or not weights.is_contiguous():
         raise ValueError("decoder_attention_weights requires contiguous f32 weights of [batch, heads, capacity].")
-    with torch.cuda.device(device):
+    with _On(device) as stream:
         q = materialize(q)
         k, ks = _readable_cache(k_cache)
         v, vs = _readable_cache(v_cache)
         ctx = torch.empty_like(q)
-        nbytes = int(capi.load().cppinf_cache_attention_scratch_bytes(batch, tokens, q_heads, kv_heads, d, capacity, 1))
-        scratch = torch.empty(max(nbytes, 0), dtype=torch.uint8, device=device)
-        capi.call("cppinf_decoder_attention_weights", q.data_ptr(), k.data_ptr(), capi.i64_array(ks), v.data_ptr(),
-                  capi.i64_array(vs), lengths.data_ptr(), _address(counts), ctx.data_ptr(), weights.data_ptr(), batch,
-                  tokens, q_heads, kv_heads, d, capacity, scratch.data_ptr(), nbytes, _address(error), _stream())
+        nbytes = _attention_scratch(device, batch, tokens, q_heads, kv_heads, d, capacity, 1)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        capi.call("cppinf_decoder_attention_weights", q.data_ptr(), k.data_ptr(), ks, v.data_ptr(), vs,
+                  lengths.data_ptr(), _address(counts), ctx.data_ptr(), weights.data_ptr(), batch, tokens, q_heads,
+                  kv_heads, d, capacity, scratch.data_ptr(), nbytes, _address(error), stream)
     return ctx
 
 
@@ -653,18 +685,18 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
         raise IndexError("cache_evict output is too small for the kept rows.")
     device = _same_device(op, k_cache, v_cache, weights, lengths)
     lengths = _row_counts(lengths, batch, op, "lengths")
-    with torch.cuda.device(device):
+    with _On(device) as stream:
         weights = materialize(weights)
         k, ks = _readable_cache(k_cache)
         v, vs = _readable_cache(v_cache)
-        k_out = torch.empty((batch, capacity, heads, d), dtype=k.dtype, device=device)
+        k_out = k.new_empty((batch, capacity, heads, d))
         v_out = torch.empty_like(k_out)
-        w_out = torch.empty((batch, heads, capacity), dtype=torch.float32, device=device)
-        left = torch.empty(batch, dtype=torch.int64, device=device)
-        index = torch.empty((batch, heads, keep), dtype=torch.int64, device=device)
-        capi.call("cppinf_cache_evict", code, k.data_ptr(), capi.i64_array(ks), v.data_ptr(), capi.i64_array(vs),
-                  weights.data_ptr(), lengths.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), w_out.data_ptr(),
-                  left.data_ptr(), index.data_ptr(), batch, heads, d, rows, keep, recent, sinks, capacity, _stream())
+        w_out = weights.new_empty((batch, heads, capacity))
+        left = torch.empty_like(lengths)
+        index = lengths.new_empty((batch, heads, keep))
+        capi.call("cppinf_cache_evict", code, k.data_ptr(), ks, v.data_ptr(), vs, weights.data_ptr(),
+                  lengths.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), w_out.data_ptr(), left.data_ptr(),
+                  index.data_ptr(), batch, heads, d, rows, keep, recent, sinks, capacity, stream)
     return k_out, v_out, w_out, left, index
 
 
