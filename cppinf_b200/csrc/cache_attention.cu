@@ -708,27 +708,24 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 }
                 if (p.mask != nullptr) {  // the tile's mask rows as bits
                     uint32_t* words = s_mask + w * 128 * 9;
-                    const uint8_t* mask = p.mask + at.b * p.mask_stride;
-                    for (int i = warp & 3; i < p.tile_tokens; i += 4) {
-                        const int64_t tt = token0 + i;
-                        bool on[8];
+                    const int tokens = r.valid - token0 < p.tile_tokens ? r.valid - token0 : p.tile_tokens;
+                    for (int u = row; u < tokens * 9; u += 128) {  // a thread makes a word of 32 nodes
+                        const int token = u / 9;
+                        const int node0 = (u - token * 9) * 32;
+                        const uint8_t* mask =
+                            p.mask + at.b * p.mask_stride + static_cast<int64_t>(token0 + token) * p.tokens + node0;
+                        uint32_t word = 0u;
+                        if (node0 < r.valid) {
+                            const int last = r.valid - 1 - node0;
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const int j = k * 32 + lane;
-                            on[k] = tt < r.valid && j < r.valid && mask[tt * p.tokens + j] != 0;
-                        }
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const uint32_t word = __ballot_sync(0xffffffffu, on[k]);
-                            if (lane == k) {
-                                words[i * 9 + k] = word;
+                            for (int i = 0; i < 32; ++i) {
+                                const uint32_t on = mask[i < last ? i : last] != 0 ? 1u : 0u;
+                                word |= i <= last ? on << i : 0u;
                             }
                         }
-                        if (lane == 8) {
-                            words[i * 9 + 8] = 0u;
-                        }
+                        words[u] = word;
                     }
-                    bits_row = words + (token_in_tile < p.tile_tokens ? token_in_tile : 0) * 9;
+                    bits_row = words + (token_in_tile < tokens ? token_in_tile : 0) * 9;
                 }
                 named_barrier(1 + w, 128);
             }
