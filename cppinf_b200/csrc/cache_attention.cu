@@ -1055,7 +1055,7 @@ struct WeightTiling {
     static constexpr uint32_t kTile = kAtom * kAtoms;
     static constexpr uint32_t kK = 0;
     static constexpr uint32_t kRing = kK + kKeySlots * kTile;
-    static constexpr uint32_t kStats = kRing + kSlots * kTile;     // [groups][2][128] (-M, 1 / l)
+    static constexpr uint32_t kStats = kRing + kSlots * kTile;     // [groups][2][2][128] M, then 1 / l
     static constexpr uint32_t kSum = kStats + 2 * 2 * 128 * 8;     // [128] the second group's sums
     static constexpr uint32_t kBars = kSum + 128 * 4;
     static constexpr std::size_t kBytes = 1024 + kBars + 256;
@@ -1118,7 +1118,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
     using L = WeightTiling<D>;
     extern __shared__ __align__(16) unsigned char raw[];
     unsigned char* sm = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
-    float2* s_stats = reinterpret_cast<float2*>(sm + L::kStats);
+    float* s_stats = reinterpret_cast<float*>(sm + L::kStats);
     float* s_sum = reinterpret_cast<float*>(sm + L::kSum);
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + L::kBars);
     uint64_t* bar_full = bars;                    // [slots] a query tile has landed
@@ -1136,7 +1136,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int lane = tid & 31;
     const int columns = p.q_box_tokens * p.group;       // rows of a query tile, columns of the product
-    const int chunks = (columns + 31) / 32;
+    const int chunks = (columns + 63) / 64;             // of 64 columns
     if (tid == 0) {
         s_stop = 0u;
         for (int i = 0; i < L::kSlots; ++i) {
@@ -1298,7 +1298,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
         }
     } else if (warp == 1) {
         {  // ---- matrix products
-            const uint32_t idesc = idesc_bf16_f32(chunks * 32);
+            const uint32_t idesc = idesc_bf16_f32(chunks * 64);
             while (at.left > 0) {
                 const int tiles = r.q_tiles - r.first(at.kt, p.tile_tokens);
                 const int count = tiles - at.q < at.left ? tiles - at.q : at.left;
@@ -1339,53 +1339,66 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const float c2 = 1.4426950408889634f / sqrtf(static_cast<float>(D));
         uint32_t turn = 0;  // which of the group's two copies of the statistics
+        // Starts the copy of a query tile's statistics into the group's next place; zeros for columns that count for
+        // nothing.
+        const auto fetch = [&](int token0) {
+            const int inside = r.valid - token0 < p.tile_tokens ? r.valid - token0 : p.tile_tokens;
+            const float2* st = p.stats + ((at.b * p.kv_heads + at.h) * p.tokens + token0) * p.group + row;
+            float* to = s_stats + (w * 2 + turn) * 256 + row;
+            const bool there = row < inside * p.group;
+            cp_async4(to, there ? &st->x : &p.stats->x, there);
+            cp_async4(to + 128, there ? &st->y : &p.stats->x, there);
+        };
         while (at.left > 0) {
             const int q0 = r.first(at.kt, p.tile_tokens);
             const int tiles = r.q_tiles - q0;
             const int count = tiles - at.q < at.left ? tiles - at.q : at.left;
             const int key = at.kt * 128 + row;
-            float part[4] = {};
-            bool mine = false;
-            for (int i = 0; i < count; ++i) {
+            const int first = (at.products & 1u) == static_cast<uint32_t>(w) ? 0 : 1;  // of the segment's products
+            float2 part[2] = {};
+            if (first < count) {
+                fetch((q0 + at.q + first) * p.tile_tokens);
+            }
+            for (int i = first; i < count; i += 2) {
                 const uint32_t n = at.products + static_cast<uint32_t>(i);
-                if ((n & 1u) != static_cast<uint32_t>(w)) {
-                    continue;
-                }
-                mine = true;
                 const uint32_t buffer = n % L::kBuffers;
                 const int token0 = (q0 + at.q + i) * p.tile_tokens;
                 const int inside = r.valid - token0 < p.tile_tokens ? r.valid - token0 : p.tile_tokens;
-                const int high = inside * p.group;  // columns from here on count for nothing
-                float2 st = make_float2(0.0f, 0.0f);
-                if (row < high) {
-                    st = p.stats[((at.b * p.kv_heads + at.h) * p.tokens + token0) * p.group + row];
-                }
-                float2* stats = s_stats + (w * 2 + turn) * 128;
+                const float* stats = s_stats + (w * 2 + turn) * 256;
                 turn ^= 1u;
-                stats[row] = make_float2(-st.x, st.y);
-                named_barrier(1 + w, 128);
+                cp_async_wait_all();
+                named_barrier(1 + w, 128);  // the statistics are there, and nobody reads the ones before
+                if (i + 2 < count) {
+                    fetch(token0 + 2 * p.tile_tokens);
+                }
                 wait(bar_s + buffer, n / L::kBuffers & 1u);
                 tc_fence_after();
                 const bool partial = inside < p.tile_tokens || at.kt * 128 + 127 - r.len > token0;
                 const int low = (key - r.len - token0) * p.group;  // columns below do not see the key
+                const int high = inside * p.group;                 // columns from here on count for nothing
 #pragma unroll 1
                 for (int c = 0; c < chunks; ++c) {
-                    float x[32];
-                    tmem_load32(tmem + lanes + buffer * 128 + c * 32, x);
-                    if (!partial) {
+                    float x[64];
+                    tmem_load_begin<64>(tmem + lanes + buffer * 128 + c * 64, x);
+                    tmem_load_end<64>(x);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const float2 s = stats[c * 32 + j];
-                            part[j & 3] = __fmaf_rn(exp2_approx(__fmaf_rn(x[j], c2, s.x)), s.y, part[j & 3]);
+                    for (int j = 0; j < 64; j += 4) {
+                        const float4 top = *reinterpret_cast<const float4*>(stats + c * 64 + j);
+                        const float4 inv = *reinterpret_cast<const float4*>(stats + 128 + c * 64 + j);
+                        float2 e0 = __ffma2_rn(make_float2(x[j], x[j + 1]), make_float2(c2, c2), make_float2(-top.x, -top.y));
+                        float2 e1 = __ffma2_rn(make_float2(x[j + 2], x[j + 3]), make_float2(c2, c2),
+                                               make_float2(-top.z, -top.w));
+                        e0 = make_float2(exp2_approx(e0.x), exp2_approx(e0.y));
+                        e1 = make_float2(exp2_approx(e1.x), exp2_approx(e1.y));
+                        if (partial) {
+                            const int column = c * 64 + j;
+                            e0.x = column >= low && column < high ? e0.x : 0.0f;
+                            e0.y = column + 1 >= low && column + 1 < high ? e0.y : 0.0f;
+                            e1.x = column + 2 >= low && column + 2 < high ? e1.x : 0.0f;
+                            e1.y = column + 3 >= low && column + 3 < high ? e1.y : 0.0f;
                         }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const int column = c * 32 + j;
-                            const float2 s = stats[column];
-                            const float e = exp2_approx(__fmaf_rn(x[j], c2, s.x)) * s.y;
-                            part[j & 3] += column >= low && column < high ? e : 0.0f;
-                        }
+                        part[0] = __ffma2_rn(e0, make_float2(inv.x, inv.y), part[0]);
+                        part[1] = __ffma2_rn(e1, make_float2(inv.z, inv.w), part[1]);
                     }
                 }
                 tc_fence_before();
@@ -1394,8 +1407,8 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
                     mbar_arrive(bar_free + buffer);
                 }
             }
-            float sum = (part[0] + part[1]) + (part[2] + part[3]);
-            bool writes = mine;
+            float sum = (part[0].x + part[0].y) + (part[1].x + part[1].y);
+            bool writes = first < count;
             if (count > 1) {  // both groups had products of the unit: the second hands its sums to the first
                 if (w == 1) {
                     s_sum[row] = sum;
