@@ -67,6 +67,7 @@ struct CacheAttentionParams {
     // Tiling (plan()) and scratch.
     int group;            // query heads of a key-value head
     int tile_tokens;      // tokens of a 128-row tile
+    FastDiv by_tile_tokens;
     int item_tokens;      // tokens of an item: one or two tiles
     int row_tiles;        // items along the tokens
     int q_box_tokens;     // tokens of one TMA box of q
@@ -1069,9 +1070,9 @@ struct KeyRange {
     int q_tiles;    // query tiles of the sequence
     int key_tiles;
 
-    __device__ __forceinline__ int first(int kt, int tile_tokens) const {  // the first query tile that sees key tile kt
+    __device__ __forceinline__ int first(int kt, const FastDiv& tile_tokens) const {  // query tile that sees key tile kt
         const int past = kt * 128 - len;
-        return past > 0 ? past / tile_tokens : 0;
+        return past > 0 ? static_cast<int>(tile_tokens.quot(static_cast<uint32_t>(past))) : 0;
     }
 };
 
@@ -1079,23 +1080,34 @@ __device__ __forceinline__ KeyRange key_range(const CacheAttentionParams& p, int
     KeyRange r;
     r.len = static_cast<int>(committed_rows(p, b));
     r.valid = static_cast<int>(valid_queries(p, b));
-    r.q_tiles = (r.valid + p.tile_tokens - 1) / p.tile_tokens;
+    r.q_tiles = static_cast<int>(p.by_tile_tokens.quot(static_cast<uint32_t>(r.valid + p.tile_tokens - 1)));
     r.key_tiles = r.valid > 0 ? (r.len + r.valid + 127) / 128 : 0;
     return r;
 }
 
-// Products of one head of a sequence: whole rows of query tiles for the key tiles that begin in committed rows.
+// Products of key tiles [kt0, kt0 + 32) of a sequence's head, one tile a lane.
+__device__ __forceinline__ int lane_products(const CacheAttentionParams& p, const KeyRange& r, int kt0) {
+    const int kt = kt0 + static_cast<int>(threadIdx.x & 31);
+    return kt < r.key_tiles ? r.q_tiles - r.first(kt, p.by_tile_tokens) : 0;
+}
+
+// Products of one head of a sequence, by a whole warp.
 __device__ __forceinline__ int head_products(const CacheAttentionParams& p, const KeyRange& r) {
-    if (r.valid == 0) {
-        return 0;
+    int sum = 0;
+    for (int kt0 = 0; kt0 < r.key_tiles; kt0 += 32) {
+        sum += lane_products(p, r, kt0);
     }
-    int kt = r.len / 128 + 1;
-    kt = kt < r.key_tiles ? kt : r.key_tiles;
-    int sum = kt * r.q_tiles;
-    for (; kt < r.key_tiles; ++kt) {
-        sum += r.q_tiles - r.first(kt, p.tile_tokens);
-    }
-    return sum;
+    return __reduce_add_sync(0xffffffffu, sum);
+}
+
+// The range that another lane of the warp holds.
+__device__ __forceinline__ KeyRange from_lane(const KeyRange& r, int lane) {
+    KeyRange other;
+    other.len = __shfl_sync(0xffffffffu, r.len, lane);
+    other.valid = __shfl_sync(0xffffffffu, r.valid, lane);
+    other.q_tiles = __shfl_sync(0xffffffffu, r.q_tiles, lane);
+    other.key_tiles = __shfl_sync(0xffffffffu, r.key_tiles, lane);
+    return other;
 }
 
 // The line of products is cut like the attention's; a unit is one key tile of one head.
@@ -1165,63 +1177,64 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
     fence_proxy_async_smem();
     grid_dependency_begin();
     if (warp == 0) {
+        // Sequences in groups of 32, a lane each; each one's products are then counted by the whole warp.
         const int heads = static_cast<int>(p.kv_heads);
+        const int batch = static_cast<int>(p.batch);
+        const auto ranges_of = [&](int b0) { return b0 + lane < batch ? key_range(p, b0 + lane) : KeyRange{}; };
+        KeyRange mine = ranges_of(0);
         int total = 0;
-        for (int64_t b = lane; b < p.batch; b += 32) {
-            total += head_products(p, key_range(p, b)) * heads;
+        for (int b = 0; b < batch; ++b) {
+            if (b > 0 && b % 32 == 0) {
+                mine = ranges_of(b);
+            }
+            total += head_products(p, from_lane(mine, b % 32)) * heads;
         }
-        total = __reduce_add_sync(0xffffffffu, total);
         const Cuts cuts(total, static_cast<int>(gridDim.x));
         const int begin = cuts.begin(static_cast<int>(blockIdx.x));
         const int end = cuts.begin(static_cast<int>(blockIdx.x) + 1);
-        if (lane == 0) {
-            UnitWalk w{};
-            w.total = total;
-            s_walk = w;
-        }
-        __syncwarp();
-        int before = 0;
-        for (int64_t b0 = 0; b0 < p.batch && begin < end; b0 += 32) {
-            const KeyRange r = b0 + lane < p.batch ? key_range(p, b0 + lane) : KeyRange{};
-            const int mine = head_products(p, r) * heads;
-            int sum = mine;
-            for (int offset = 1; offset < 32; offset <<= 1) {
-                const int other = __shfl_up_sync(0xffffffffu, sum, offset);
-                sum += lane >= offset ? other : 0;
+        UnitWalk w{};
+        w.total = total;
+        if (begin < end) {
+            if (batch > 32) {
+                mine = ranges_of(0);
             }
-            const int lo = before + sum - mine;
-            if (begin >= lo && begin < lo + mine) {
-                // Order within a sequence: key tile, head, query tile.
-                int rest = begin - lo;
-                const int whole = r.q_tiles * heads;
-                const int most = r.len / 128 < r.key_tiles - 1 ? r.len / 128 : r.key_tiles - 1;
-                int kt = rest / whole < most ? rest / whole : most;
-                rest -= kt * whole;
-                for (;;) {
-                    const int here = (r.q_tiles - r.first(kt, p.tile_tokens)) * heads;
-                    if (rest < here) {
-                        break;
-                    }
-                    rest -= here;
-                    ++kt;
+            KeyRange r{};
+            int rest = begin;
+            for (;; ++w.b) {  // the sequence that `begin` lies in
+                if (w.b > 0 && w.b % 32 == 0) {
+                    mine = ranges_of(w.b);
                 }
-                const int each = r.q_tiles - r.first(kt, p.tile_tokens);
-                UnitWalk w;
-                w.b = static_cast<int>(b0 + lane);
-                w.kt = kt;
-                w.h = rest / each;
-                w.q = rest % each;
-                w.left = end - begin;
-                w.begin = begin;
-                w.total = total;
-                w.products = 0;
-                w.index = 0;
-                s_walk = w;
+                r = from_lane(mine, w.b % 32);
+                const int here = head_products(p, r) * heads;
+                if (rest < here) {
+                    break;
+                }
+                rest -= here;
             }
-            before += __shfl_sync(0xffffffffu, sum, 31);
-            if (before > begin) {
-                break;
+            for (int kt0 = 0;; kt0 += 32) {  // the key tile; order within a sequence: key tile, head, query tile
+                const int here = lane_products(p, r, kt0) * heads;
+                int sum = here;
+                for (int offset = 1; offset < 32; offset <<= 1) {
+                    const int other = __shfl_up_sync(0xffffffffu, sum, offset);
+                    sum += lane >= offset ? other : 0;
+                }
+                const unsigned reached = __ballot_sync(0xffffffffu, sum > rest);
+                if (reached != 0u) {
+                    const int at_lane = __ffs(reached) - 1;
+                    w.kt = kt0 + at_lane;
+                    rest -= __shfl_sync(0xffffffffu, sum - here, at_lane);
+                    break;
+                }
+                rest -= __shfl_sync(0xffffffffu, sum, 31);
             }
+            const int each = r.q_tiles - r.first(w.kt, p.by_tile_tokens);
+            w.h = rest / each;
+            w.q = rest - w.h * each;
+            w.left = end - begin;
+            w.begin = begin;
+        }
+        if (lane == 0) {
+            s_walk = w;
         }
     }
     tc_fence_before();
@@ -1260,7 +1273,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
     if (warp == 0) {
         {  // ---- loads
             while (at.left > 0) {
-                const int q0 = r.first(at.kt, p.tile_tokens);
+                const int q0 = r.first(at.kt, p.by_tile_tokens);
                 const int tiles = r.q_tiles - q0;
                 const int count = tiles - at.q < at.left ? tiles - at.q : at.left;
                 const uint32_t ks = static_cast<uint32_t>(at.index) % L::kKeySlots;
@@ -1300,7 +1313,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
         {  // ---- matrix products
             const uint32_t idesc = idesc_bf16_f32(chunks * 64);
             while (at.left > 0) {
-                const int tiles = r.q_tiles - r.first(at.kt, p.tile_tokens);
+                const int tiles = r.q_tiles - r.first(at.kt, p.by_tile_tokens);
                 const int count = tiles - at.q < at.left ? tiles - at.q : at.left;
                 const uint32_t ks = static_cast<uint32_t>(at.index) % L::kKeySlots;
                 wait(bar_k_full + ks, static_cast<uint32_t>(at.index) / L::kKeySlots & 1u);
@@ -1350,7 +1363,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
             cp_async4(to + 128, there ? &st->y : &p.stats->x, there);
         };
         while (at.left > 0) {
-            const int q0 = r.first(at.kt, p.tile_tokens);
+            const int q0 = r.first(at.kt, p.by_tile_tokens);
             const int tiles = r.q_tiles - q0;
             const int count = tiles - at.q < at.left ? tiles - at.q : at.left;
             const int key = at.kt * 128 + row;
@@ -1698,6 +1711,7 @@ int run_attention(const char* op, CacheAttentionParams& p, int64_t head_dim, voi
     char* base = static_cast<char*>(scratch);
     p.group = static_cast<int>(p.q_heads / p.kv_heads);
     p.tile_tokens = pl.tile_tokens;
+    p.by_tile_tokens = FastDiv(static_cast<uint32_t>(pl.tile_tokens));
     p.item_tokens = pl.item_tokens;
     p.row_tiles = pl.row_tiles;
     p.q_box_tokens = static_cast<int>(p.tokens < pl.tile_tokens ? p.tokens : pl.tile_tokens);
