@@ -456,7 +456,9 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 w.left = end - begin;
                 w.set_up = set_up;
                 s_walk = w;
-                p.cuts[blockIdx.x] = make_int4(w.b, w.row_tile, w.h, w.piece);
+                if (!p.whole_items) {
+                    p.cuts[blockIdx.x] = make_int4(w.b, w.row_tile, w.h, w.piece);
+                }
             }
             before += __shfl_sync(0xffffffffu, sum, 31);
             if (before > begin) {
@@ -464,7 +466,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             }
         }
         if (blockIdx.x == 0) {
-            if (lane == 0) {
+            if (lane == 0 && !p.whole_items) {
                 p.line[0] = total;
                 p.line[1] = set_up;
             }
@@ -1556,9 +1558,9 @@ Plan plan(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads, int6
     const int64_t products = batch * kv_heads * runtime::ceil_div(capacity, 128) * runtime::ceil_div(tokens, pl.tile_tokens);
     pl.fits = most < (int64_t{1} << 29) && products < (int64_t{1} << 31);
     const auto up = [](int64_t n) { return (n + 127) / 128 * 128; };
-    pl.cuts = 128;  // after the line's length
     const int64_t parts = pl.whole_items ? 0 : 2 * pl.ctas;
-    pl.ml = pl.cuts + up(pl.ctas * static_cast<int64_t>(sizeof(int4)));
+    pl.cuts = pl.whole_items ? 0 : 128;  // after the line's length
+    pl.ml = pl.cuts + (pl.whole_items ? 0 : up(pl.ctas * static_cast<int64_t>(sizeof(int4))));
     pl.o = pl.ml + up(parts * pl.part_rows * static_cast<int64_t>(sizeof(float2)));
     pl.stats = pl.o + parts * pl.part_rows * head_dim * static_cast<int64_t>(sizeof(float));
     pl.bytes = pl.stats;
@@ -1705,7 +1707,7 @@ int run_attention(const char* op, CacheAttentionParams& p, int64_t head_dim, voi
     const std::string name(op);
     const Plan pl = plan(p.batch, p.tokens, p.q_heads, p.kv_heads, head_dim, p.capacity, p.weights != nullptr);
     CPPINF_REQUIRE(pl.fits, CPPINF_ERR_OVERFLOW, name + " sizes exceed the kernels' index range.");
-    CPPINF_REQUIRE(scratch && scratch_bytes >= pl.bytes, CPPINF_ERR_INVALID_ARGUMENT,
+    CPPINF_REQUIRE((scratch || pl.bytes == 0) && scratch_bytes >= pl.bytes, CPPINF_ERR_INVALID_ARGUMENT,
                    name + " requires a scratch of cppinf_cache_attention_scratch_bytes.");
     CPPINF_REQUIRE(runtime::aligned16(scratch), CPPINF_ERR_UNSUPPORTED, name + " requires a 16-byte aligned scratch.");
     char* base = static_cast<char*>(scratch);

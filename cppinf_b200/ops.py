@@ -458,27 +458,6 @@ def decoder_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Ten
 # ---- batches of cached sequences: drafted trees, attention weights, eviction -------------------------------------
 
 
-class _On:
-    """The tensors' device as the current one, for calls made while another is (entering torch.cuda.device always costs
-    more than the comparison)."""
-
-    __slots__ = ("index", "other")
-
-    def __init__(self, index: int):
-        self.index = index
-
-    def __enter__(self) -> int:
-        self.other = None
-        if torch.cuda.current_device() != self.index:
-            self.other = torch.cuda.device(self.index)
-            self.other.__enter__()
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc) -> None:
-        if self.other is not None:
-            self.other.__exit__(*exc)
-
-
 def _same_device(op: str, *tensors: torch.Tensor | None) -> int:
     first = tensors[0].get_device()
     for t in tensors:
@@ -558,10 +537,24 @@ def _address(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def _elsewhere(device: int) -> torch.cuda.device | None:
+    """What makes the tensors' device the current one, where another is."""
+    return None if torch.cuda.current_device() == device else torch.cuda.device(device)
+
+
+def _stream_of(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
 @functools.lru_cache(maxsize=256)
-def _attention_scratch(device: int, *sizes: int) -> int:
+def _attention_scratch_bytes(device: int, *sizes: int) -> int:
     """cppinf_cache_attention_scratch_bytes of the current device; sizes that the call will refuse need none."""
     return max(int(capi.load().cppinf_cache_attention_scratch_bytes(*sizes)), 0)
+
+
+def _attention_scratch(q: torch.Tensor, device: int, *sizes: int) -> tuple[int, torch.Tensor | None]:
+    nbytes = _attention_scratch_bytes(device, *sizes)
+    return nbytes, torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
 
 
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
@@ -577,18 +570,19 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
             mask.shape[-2:] != (q.shape[1], q.shape[1]) or (mask.dim() == 3 and mask.shape[0] != q.shape[0]):
         raise ValueError("tree_attention requires a bool mask of [tokens, tokens], shared or one per sequence.")
     device, lengths, nodes = _cache_attention(op, q, k_cache, v_cache, lengths, nodes, mask, error)
+    if (other := _elsewhere(device)) is not None:
+        with other:
+            return tree_attention(q, k_cache, v_cache, lengths, mask, nodes, error)
     batch, tokens, q_heads, d = q.shape
     _, capacity, kv_heads, _ = k_cache.shape
-    with _On(device) as stream:
-        q, mask = materialize(q), mask.contiguous()
-        k, ks = _readable_cache(k_cache)
-        v, vs = _readable_cache(v_cache)
-        ctx = torch.empty_like(q)
-        nbytes = _attention_scratch(device, batch, tokens, q_heads, kv_heads, d, capacity, 0)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        capi.call("cppinf_tree_attention", q.data_ptr(), k.data_ptr(), ks, v.data_ptr(), vs, lengths.data_ptr(),
-                  mask.data_ptr(), tokens * tokens if mask.dim() == 3 else 0, _address(nodes), ctx.data_ptr(), batch,
-                  tokens, q_heads, kv_heads, d, capacity, scratch.data_ptr(), nbytes, _address(error), stream)
+    q, mask = materialize(q), mask.contiguous()
+    k, ks = _readable_cache(k_cache)
+    v, vs = _readable_cache(v_cache)
+    ctx = torch.empty_like(q)
+    nbytes, scratch = _attention_scratch(q, device, batch, tokens, q_heads, kv_heads, d, capacity, 0)
+    capi.call("cppinf_tree_attention", q.data_ptr(), k.data_ptr(), ks, v.data_ptr(), vs, lengths.data_ptr(),
+              mask.data_ptr(), tokens * tokens if mask.dim() == 3 else 0, _address(nodes), ctx.data_ptr(), batch,
+              tokens, q_heads, kv_heads, d, capacity, _address(scratch), nbytes, _address(error), _stream_of(device))
     return ctx
 
 
@@ -603,14 +597,16 @@ def tree_accept(token_ids: torch.Tensor, parents: torch.Tensor, predicted: torch
     if any(t.dtype != torch.int64 for t in (token_ids, parents, predicted)):
         raise ValueError("tree_accept requires int64 tokens, parents and predictions.")
     device = _same_device(op, token_ids, parents, predicted, nodes)
+    if (other := _elsewhere(device)) is not None:
+        with other:
+            return tree_accept(token_ids, parents, predicted, nodes)
     batch, tokens = token_ids.shape
     nodes = _row_counts(nodes, batch, op, "nodes")
-    with _On(device) as stream:
-        token_ids, parents, predicted = token_ids.contiguous(), parents.contiguous(), predicted.contiguous()
-        path = torch.empty_like(token_ids)
-        counts, following = token_ids.new_empty(batch), token_ids.new_empty(batch)
-        capi.call("cppinf_tree_accept", token_ids.data_ptr(), parents.data_ptr(), predicted.data_ptr(), _address(nodes),
-                  path.data_ptr(), counts.data_ptr(), following.data_ptr(), batch, tokens, stream)
+    token_ids, parents, predicted = token_ids.contiguous(), parents.contiguous(), predicted.contiguous()
+    path = torch.empty_like(token_ids)
+    counts, following = token_ids.new_empty(batch), token_ids.new_empty(batch)
+    capi.call("cppinf_tree_accept", token_ids.data_ptr(), parents.data_ptr(), predicted.data_ptr(), _address(nodes),
+              path.data_ptr(), counts.data_ptr(), following.data_ptr(), batch, tokens, _stream_of(device))
     return path, counts, following
 
 
@@ -631,11 +627,13 @@ def tree_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Ten
     ks, vs = _cache_strides(k_cache), _cache_strides(v_cache)
     if ks is None or vs is None:
         raise ValueError("tree_commit requires caches with dense 16-byte aligned rows.")
-    with _On(device) as stream:
-        path = path.contiguous()
-        capi.call("cppinf_tree_commit", code, k_cache.data_ptr(), _Strides(*ks), v_cache.data_ptr(), _Strides(*vs),
-                  lengths.data_ptr(), path.data_ptr(), counts.data_ptr(), batch, path.shape[1], heads, d, capacity,
-                  stream)
+    if (other := _elsewhere(device)) is not None:
+        with other:
+            return tree_commit(k_cache, v_cache, lengths, path, counts)
+    path = path.contiguous()
+    capi.call("cppinf_tree_commit", code, k_cache.data_ptr(), _Strides(*ks), v_cache.data_ptr(), _Strides(*vs),
+              lengths.data_ptr(), path.data_ptr(), counts.data_ptr(), batch, path.shape[1], heads, d, capacity,
+              _stream_of(device))
 
 
 def decoder_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
@@ -652,16 +650,17 @@ def decoder_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     _, capacity, kv_heads, _ = k_cache.shape
     if weights.dtype != torch.float32 or weights.shape != (batch, kv_heads, capacity) or not weights.is_contiguous():
         raise ValueError("decoder_attention_weights requires contiguous f32 weights of [batch, heads, capacity].")
-    with _On(device) as stream:
-        q = materialize(q)
-        k, ks = _readable_cache(k_cache)
-        v, vs = _readable_cache(v_cache)
-        ctx = torch.empty_like(q)
-        nbytes = _attention_scratch(device, batch, tokens, q_heads, kv_heads, d, capacity, 1)
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        capi.call("cppinf_decoder_attention_weights", q.data_ptr(), k.data_ptr(), ks, v.data_ptr(), vs,
-                  lengths.data_ptr(), _address(counts), ctx.data_ptr(), weights.data_ptr(), batch, tokens, q_heads,
-                  kv_heads, d, capacity, scratch.data_ptr(), nbytes, _address(error), stream)
+    if (other := _elsewhere(device)) is not None:
+        with other:
+            return decoder_attention_weights(q, k_cache, v_cache, lengths, weights, counts, error)
+    q = materialize(q)
+    k, ks = _readable_cache(k_cache)
+    v, vs = _readable_cache(v_cache)
+    ctx = torch.empty_like(q)
+    nbytes, scratch = _attention_scratch(q, device, batch, tokens, q_heads, kv_heads, d, capacity, 1)
+    capi.call("cppinf_decoder_attention_weights", q.data_ptr(), k.data_ptr(), ks, v.data_ptr(), vs, lengths.data_ptr(),
+              _address(counts), ctx.data_ptr(), weights.data_ptr(), batch, tokens, q_heads, kv_heads, d, capacity,
+              _address(scratch), nbytes, _address(error), _stream_of(device))
     return ctx
 
 
@@ -685,18 +684,20 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
         raise IndexError("cache_evict output is too small for the kept rows.")
     device = _same_device(op, k_cache, v_cache, weights, lengths)
     lengths = _row_counts(lengths, batch, op, "lengths")
-    with _On(device) as stream:
-        weights = materialize(weights)
-        k, ks = _readable_cache(k_cache)
-        v, vs = _readable_cache(v_cache)
-        k_out = k.new_empty((batch, capacity, heads, d))
-        v_out = torch.empty_like(k_out)
-        w_out = weights.new_empty((batch, heads, capacity))
-        left = torch.empty_like(lengths)
-        index = lengths.new_empty((batch, heads, keep))
-        capi.call("cppinf_cache_evict", code, k.data_ptr(), ks, v.data_ptr(), vs, weights.data_ptr(),
-                  lengths.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), w_out.data_ptr(), left.data_ptr(),
-                  index.data_ptr(), batch, heads, d, rows, keep, recent, sinks, capacity, stream)
+    if (other := _elsewhere(device)) is not None:
+        with other:
+            return cache_evict(k_cache, v_cache, weights, lengths, keep, recent, sinks, capacity)
+    weights = materialize(weights)
+    k, ks = _readable_cache(k_cache)
+    v, vs = _readable_cache(v_cache)
+    k_out = k.new_empty((batch, capacity, heads, d))
+    v_out = torch.empty_like(k_out)
+    w_out = weights.new_empty((batch, heads, capacity))
+    left = torch.empty_like(lengths)
+    index = lengths.new_empty((batch, heads, keep))
+    capi.call("cppinf_cache_evict", code, k.data_ptr(), ks, v.data_ptr(), vs, weights.data_ptr(), lengths.data_ptr(),
+              k_out.data_ptr(), v_out.data_ptr(), w_out.data_ptr(), left.data_ptr(), index.data_ptr(), batch, heads, d,
+              rows, keep, recent, sinks, capacity, _stream_of(device))
     return k_out, v_out, w_out, left, index
 
 
