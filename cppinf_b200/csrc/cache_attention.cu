@@ -46,6 +46,18 @@ constexpr int kMaxNodes = 256;  // drafted tokens of a sequence
 constexpr int kMaxGroup = 128;  // query heads of a key-value head
 constexpr int kMaxKeptRows = 32;  // rows of a head whose scores are kept for the weights
 
+// Where a CTA's part of the line begins, for the kernel that joins the parts.
+struct __align__(16) Cut {
+    int b;
+    int row_tile;
+    int h;
+    int piece;
+    int total;   // pieces of the line
+    int set_up;  // pieces of an item before its tiles
+    int len;     // of sequence b
+    int valid;
+};
+
 struct CacheAttentionParams {
     const bf16* q;  // [B, T, Hq, D]
     const bf16* k;  // rows of D elements, element strides {batch, row, head}
@@ -73,8 +85,7 @@ struct CacheAttentionParams {
     int q_box_tokens;     // tokens of one TMA box of q
     bool whole_items;     // the line is cut between items only
     int part_rows;        // rows of a part in the scratch
-    int4* cuts;           // [CTAs] where each CTA's part of the line begins: sequence, row tile, head, piece
-    int* line;            // length of the line, pieces of an item before its tiles
+    Cut* cuts;            // [CTAs]
     float2* part_ml;      // [2 CTAs][part_rows] (M in base 2, l)
     float* part_o;        // [2 CTAs][D / 4][part_rows][4]
     float* scores;          // [B, Hkv][rows][score_stride] S of few rows, kept for the weights, or null
@@ -176,11 +187,10 @@ constexpr uint32_t kTmemAll = 512;
 
 // An item's share of the line: its key tiles, and before them `kSetUp` pieces without any for what an item costs besides
 // its tiles (loading Q, the first S, writing the rows: 9000 to 12000 cycles, where a tile takes about 3000). Left out
-// where CTAs have few tiles each and a set-up's place would be better taken by a tile.
+// where CTAs have few tiles each and a set-up's place would be better taken by a tile. 64 sequences of up to 4000 rows:
+// 132 us without, 122 us with 3, 121 us with 6.
 constexpr int kSetUp = 3;
 constexpr int kSetUpFrom = 8;  // tiles per CTA
-// Items of up to so many key tiles are not cut at all (a piece is then an item): nothing is left to join.
-constexpr int kWholeTiles = 8;
 
 // Where a CTA's part of the line is, item by item; every role of the CTA walks it for itself.
 struct Walk {
@@ -457,7 +467,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 w.set_up = set_up;
                 s_walk = w;
                 if (!p.whole_items) {
-                    p.cuts[blockIdx.x] = make_int4(w.b, w.row_tile, w.h, w.piece);
+                    p.cuts[blockIdx.x] = Cut{w.b, w.row_tile, w.h, w.piece, total, set_up, w.len, w.valid};
                 }
             }
             before += __shfl_sync(0xffffffffu, sum, 31);
@@ -466,10 +476,6 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             }
         }
         if (blockIdx.x == 0) {
-            if (lane == 0 && !p.whole_items) {
-                p.line[0] = total;
-                p.line[1] = set_up;
-            }
             for (int i = lane; i < p.weight_ctas; i += 32) {
                 p.tickets[i] = 0u;
             }
@@ -972,15 +978,14 @@ __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAt
     __shared__ int64_t s_places[32];
     grid_dependency_begin();
     const int cut = static_cast<int>(blockIdx.x) + 1;
-    const int4 where = p.cuts[cut];
-    const int set_up = p.line[1];
-    const Cuts cuts(p.line[0], ctas);
-    const int first = cuts.begin(cut) - where.w;  // the item's first piece on the line
-    if (cuts.empty(cut) || where.w <= set_up || cuts.begin(cut - 1) > first + set_up) {
+    const Cut where = p.cuts[cut];
+    const int set_up = where.set_up;
+    const Cuts cuts(p.cuts[0].total, ctas);  // a cut at the line's end has no record of its own
+    const int first = cuts.begin(cut) - where.piece;  // the item's first piece on the line
+    if (cuts.empty(cut) || where.piece <= set_up || cuts.begin(cut - 1) > first + set_up) {
         return;
     }
-    const ItemRange r = item_range(p, static_cast<int>(committed_rows(p, where.x)),
-                                   static_cast<int>(valid_queries(p, where.x)), where.y);
+    const ItemRange r = item_range(p, where.len, where.valid, where.row_tile);
     const int last = cuts.of(first + set_up + item_tiles<kKeys>(r) - 1);  // parts before it are not empty
     const int lane = threadIdx.x & 31;
     const int warp = threadIdx.x >> 5;
@@ -993,28 +998,39 @@ __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAt
     float top = -INFINITY;
     float sum = 0.0f;
     float o[kPieces][4] = {};
-    if (inside) {
-#pragma unroll 2
-        for (int c = cut - 1; c <= last; ++c) {
-            const int64_t slot = 2 * static_cast<int64_t>(c) + (cuts.begin(c) >= first ? 0 : 1);
-            const float2 ml = p.part_ml[slot * p.part_rows + row];
-            float4 x[kPieces];
+    constexpr int kBatch = D == 256 ? 2 : 4;  // parts whose loads are in flight together
+    for (int c0 = cut - 1; inside && c0 <= last; c0 += kBatch) {
+        float2 ml[kBatch];
+        float4 x[kBatch][kPieces];
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                x[i] = reinterpret_cast<const float4*>(p.part_o)[(slot * (D / 4) + warp * kPieces + i) * p.part_rows +
-                                                                 row];
+        for (int j = 0; j < kBatch; ++j) {
+            ml[j] = make_float2(-INFINITY, 0.0f);
+            if (c0 + j <= last) {
+                const int64_t slot = 2 * static_cast<int64_t>(c0 + j) + (cuts.begin(c0 + j) >= first ? 0 : 1);
+                ml[j] = p.part_ml[slot * p.part_rows + row];
+#pragma unroll
+                for (int i = 0; i < kPieces; ++i) {
+                    x[j][i] = reinterpret_cast<const float4*>(
+                        p.part_o)[(slot * (D / 4) + warp * kPieces + i) * p.part_rows + row];
+                }
             }
-            const float most = fmaxf(top, ml.x);
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            if (c0 + j > last) {
+                break;
+            }
+            const float most = fmaxf(top, ml[j].x);
             const float f0 = top == -INFINITY ? 0.0f : exp2_approx(top - most);
-            const float f1 = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - most);
+            const float f1 = ml[j].x == -INFINITY ? 0.0f : exp2_approx(ml[j].x - most);
             top = most;
-            sum = __fmaf_rn(ml.y, f1, sum * f0);
+            sum = __fmaf_rn(ml[j].y, f1, sum * f0);
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
-                o[i][0] = __fmaf_rn(x[i].x, f1, o[i][0] * f0);
-                o[i][1] = __fmaf_rn(x[i].y, f1, o[i][1] * f0);
-                o[i][2] = __fmaf_rn(x[i].z, f1, o[i][2] * f0);
-                o[i][3] = __fmaf_rn(x[i].w, f1, o[i][3] * f0);
+                o[i][0] = __fmaf_rn(x[j][i].x, f1, o[i][0] * f0);
+                o[i][1] = __fmaf_rn(x[j][i].y, f1, o[i][1] * f0);
+                o[i][2] = __fmaf_rn(x[j][i].z, f1, o[i][2] * f0);
+                o[i][3] = __fmaf_rn(x[j][i].w, f1, o[i][3] * f0);
             }
         }
     }
@@ -1026,9 +1042,9 @@ __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAt
                   : make_uint2(0u, 0u);
     }
     if (warp == 0) {
-        s_places[lane] = inside ? ((where.x * p.tokens + t) * p.q_heads + where.z * p.group + g) * D : -1;
+        s_places[lane] = inside ? ((where.b * p.tokens + t) * p.q_heads + where.h * p.group + g) * D : -1;
         if (inside && p.stats != nullptr) {
-            p.stats[((where.x * p.kv_heads + where.z) * p.tokens + t) * p.group + g] =
+            p.stats[((where.b * p.kv_heads + where.h) * p.tokens + t) * p.group + g] =
                 valid ? make_float2(top == -INFINITY ? 0.0f : top, inv) : make_float2(0.0f, 0.0f);
         }
     }
@@ -1530,7 +1546,6 @@ struct Plan {
     int item_tokens;
     int row_tiles;
     int part_rows;
-    int64_t cuts;
     int64_t ml;
     int64_t o;
     int64_t stats;
@@ -1552,15 +1567,21 @@ Plan plan(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads, int6
     pl.row_tiles = static_cast<int>(runtime::ceil_div(tokens, pl.item_tokens));
     pl.part_rows = pl.pair ? 2 * kBM : static_cast<int>((tokens < pl.tile_tokens ? tokens : pl.tile_tokens) * group);
     const int64_t most = batch * pl.row_tiles * kv_heads * runtime::ceil_div(capacity, keys);  // tiles of the line
-    pl.whole_items = runtime::ceil_div(capacity, keys) <= kWholeTiles;
-    const int64_t pieces = pl.whole_items ? batch * pl.row_tiles * kv_heads : most;
+    // Items of few key tiles are not cut (a piece of the line is then an item): nothing is left to join, which one
+    // sequence of 600 rows gains by (11.6 us against 13.0 us cut) and one of 1000 no longer (13.9 against 10.8). Where
+    // there are many items of one length of tokens, longer ones too: 16 sequences of up to 1000 rows 15.4 against 22.8,
+    // of up to 1900 rows 22.4 against 25.2.
+    const int64_t items = batch * pl.row_tiles * kv_heads;
+    const int64_t tiles = runtime::ceil_div(capacity, keys);
+    pl.whole_items = tiles <= 6 || (tiles <= 16 && pl.row_tiles == 1 && items >= runtime::sm_count() / 2);
+    // A CTA whose two chains share a row tile is given two key tiles at least.
+    const int64_t pieces = pl.whole_items ? items : pl.pair || head_dim == 256 ? most : (most + 1) / 2;
     pl.ctas = static_cast<int>(pieces < runtime::sm_count() ? pieces : runtime::sm_count());
     const int64_t products = batch * kv_heads * runtime::ceil_div(capacity, 128) * runtime::ceil_div(tokens, pl.tile_tokens);
     pl.fits = most < (int64_t{1} << 29) && products < (int64_t{1} << 31);
     const auto up = [](int64_t n) { return (n + 127) / 128 * 128; };
     const int64_t parts = pl.whole_items ? 0 : 2 * pl.ctas;
-    pl.cuts = pl.whole_items ? 0 : 128;  // after the line's length
-    pl.ml = pl.cuts + (pl.whole_items ? 0 : up(pl.ctas * static_cast<int64_t>(sizeof(int4))));
+    pl.ml = pl.whole_items ? 0 : up(pl.ctas * static_cast<int64_t>(sizeof(Cut)));
     pl.o = pl.ml + up(parts * pl.part_rows * static_cast<int64_t>(sizeof(float2)));
     pl.stats = pl.o + parts * pl.part_rows * head_dim * static_cast<int64_t>(sizeof(float));
     pl.bytes = pl.stats;
@@ -1721,8 +1742,7 @@ int run_attention(const char* op, CacheAttentionParams& p, int64_t head_dim, voi
     p.q_box_tokens = static_cast<int>(p.tokens < pl.tile_tokens ? p.tokens : pl.tile_tokens);
     p.whole_items = pl.whole_items;
     p.part_rows = pl.part_rows;
-    p.line = reinterpret_cast<int*>(base);
-    p.cuts = reinterpret_cast<int4*>(base + pl.cuts);
+    p.cuts = reinterpret_cast<Cut*>(base);
     p.part_ml = reinterpret_cast<float2*>(base + pl.ml);
     p.part_o = reinterpret_cast<float*>(base + pl.o);
     if (p.weights != nullptr) {
