@@ -539,6 +539,83 @@ def test_calls_on_two_streams_do_not_share_anything(ops):
         assert all(torch.equal(x, want[i]) for x in got[i])
 
 
+@pytest.mark.parametrize("tokens,capacity", [(3, 500), (3, 4000), (150, 700)])
+def test_waits_that_run_out_are_reported(ops, tokens, capacity):
+    """With a poll limit of 0 every first wait gives up at once: the error word is set, the copies still land and the
+    results stand; with the default limit it stays clear."""
+    from cppinf_b200 import capi
+
+    g = torch.Generator(device="cuda").manual_seed(14)
+    k, v = caches(g, 2, capacity, 4, 128, "dense")
+    q = torch.randn((2, tokens, 8, 128), generator=g, device="cuda").bfloat16()
+    n = torch.full((2,), capacity - tokens, device="cuda")
+    mask = torch.ones((tokens, tokens), dtype=torch.bool, device="cuda").tril()
+    error = torch.zeros(1, dtype=torch.int32, device="cuda")
+    w = torch.zeros((2, 4, capacity), device="cuda")
+    ctx = ops.tree_attention(q, k, v, n, mask, error=error)
+    ctx2 = ops.decoder_attention_weights(q, k, v, n, w, error=error)
+    assert error.item() == 0
+    previous = capi.set_wait_poll_limit(0)
+    try:
+        w2 = torch.zeros_like(w)
+        got = ops.tree_attention(q, k, v, n, mask, error=error)
+        assert error.item() == 1
+        error.zero_()
+        got2 = ops.decoder_attention_weights(q, k, v, n, w2, error=error)
+        assert error.item() == 1
+        ops.tree_attention(q, k, v, n, mask)  # nobody asked: nothing to report to
+    finally:
+        capi.set_wait_poll_limit(previous)
+    assert torch.equal(got, ctx) and torch.equal(got2, ctx2) and torch.equal(w2, w)
+
+
+def test_rows_past_32_bit_offsets(ops):
+    """Caches of more than 2^31 elements: the rows that count lie at the end."""
+    g = torch.Generator(device="cuda").manual_seed(15)
+    h, d, tail = 8, 256, 300
+    capacity = (1 << 31) // (h * d) + 2000
+    cache = torch.zeros((1, capacity, h, d), dtype=torch.bfloat16, device="cuda")
+    cache[:, -tail:] = torch.randn((1, tail, h, d), generator=g, device="cuda").bfloat16()
+    q = torch.randn((1, 4, 16, d), generator=g, device="cuda").bfloat16()
+    n = torch.tensor([capacity - 4], device="cuda")
+    mask = torch.ones((4, 4), dtype=torch.bool, device="cuda").tril()
+    got = ops.tree_attention(q, cache, cache, n, mask)
+    w = torch.zeros((1, h, capacity), device="cuda")
+    got2 = ops.decoder_attention_weights(q, cache, cache, n, w)
+    assert torch.equal(got, got2)
+    for head in (0, 15):
+        rows = cache[0, -tail:, head // 2].double()
+        s = q[0, :, head].double() @ rows.T / math.sqrt(d)
+        s.masked_fill_(~torch.ones_like(s, dtype=torch.bool).tril(tail - 4), -math.inf)
+        e = torch.exp(s - s.max(1, keepdim=True).values)
+        others = torch.exp(-s.max(1, keepdim=True).values) * (capacity - tail)  # zero keys: score 0
+        p = e / (e.sum(1, keepdim=True) + others)
+        ctx = p @ rows
+        off = (p @ rows.abs()) * (2.0 ** -8 + 2.0 ** -10)
+        assert ((got[0, :, head].double() - ctx).abs() <= off + 2.0 ** -8 * ctx.abs()).all()
+    total = w.double().sum(2)
+    assert ((total - 8).abs() < 8 * 2.0 ** -12).all()  # probabilities of 4 queries and 2 heads; f32 sums of 2^20 parts
+    k2, v2, w2, left, index = ops.cache_evict(cache, cache, w, n + 4, 64, 32)
+    assert int(left) == 64
+    for head in range(h):
+        rows = index[0, head]
+        assert (rows[1:] > rows[:-1]).all() and rows[-32:].tolist() == list(range(capacity - 32, capacity))
+        rest = w[0, head, :capacity - 32]
+        assert torch.equal(w2[0, head, :32].sort().values, rest.topk(32).values.sort().values)
+        assert torch.equal(k2[0, :, head], cache[0, rows, head]) and torch.equal(v2[0, :, head], cache[0, rows, head])
+    before = cache[0, -12:].clone()
+    n = torch.tensor([capacity - 12], device="cuda")
+    path = torch.tensor([[0, 3, 5]], device="cuda")
+    ops.tree_commit(cache, cache.clone(), n, path, torch.tensor([3], device="cuda"))
+    assert torch.equal(cache[0, -12:], before)  # of three nodes: 3 and 5 are none
+    path = torch.tensor([[0, 3, 5, -1, -1, -1]], device="cuda")
+    ops.tree_commit(cache, cache.clone(), n, path, torch.tensor([3], device="cuda"))
+    before[1], before[2] = before[3].clone(), before[5].clone()
+    assert torch.equal(cache[0, -12:], before)
+    del cache
+    torch.cuda.empty_cache()
+
+
 def test_refusals_on_the_device(ops):
     t = torch.zeros((1, 8, 2, 64), dtype=torch.bfloat16, device="cuda")
     q = torch.zeros((1, 2, 4, 64), dtype=torch.bfloat16, device="cuda")
