@@ -202,6 +202,26 @@ def test_tree_attention_nan_in_a_seen_row_and_in_a_query(ops):
     assert torch.equal(got[0, :, 3], clean[0, :, 3])
 
 
+@pytest.mark.parametrize("tokens,rows", [(2, 3000), (150, 3000)])
+def test_a_nan_query_stays_nan_through_the_join(ops, tokens, rows):
+    """Rows whose key tiles several CTAs take: a NaN query gives NaN, an infinite score too, and no other row does."""
+    g = torch.Generator(device="cuda").manual_seed(16)
+    q = torch.randn((1, tokens, 4, 128), generator=g, device="cuda").bfloat16()
+    k, v = caches(g, 1, rows + tokens, 2, 128, "dense")
+    n = torch.tensor([rows], device="cuda")
+    w = torch.zeros((1, 2, rows + tokens), device="cuda")
+    clean = ops.decoder_attention_weights(q, k, v, n, w)
+    q[0, 0, 1] = math.nan
+    got = ops.decoder_attention_weights(q, k, v, n, w.zero_())
+    assert torch.isnan(got[0, 0, 1]).all() and torch.isnan(w[0, 0, :rows + 1]).all() and torch.isfinite(w[0, 1]).all()
+    got[0, 0, 1] = clean[0, 0, 1]
+    assert torch.equal(got, clean)
+    q[0, 0, 1] = 1.0
+    k[0, rows // 2, 0] = math.inf
+    got = ops.decoder_attention_weights(q, k, v, n, w.zero_())
+    assert torch.isnan(got[0, 0, 1]).all()
+
+
 def test_new_rows_past_the_capacity_are_padding(ops):
     g = torch.Generator(device="cuda").manual_seed(6)
     q = torch.randn((3, 8, 4, 64), generator=g, device="cuda").bfloat16()
