@@ -249,8 +249,10 @@ int cppinf_cache_evict(cppinf_dtype dtype, const void* k_cache, const int64_t* k
                        int64_t kv_heads, int64_t head_dim, int64_t capacity, int64_t keep, int64_t recent,
                        int64_t sinks, int64_t out_capacity, void* stream) {
     CPPINF_REQUIRE(rt::valid_dtype(dtype), CPPINF_ERR_INVALID_ARGUMENT, "cache_evict received an unsupported dtype.");
-    CPPINF_REQUIRE(batch >= 0 && kv_heads >= 0 && head_dim >= 0 && capacity >= 0, CPPINF_ERR_INVALID_ARGUMENT,
+    CPPINF_REQUIRE(batch >= 0 && capacity >= 0, CPPINF_ERR_INVALID_ARGUMENT,
                    "cache_evict requires non-negative sizes.");
+    CPPINF_REQUIRE(kv_heads > 0 && head_dim > 0, CPPINF_ERR_INVALID_ARGUMENT,
+                   "cache_evict requires non-zero head configuration.");
     CPPINF_REQUIRE(recent >= 0 && sinks >= 0, CPPINF_ERR_INVALID_ARGUMENT,
                    "cache_evict requires non-negative recent and sinks.");
     CPPINF_REQUIRE(keep >= 1 && sinks <= keep && recent <= keep - sinks, CPPINF_ERR_INVALID_ARGUMENT,
@@ -260,11 +262,11 @@ int cppinf_cache_evict(cppinf_dtype dtype, const void* k_cache, const int64_t* k
     CPPINF_REQUIRE(head_dim * size % 16 == 0, CPPINF_ERR_UNSUPPORTED,
                    "cache_evict requires head sizes in multiples of 16 bytes.");
     constexpr int64_t kMost = int64_t{1} << 31;
-    CPPINF_REQUIRE(capacity < kMost && out_capacity < kMost && batch < (1 << 24) && kv_heads < (1 << 16) &&
+    CPPINF_REQUIRE(capacity < kMost / 2 && out_capacity < kMost / 2 && batch < (1 << 24) && kv_heads < (1 << 16) &&
                        head_dim < (1 << 16) && batch * kv_heads < kMost &&
-                       (batch * kv_heads == 0 || rt::ceil_div(out_capacity, kCopyRows) < kMost / (batch * kv_heads)),
+                       (batch == 0 || rt::ceil_div(out_capacity, kCopyRows) < kMost / (batch * kv_heads)),
                    CPPINF_ERR_OVERFLOW, "cache_evict sizes exceed the launch range.");
-    if (batch == 0 || kv_heads == 0 || head_dim == 0) {
+    if (batch == 0) {
         return rt::ok();
     }
     CPPINF_REQUIRE((capacity == 0 || (k_cache && v_cache && weights)) && k_strides && v_strides && lengths && k_out &&

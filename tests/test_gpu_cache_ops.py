@@ -501,10 +501,11 @@ def test_prompt_eviction_and_drafted_steps_together(ops):
             assert torch.equal(k2[b, :int(n2[b])], kept_k[b]) and torch.equal(v2[b, :int(n2[b])], kept_v[b])
 
 
-def test_captured_calls_follow_the_lengths(ops):
+@pytest.mark.parametrize("capacity,tokens", [(700, 10), (5000, 10), (3000, 200)])
+def test_captured_calls_follow_the_lengths(ops, capacity, tokens):
     """One graph of attention, accept, commit, weights and eviction, replayed for lengths and inputs that change."""
     g = torch.Generator(device="cuda").manual_seed(12)
-    batch, tokens, hq, h, d, capacity = 2, 10, 8, 2, 128, 700
+    batch, hq, h, d = 2, 8, 2, 128
     k, v = caches(g, batch, capacity, h, d, "dense")
     q = torch.randn((batch, tokens, hq, d), generator=g, device="cuda").bfloat16()
     n = torch.tensor([600, 100], device="cuda")
@@ -527,7 +528,7 @@ def test_captured_calls_follow_the_lengths(ops):
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         out = step(k, v, w)
-    for lengths in ([600, 100], [3, 0], [690, 333]):
+    for lengths in ([600, 100], [3, 0], [capacity - tokens, 333]):
         n.copy_(torch.tensor(lengths))
         q.copy_(torch.randn(q.shape, generator=g, device="cuda"))
         w.zero_()
@@ -536,6 +537,49 @@ def test_captured_calls_follow_the_lengths(ops):
         torch.cuda.synchronize()
         for x, y in zip(out, want):
             assert torch.equal(x, y)
+
+
+def test_empty_calls(ops):
+    none = torch.empty(0, dtype=torch.int64, device="cuda")
+    cache = torch.zeros((0, 8, 2, 64), dtype=torch.bfloat16, device="cuda")
+    q = torch.zeros((0, 3, 4, 64), dtype=torch.bfloat16, device="cuda")
+    mask = torch.ones((3, 3), dtype=torch.bool, device="cuda")
+    assert ops.tree_attention(q, cache, cache, none, mask).shape == q.shape
+    assert ops.decoder_attention_weights(q, cache, cache, none, torch.zeros((0, 2, 8), device="cuda")).shape == q.shape
+    ops.tree_commit(cache, cache, none, none.view(0, 0), none)
+    assert ops.cache_evict(cache, cache, torch.zeros((0, 2, 8), device="cuda"), none, 4, 2)[0].shape == (0, 4, 2, 64)
+    # no rows at all: every query is padding, every eviction keeps nothing
+    cache = torch.zeros((2, 0, 2, 64), dtype=torch.bfloat16, device="cuda")
+    q = torch.ones((2, 3, 4, 64), dtype=torch.bfloat16, device="cuda")
+    n = torch.zeros(2, dtype=torch.int64, device="cuda")
+    w = torch.zeros((2, 2, 0), device="cuda")
+    assert not ops.tree_attention(q, cache, cache, n, mask).any()
+    assert not ops.decoder_attention_weights(q, cache, cache, n, w).any()
+    k2, v2, w2, left, index = ops.cache_evict(cache, cache, w, n, 4, 2)
+    assert not k2.any() and not v2.any() and not w2.any() and left.tolist() == [0, 0] and (index == -1).all()
+    # and no tokens
+    cache = torch.zeros((2, 8, 2, 64), dtype=torch.bfloat16, device="cuda")
+    assert ops.tree_attention(q[:, :0], cache, cache, n, mask[:0, :0]).shape == (2, 0, 4, 64)
+
+
+@pytest.mark.parametrize("batch,tokens", [(700, 1), (300, 40)])
+def test_many_short_sequences(ops, batch, tokens):
+    """More sequences than a warp has lanes, lengths of every kind: each equals the sequence alone within its bound."""
+    g = torch.Generator(device="cuda").manual_seed(17)
+    h, d, capacity = 2, 64, 400
+    k, v = caches(g, batch, capacity, h, d, "dense")
+    q = torch.randn((batch, tokens, 2 * h, d), generator=g, device="cuda").bfloat16()
+    n = torch.randint(0, capacity - tokens + 1, (batch,), generator=g, device="cuda")
+    m = torch.randint(0, tokens + 1, (batch,), generator=g, device="cuda")
+    w = torch.zeros((batch, h, capacity), device="cuda")
+    got = ops.decoder_attention_weights(q, k, v, n, w, m)
+    causal = torch.ones((tokens, tokens), dtype=torch.bool, device="cuda").tril()
+    assert torch.equal(got, ops.tree_attention(q, k, v, n, causal, m))
+    some = list(range(0, batch, 37))
+    ctx, bound, weights, w_bound = reference(q[some], k[some], v[some], n[some].tolist(), m[some].tolist(),
+                                             lambda b: causal, capacity)
+    assert ((got[some].double() - ctx).abs() <= bound).all()
+    assert ((w[some].double() - weights).abs() <= w_bound + (2 * tokens + 2) * U * weights).all()
 
 
 def test_calls_on_two_streams_do_not_share_anything(ops):
