@@ -696,6 +696,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
         const uint32_t t_s = tmem + lanes + w * 128;
         const uint32_t t_o = tmem + lanes + L::kTmemO + w * D;
         const float c2 = 1.4426950408889634f / sqrtf(static_cast<float>(D));
+        int masked = -1;       // the entry whose mask bits the chain has in shared memory
         uint32_t s_phase = 0;  // a bit for each of the chain's two S
         uint32_t n = 0;        // tiles of the chain before the segment
         // Waits until the product of a tile, the last one whose S has been taken or the one before it, has reached O.
@@ -741,10 +742,15 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 if (row < 16) {
                     s_flags[w * 16 + row] = 0u;
                 }
-                if (p.mask != nullptr) {  // the tile's mask rows as bits
+                // The tile's mask rows as bits, the same for all heads of an entry. 1024 sequences of up to 300 rows: 425 us
+                // where each item makes them, 370 us.
+                if (p.mask != nullptr) {
                     uint32_t* words = s_mask + w * 128 * 9;
                     const int tokens = r.valid - token0 < p.tile_tokens ? r.valid - token0 : p.tile_tokens;
-                    for (int u = row; u < tokens * 9; u += 128) {  // a thread makes a word of 32 nodes
+                    const int entry = at.b * p.row_tiles + at.row_tile;
+                    const bool made = entry == masked;
+                    masked = entry;
+                    for (int u = row; u < tokens * 9 && !made; u += 128) {  // a thread makes a word of 32 nodes
                         const int token = u / 9;
                         const int node0 = (u - token * 9) * 32;
                         const uint8_t* mask =
