@@ -1001,12 +1001,15 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
     }
 }
 
-// Joins the parts of the items that a cut of the line went through: block (c, i) takes rows 32 i to 32 i + 31 of the
-// item that cut c + 1 is the first to go through, a lane a row, the columns over the warps.
-template <int D, int kKeys>
+// Joins the parts of the items that a cut of the line went through: block (c, i, j) takes rows 32 i to 32 i + 31 of the
+// item that cut c + 1 is the first to go through, a lane a row, and columns 32 kPieces j and on, a warp 4 kPieces of
+// them. An item has few parts, and a block takes all its columns; or, where few items have the whole line, over a hundred
+// of few rows, which blocks of 32 columns then share (one sequence of 32000 rows and one key-value head: 36.6 -> 28.6
+// us; but a batch of 66 rows a head would go from 31.0 to 34.3 us).
+template <int D, int kKeys, int kPieces>
 __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAttentionParams p, int ctas) {
-    constexpr int kPieces = D / 32;  // of four columns, for each thread
-    __shared__ uint2 s_rows[32][D / 4 + 1];
+    constexpr int kColumns = kPieces * 8;  // of four elements, of the block
+    __shared__ uint2 s_rows[32][kColumns + 1];
     __shared__ int64_t s_places[32];
     grid_dependency_begin();
     const int cut = static_cast<int>(blockIdx.x) + 1;
@@ -1030,20 +1033,19 @@ __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAt
     float top = -INFINITY;
     float sum = 0.0f;
     float o[kPieces][4] = {};
-    constexpr int kBatch = D == 256 ? 2 : 4;  // parts whose loads are in flight together
+    constexpr int kBatch = kPieces == 1 ? 8 : kPieces == 8 ? 2 : 4;  // parts whose loads are in flight together
+    const int64_t column = static_cast<int64_t>(blockIdx.z) * kColumns + warp * kPieces;
     for (int c0 = cut - 1; inside && c0 <= last; c0 += kBatch) {
         float2 ml[kBatch];
         float4 x[kBatch][kPieces];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            ml[j] = make_float2(-INFINITY, 0.0f);
             if (c0 + j <= last) {
                 const int64_t slot = 2 * static_cast<int64_t>(c0 + j) + (cuts.begin(c0 + j) >= first ? 0 : 1);
                 ml[j] = p.part_ml[slot * p.part_rows + row];
 #pragma unroll
                 for (int i = 0; i < kPieces; ++i) {
-                    x[j][i] = reinterpret_cast<const float4*>(
-                        p.part_o)[(slot * (D / 4) + warp * kPieces + i) * p.part_rows + row];
+                    x[j][i] = reinterpret_cast<const float4*>(p.part_o)[(slot * (D / 4) + column + i) * p.part_rows + row];
                 }
             }
         }
@@ -1074,17 +1076,18 @@ __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAt
                   : make_uint2(0u, 0u);
     }
     if (warp == 0) {
-        s_places[lane] = inside ? ((where.b * p.tokens + t) * p.q_heads + where.h * p.group + g) * D : -1;
-        if (inside && p.stats != nullptr) {
+        s_places[lane] =
+            inside ? ((where.b * p.tokens + t) * p.q_heads + where.h * p.group + g) * D + blockIdx.z * kColumns * 4 : -1;
+        if (inside && blockIdx.z == 0 && p.stats != nullptr) {
             p.stats[((where.b * p.kv_heads + where.h) * p.tokens + t) * p.group + g] =
                 valid ? make_float2(top == -INFINITY ? 0.0f : top, inv) : make_float2(0.0f, 0.0f);
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 32 * (D / 4); i += 256) {
-        const int64_t place = s_places[i / (D / 4)];
+    for (int i = threadIdx.x; i < 32 * kColumns; i += 256) {
+        const int64_t place = s_places[i / kColumns];
         if (place >= 0) {
-            reinterpret_cast<uint2*>(p.ctx + place)[i % (D / 4)] = s_rows[i / (D / 4)][i % (D / 4)];
+            reinterpret_cast<uint2*>(p.ctx + place)[i % kColumns] = s_rows[i / kColumns][i % kColumns];
         }
     }
 }
@@ -1700,8 +1703,11 @@ cudaError_t launch_cache_attention(const CacheAttentionParams& p, const Plan& pl
         return err;
     }
     runtime::count_launches(1);
-    return runtime::launch(cache_attention_join_kernel<D, L::kKeys>,
-                           dim3(static_cast<unsigned>(pl.ctas - 1), (static_cast<unsigned>(p.part_rows) + 31) / 32),
+    const bool shared = pl.part_rows <= 32 && pl.ctas > 4 * p.batch * p.row_tiles * p.kv_heads;
+    return runtime::launch(shared ? cache_attention_join_kernel<D, L::kKeys, 1>
+                                  : cache_attention_join_kernel<D, L::kKeys, D / 32>,
+                           dim3(static_cast<unsigned>(pl.ctas - 1), (static_cast<unsigned>(p.part_rows) + 31) / 32,
+                                shared ? D / 32 : 1),
                            dim3(256), s, 1u, p, pl.ctas);
 }
 

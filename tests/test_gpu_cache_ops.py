@@ -120,6 +120,9 @@ TREES = [
     (2, 3, 128, 1, 128, [2000, 129], None, "dense"),
     (3, 7, 5, 5, 64, [3000, 10, 1537], [7, 6, 2], "layer"),
     (1, 2, 10, 2, 256, [5000], None, "heads_first"),
+    (1, 1, 32, 1, 128, [30000], None, "dense"),
+    (1, 2, 8, 1, 64, [20000], None, "dense"),
+    (1, 3, 4, 1, 256, [9000], [2], "dense"),
 ]
 
 
