@@ -6,7 +6,9 @@ is the library's. Argument meaning, validation order and messages follow the ref
 Non-contiguous inputs are materialised with the library's own strided-gather kernel before the op runs.
 
 Also exposed: the fused forms the Qwen3 decoder block uses (residual add + RMSNorm, SiLU(gate)*up, per-head q/k
-RMSNorm + RoPE), the row argmax of the greedy sampler, and the position-aware causal softmax of attention.
+RMSNorm + RoPE), the row argmax of the greedy sampler, and the position-aware causal softmax of attention; and, without
+a counterpart in the reference, operators over batches of cached sequences: attention of drafted trees with the accepted
+path and its commit, attention that accumulates each cached row's weight, and eviction of the rows with the least of it.
 """
 
 from __future__ import annotations

@@ -504,6 +504,27 @@ def test_prompt_eviction_and_drafted_steps_together(ops):
             assert torch.equal(k2[b, :int(n2[b])], kept_k[b]) and torch.equal(v2[b, :int(n2[b])], kept_v[b])
 
 
+def test_rotary_positions_of_a_tree_from_a_gathered_table(ops):
+    """Nodes at one depth share a position: q/k norm + RoPE on a gathered table equals a call for each node."""
+    from cppinf_b200 import capi
+
+    g = torch.Generator(device="cuda").manual_seed(18)
+    hq, h, d, length = 16, 8, 128, 77
+    depth = torch.tensor([0, 1, 1, 2, 2, 3], device="cuda")
+    n = len(depth)
+    q = torch.randn((n, hq, d), generator=g, device="cuda").bfloat16()
+    k = torch.randn((n, h, d), generator=g, device="cuda").bfloat16()
+    wq, wk = (torch.randn(d, generator=g, device="cuda").bfloat16() for _ in "qk")
+    table = ops.rope_table(1e6, d, length + 4)[length + depth].contiguous()
+    q_out, k_out = torch.empty_like(q), torch.empty_like(k)
+    capi.call("cppinf_qk_norm_rope", capi.DTYPE_BF16, q.data_ptr(), k.data_ptr(), wq.data_ptr(), wk.data_ptr(),
+              q_out.data_ptr(), k_out.data_ptr(), n, hq, h, d, 0, 1e-6, table.data_ptr(), n,
+              torch.cuda.current_stream().cuda_stream)
+    for t in range(n):
+        want = ops.qk_norm_rope(q[t:t + 1], k[t:t + 1], wq, wk, 1e-6, length + int(depth[t]))
+        assert torch.equal(q_out[t:t + 1], want[0]) and torch.equal(k_out[t:t + 1], want[1])
+
+
 @pytest.mark.parametrize("capacity,tokens", [(700, 10), (5000, 10), (3000, 200)])
 def test_captured_calls_follow_the_lengths(ops, capacity, tokens):
     """One graph of attention, accept, commit, weights and eviction, replayed for lengths and inputs that change."""
