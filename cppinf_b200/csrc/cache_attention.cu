@@ -30,7 +30,6 @@
 // before the softmax, and V tiles in which some row is hidden from some query are cleared of such values in shared
 // memory before the product (0 * NaN would be NaN); values that are not finite in a row that a query does see are added
 // to its O afterwards.
-#include <atomic>
 #include <cmath>
 
 #include "common.cuh"
@@ -507,6 +506,9 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             }
         }
     }
+    if (groups > 1) {
+        fence_proxy_async_smem();  // the ring's loads come after the counts
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -699,8 +701,6 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
         int masked = -1;       // the entry whose mask bits the chain has in shared memory
         uint32_t s_phase = 0;  // a bit for each of the chain's two S
         uint32_t n = 0;        // tiles of the chain before the segment
-        // Waits until the product of a tile, the last one whose S has been taken or the one before it, has reached O.
-        // With two S each has a barrier for this: its last phase but one is over, since its S was complete after that.
         const auto hand_over = [&](uint64_t* bar) {
             tc_fence_before();
             __syncwarp();
@@ -708,6 +708,8 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 mbar_arrive(bar);
             }
         };
+        // Waits until the product of a tile, the last one whose S has been taken or the one before it, has reached O.
+        // With two S each has a barrier for this: its last phase but one is over, since its S was complete after that.
         const auto settled = [&](int i) {
             wait(bar_pv + 2 * w + i % L::kAhead, (s_phase >> (i % L::kAhead) & 1u) ^ 1u);
             tc_fence_after();
@@ -1613,7 +1615,8 @@ Plan plan(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads, int6
     const int64_t pieces = pl.whole_items ? items : pl.pair || head_dim == 256 ? most : (most + 1) / 2;
     pl.ctas = static_cast<int>(pieces < runtime::sm_count() ? pieces : runtime::sm_count());
     const int64_t products = batch * kv_heads * runtime::ceil_div(capacity, 128) * runtime::ceil_div(tokens, pl.tile_tokens);
-    pl.fits = batch * pl.row_tiles <= kMostEntries && most < (int64_t{1} << 29) && products < (int64_t{1} << 31);
+    // A line has up to four pieces for each tile (kSetUp and the tile itself).
+    pl.fits = batch * pl.row_tiles <= kMostEntries && most * (kSetUp + 1) < (int64_t{1} << 31) && products < (int64_t{1} << 31);
     const auto up = [](int64_t n) { return (n + 127) / 128 * 128; };
     const int64_t parts = pl.whole_items ? 0 : 2 * pl.ctas;
     pl.ml = pl.whole_items ? 0 : up(pl.ctas * static_cast<int64_t>(sizeof(Cut)));
@@ -1661,25 +1664,6 @@ bool encode_4d(CUtensorMap* map, const void* base, const int64_t (&dims)[4], con
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// A kernel's limit of dynamic shared memory, raised once on each device (the call costs a microsecond).
-struct SharedMemoryLimit {
-    std::atomic<uint64_t> raised{0};  // a bit for each of the first 64 devices
-
-    template <typename Kernel>
-    cudaError_t raise(Kernel kernel, std::size_t bytes) {
-        int device = 0;
-        cudaError_t err = cudaGetDevice(&device);
-        const uint64_t bit = device < 64 ? uint64_t{1} << device : 0;
-        if (err == cudaSuccess && (raised.load(std::memory_order_acquire) & bit) == 0) {
-            err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
-            if (err == cudaSuccess) {
-                raised.fetch_or(bit, std::memory_order_release);
-            }
-        }
-        return err;
-    }
-};
-
 template <int D, bool kPair>
 cudaError_t launch_cache_attention(const CacheAttentionParams& p, const Plan& pl, cudaStream_t s) {
     using L = Tiling<D, kPair>;
@@ -1692,7 +1676,7 @@ cudaError_t launch_cache_attention(const CacheAttentionParams& p, const Plan& pl
         !encode_4d(&mv, p.v, {D, p.kv_heads, p.capacity, p.batch}, {p.vs[2], p.vs[1], p.vs[0]}, {64, 1, L::kKeys, 1})) {
         return cudaErrorInvalidValue;
     }
-    static SharedMemoryLimit limit;
+    static runtime::SharedMemoryLimit limit;
     cudaError_t err = limit.raise(cache_attention_kernel<D, kPair>, L::kBytes);
     if (err != cudaSuccess) {
         return err;
@@ -1721,7 +1705,7 @@ cudaError_t launch_cache_weights(const CacheAttentionParams& p, cudaStream_t s) 
         !encode_4d(&mk, p.k, {D, p.kv_heads, p.capacity, p.batch}, {p.ks[2], p.ks[1], p.ks[0]}, {64, 1, 128, 1})) {
         return cudaErrorInvalidValue;
     }
-    static SharedMemoryLimit limit;
+    static runtime::SharedMemoryLimit limit;
     const cudaError_t err = limit.raise(cache_weights_kernel<D>, L::kBytes);
     if (err != cudaSuccess) {
         return err;
@@ -1744,7 +1728,7 @@ int check_sizes(const char* op, int64_t batch, int64_t tokens, int64_t q_heads, 
     CPPINF_REQUIRE(q_heads / kv_heads <= kMaxGroup, CPPINF_ERR_UNSUPPORTED,
                    name + " supports up to 128 query heads per key/value head.");
     constexpr int64_t kMost = int64_t{1} << 31;
-    CPPINF_REQUIRE(capacity < kMost / 2 && q_heads < (1 << 16) && batch < (1 << 24) &&
+    CPPINF_REQUIRE(capacity < kMost / 2 && q_heads < (1 << 16) && batch < (1 << 24) && tokens < kMost &&
                        (batch == 0 || tokens == 0 || tokens * q_heads < kMost / batch) &&
                        (batch == 0 || capacity == 0 || kv_heads < kMost * 4 / (batch * capacity)),
                    CPPINF_ERR_OVERFLOW, name + " sizes exceed the kernels' index range.");

@@ -274,8 +274,8 @@ int cppinf_cache_evict(cppinf_dtype dtype, const void* k_cache, const int64_t* k
                    CPPINF_ERR_INVALID_ARGUMENT, "cache_evict received a null pointer.");
     EvictParams p{};
     for (int i = 0; i < 3; ++i) {
-        CPPINF_REQUIRE(k_strides[i] >= 0 && v_strides[i] >= 0, CPPINF_ERR_INVALID_ARGUMENT,
-                       "cache_evict requires non-negative cache strides.");
+        CPPINF_REQUIRE(k_strides[i] > 0 && v_strides[i] > 0, CPPINF_ERR_INVALID_ARGUMENT,
+                       "cache_evict requires positive cache strides.");
         CPPINF_REQUIRE(k_strides[i] * size % 16 == 0 && v_strides[i] * size % 16 == 0, CPPINF_ERR_UNSUPPORTED,
                        "cache_evict requires cache strides in multiples of 16 bytes.");
         p.ks[i] = k_strides[i] * size;
@@ -304,10 +304,8 @@ int cppinf_cache_evict(cppinf_dtype dtype, const void* k_cache, const int64_t* k
     cudaError_t err = cudaSuccess;
     if (capacity <= kSharedKeys) {
         const std::size_t bytes = static_cast<std::size_t>(capacity) * sizeof(uint32_t);
-        if (bytes > 40960) {  // beside the kernel's own arrays, more than a CTA has without asking
-            CPPINF_CUDA_TRY(cudaFuncSetAttribute(evict_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 static_cast<int>(kSharedKeys * sizeof(uint32_t))));
-        }
+        static rt::SharedMemoryLimit limit;
+        CPPINF_CUDA_TRY(limit.raise(evict_select_kernel<true>, kSharedKeys * sizeof(uint32_t)));
         err = rt::launch_smem(evict_select_kernel<true>, dim3(heads), dim3(kSelectThreads), bytes, s, 1u, p);
     } else {
         err = rt::launch(evict_select_kernel<false>, dim3(heads), dim3(kSelectThreads), s, 1u, p);

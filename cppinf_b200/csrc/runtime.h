@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cstddef>
 #include <cstdint>
 #include <string>
 #include <utility>
@@ -108,6 +109,25 @@ cudaError_t launch(void (*kernel)(KernelArgs...), dim3 grid, dim3 block, cudaStr
                    Args&&... args) {
     return launch_smem(kernel, grid, block, 0, stream, cluster_x, std::forward<Args>(args)...);
 }
+
+// A kernel's limit of dynamic shared memory, raised once on each device (the call costs a microsecond).
+struct SharedMemoryLimit {
+    std::atomic<uint64_t> raised{0};  // a bit for each of the first 64 devices
+
+    template <typename Kernel>
+    cudaError_t raise(Kernel kernel, std::size_t bytes) {
+        int device = 0;
+        cudaError_t err = cudaGetDevice(&device);
+        const uint64_t bit = device < 64 ? uint64_t{1} << device : 0;
+        if (err == cudaSuccess && (raised.load(std::memory_order_acquire) & bit) == 0) {
+            err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+            if (err == cudaSuccess) {
+                raised.fetch_or(bit, std::memory_order_release);
+            }
+        }
+        return err;
+    }
+};
 
 // Adds `n` (possibly negative) to the launch count: replays of a captured graph, or captured launches that only
 // execute when the graph is replayed.

@@ -291,11 +291,6 @@ __device__ __forceinline__ bool elect_one() {
     return picked != 0u;
 }
 
-// Arrives at barrier `id` without waiting for it.
-__device__ __forceinline__ void named_barrier_arrive(int id, int threads) {
-    asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
-}
-
 // 2^x of the hardware, within 2 ulp.
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;

@@ -171,8 +171,8 @@ int cppinf_tree_commit(cppinf_dtype dtype, void* k_cache, const int64_t* k_strid
                    CPPINF_ERR_INVALID_ARGUMENT, "tree_commit received a null pointer.");
     CommitParams p{};
     for (int i = 0; i < 3; ++i) {
-        CPPINF_REQUIRE(k_strides[i] >= 0 && v_strides[i] >= 0, CPPINF_ERR_INVALID_ARGUMENT,
-                       "tree_commit requires non-negative cache strides.");
+        CPPINF_REQUIRE(k_strides[i] > 0 && v_strides[i] > 0, CPPINF_ERR_INVALID_ARGUMENT,
+                       "tree_commit requires positive cache strides.");
         CPPINF_REQUIRE(k_strides[i] * size % 16 == 0 && v_strides[i] * size % 16 == 0, CPPINF_ERR_UNSUPPORTED,
                        "tree_commit requires cache strides in multiples of 16 bytes.");
         p.ks[i] = k_strides[i] * size;
@@ -180,6 +180,7 @@ int cppinf_tree_commit(cppinf_dtype dtype, void* k_cache, const int64_t* k_strid
     }
     CPPINF_REQUIRE(rt::aligned16(k_cache) && rt::aligned16(v_cache), CPPINF_ERR_UNSUPPORTED,
                    "tree_commit requires 16-byte aligned caches.");
+    CPPINF_REQUIRE(k_cache != v_cache, CPPINF_ERR_INVALID_ARGUMENT, "tree_commit requires K and V caches of their own.");
     p.k = static_cast<char*>(k_cache);
     p.v = static_cast<char*>(v_cache);
     p.lengths = lengths;

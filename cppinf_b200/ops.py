@@ -489,9 +489,9 @@ def _cache_strides(t: torch.Tensor) -> tuple[int, int, int] | None:
     if h <= 1:
         sh = d
     if n <= 1:
-        sn = h * sh
+        sn = max(h, 1) * sh
     if b <= 1:
-        sb = n * sn
+        sb = max(n, 1) * sn
     vec = 16 // t.element_size()
     if sh < d or sb < d or sn < d or (sb | sn | sh) % vec or t.data_ptr() % 16:
         return None

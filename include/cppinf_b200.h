@@ -274,12 +274,12 @@ CPPINF_API int cppinf_decoder_attention_tc(const void* q, const void* k_cache, c
  * A cache is a K and a V tensor of [batch, capacity, kv_heads, head_dim] whose rows of head_dim elements are dense;
  * `k_strides` / `v_strides` are HOST arrays of 3 element strides {batch, row, head}, so views of a larger cache (one
  * layer of many, K and V interleaved) are read and written in place. Strides must be positive multiples of 16 bytes,
- * the base addresses 16-byte aligned, `ctx` 32-byte aligned. `lengths` (DEVICE int64, one per sequence) are the committed rows; the new tokens of
- * a call occupy the rows after them. They are read on the device, so a captured call follows them from replay to
- * replay; they cannot be refused there, so a length is taken as 0 below 0 and as the capacity above it, and a new token
- * whose row would lie past the capacity counts as padding. Query head h reads key-value head
- * h / (q_heads / kv_heads); up to 128 query heads share one. Rows of a cache that no query sees may hold anything, NaN
- * and infinities included.
+ * the base addresses 16-byte aligned, `ctx` 32-byte aligned. `lengths` (DEVICE int64, one per sequence) are the
+ * committed rows; the new tokens of a call occupy the rows after them. They are read on the device, so a captured call
+ * follows them from replay to replay; they cannot be refused there, so a length is taken as 0 below 0 and as the
+ * capacity above it, and a new token whose row would lie past the capacity counts as padding. Query head h reads
+ * key-value head h / (q_heads / kv_heads); up to 128 query heads share one. Rows of a cache that no query sees may hold
+ * anything, NaN and infinities included.
  * ------------------------------------------------------------------------------------------------------------- */
 
 /* Device scratch, in bytes, that cppinf_tree_attention (with_weights 0) or cppinf_decoder_attention_weights (1) needs
@@ -317,8 +317,8 @@ CPPINF_API int cppinf_tree_accept(const int64_t* tokens, const int64_t* parents,
 
 /* Moves an accepted path's cache rows behind the committed ones, in place: row lengths[b] + i of K and V takes row
  * lengths[b] + path[b, i] for i < counts[b] (path [batch, tokens] and counts as cppinf_tree_accept writes them;
- * ascending, path[b, i] >= i; an entry outside that order or past the new rows is skipped). Other rows, and `lengths`,
- * are left as they are: the caller adds counts to lengths when every layer's cache has been committed. */
+ * ascending, path[b, i] >= i; an entry below i or past the new rows is skipped). K and V share no rows. Other rows, and
+ * `lengths`, are left as they are: the caller adds counts to lengths when every layer's cache has been committed. */
 CPPINF_API int cppinf_tree_commit(cppinf_dtype dtype, void* k_cache, const int64_t* k_strides, void* v_cache,
                                   const int64_t* v_strides, const int64_t* lengths, const int64_t* path,
                                   const int64_t* counts, int64_t batch, int64_t tokens, int64_t kv_heads,

@@ -207,3 +207,23 @@ def test_cache_strides_say_which_views_are_read_in_place():
     assert ops._cache_strides(host(2, 8, 2, 68)[..., :64]) is None  # rows off the 16-byte grid
     assert ops._cache_strides(host(2, 8, 64, 2).transpose(2, 3)) is None
     assert ops._cache_strides(host(1, 8, 1, 64)) == (512, 64, 64)
+
+
+def test_cache_strides_of_empty_caches():
+    assert ops._cache_strides(host(1, 0, 2, 64)) == (128, 128, 64)
+    assert ops._cache_strides(host(1, 8, 2, 64)[:, :0]) == (128, 128, 64)
+
+
+def test_commit_refuses_one_cache_for_both_and_broadcast_strides(lib):
+    assert commit(lib) == capi.ERR_INVALID_ARGUMENT
+    assert b"of their own" in lib.cppinf_last_error()
+    assert commit(lib, k=P + 4096, ks=(0, 128, 64)) == capi.ERR_INVALID_ARGUMENT
+    assert evict(lib, ks=(0, 128, 64)) == capi.ERR_INVALID_ARGUMENT
+
+
+def test_attention_sizes_that_pass_the_index_range(lib):
+    args = (8, 2, 64, 1024)
+    assert lib.cppinf_cache_attention_scratch_bytes(1, 1 << 60, *args, 1) == -1  # tokens * q_heads wraps round
+    assert lib.cppinf_cache_attention_scratch_bytes(1, 1 << 61, *args, 1) == -1
+    # 2^16 * 2^13 heads of one tile each: 2^29 tiles, and with an item's set-up before each 2^31 pieces.
+    assert lib.cppinf_cache_attention_scratch_bytes(1 << 16, 1, 1 << 13, 1 << 13, 64, 16, 0) == -1

@@ -14,6 +14,9 @@ the exponential and the sum: |dp_j| <= p_j (4.5 e + 2^-18), while 4e stays below
 from __future__ import annotations
 
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -725,3 +728,29 @@ def test_refusals_on_the_device(ops):
     with pytest.raises(ValueError, match="dense 16-byte aligned rows"):
         odd = torch.zeros((1, 8, 2, 68), dtype=torch.bfloat16, device="cuda")[..., :64]
         ops.tree_commit(odd, odd, n, torch.zeros((1, 2), dtype=torch.int64, device="cuda"), n)
+
+
+@pytest.mark.parametrize("capacity", [8192, 10174, 10175, 10240, 12288])
+def test_cache_evict_around_the_default_shared_memory(ops, capacity):
+    """In a process of its own, whose first eviction it is: an earlier one of a longer cache raises the kernel's limit."""
+    code = (
+        "import torch\n"
+        "from cppinf_b200 import ops\n"
+        f"n = {capacity}\n"
+        "g = torch.Generator(device='cuda').manual_seed(5)\n"
+        "k = torch.randn(1, n, 1, 64, device='cuda', generator=g).bfloat16()\n"
+        "w = torch.rand(1, 1, n, device='cuda', generator=g)\n"
+        "out = ops.cache_evict(k, k, w, torch.tensor([n], device='cuda'), 64, 16)\n"
+        "rows = w[0, 0, :n - 16].sort(descending=True, stable=True).indices[:48].sort().values\n"
+        "assert torch.equal(out[4][0, 0, :48], rows)\n"
+        "assert torch.equal(out[0][0, :48], k[0, rows])\n"
+    )
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr
+
+
+def test_commit_of_an_empty_cache(ops):
+    k = torch.zeros(1, 0, 2, 64, dtype=torch.bfloat16, device="cuda")
+    n = torch.zeros(1, dtype=torch.int64, device="cuda")
+    ops.tree_commit(k, k.clone(), n, torch.zeros(1, 4, dtype=torch.int64, device="cuda"), n)
