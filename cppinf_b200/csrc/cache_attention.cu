@@ -68,7 +68,7 @@ struct CacheAttentionParams {
     const uint8_t* mask;     // tree: [T, T] at mask + b * mask_stride; null: causal
     int64_t mask_stride;
     bf16* ctx;        // [B, T, Hq, D]
-    float2* stats;    // [B, Hkv, T, G] (M in base 2, 1 / l), or null
+    float* stats;     // [B, Hkv, T, G] M + log2(l) in base 2, infinite for rows of no weight, or null
     float* weights;   // [B, Hkv, capacity]
     int64_t batch;
     int64_t tokens;
@@ -364,6 +364,12 @@ __device__ __forceinline__ uint32_t zero_times(uint32_t pair, uint32_t acc) {
     uint32_t d;
     asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(pair), "r"(0u), "r"(acc));
     return d;
+}
+
+// What a row's probabilities are taken against for the weights: exp2(s - M) / l = exp2(s - (M + log2 l)). Its rounding
+// counts for less than that of the scores, whose largest it exceeds by log2(l) at most.
+__device__ __forceinline__ float whole_statistic(float top, float sum) {
+    return sum == 0.0f ? INFINITY : top + log2f(sum);
 }
 
 template <int D, bool kPair>
@@ -719,14 +725,14 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             const int t = token0 + token_in_tile;
             const bool inside = token_in_tile < p.tile_tokens && t < p.tokens;  // a row of ctx
             bf16* ctx = p.ctx + ((at.b * p.tokens + t) * p.q_heads + at.h * p.group + g) * D;
-            float2* stats = p.stats + ((at.b * p.kv_heads + at.h) * p.tokens + t) * p.group + g;
+            float* stats = p.stats + ((at.b * p.kv_heads + at.h) * p.tokens + t) * p.group + g;
             if (w >= chains) {  // nothing to do in this segment, but for rows of padding
                 if (kPair && inside && tile0 == 0) {
                     for (int c = 0; c < D; c += 16) {
                         st_stream32(ctx + c, U8{});
                     }
                     if (p.stats != nullptr) {
-                        *stats = make_float2(0.0f, 0.0f);
+                        *stats = INFINITY;
                     }
                 }
                 n += kPair ? static_cast<uint32_t>(count) : 0u;
@@ -982,8 +988,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 if (inside && !whole) {
                     p.part_ml[part * p.part_rows + part_row] = make_float2(scaled_top, sum);
                 } else if (inside && p.stats != nullptr) {
-                    *stats = valid ? make_float2(scaled_top == -INFINITY ? 0.0f : scaled_top, inv)
-                                   : make_float2(0.0f, 0.0f);
+                    *stats = valid ? whole_statistic(scaled_top, sum) : INFINITY;
                 }
             }
             tc_fence_before();
@@ -1082,7 +1087,7 @@ __global__ void __launch_bounds__(256) cache_attention_join_kernel(const CacheAt
             inside ? ((where.b * p.tokens + t) * p.q_heads + where.h * p.group + g) * D + blockIdx.z * kColumns * 4 : -1;
         if (inside && blockIdx.z == 0 && p.stats != nullptr) {
             p.stats[((where.b * p.kv_heads + where.h) * p.tokens + t) * p.group + g] =
-                valid ? make_float2(top == -INFINITY ? 0.0f : top, inv) : make_float2(0.0f, 0.0f);
+                valid ? whole_statistic(top, sum) : INFINITY;
         }
     }
     __syncthreads();
@@ -1106,14 +1111,15 @@ struct WeightTiling {
     static constexpr int kKeySlots = D == 256 ? 1 : 2;
     static constexpr int kSlots = D == 64 ? 8 : D == 128 ? 4 : 2;
     static constexpr int kBuffers = 4;
-    static constexpr int kThreads = 384;
+    static constexpr int kGroups = 4;  // warpgroups that turn products into sums; a group keeps to one buffer
+    static constexpr int kThreads = 128 + 128 * kGroups;
     static constexpr uint32_t kAtom = 128 * 128;
     static constexpr uint32_t kTile = kAtom * kAtoms;
     static constexpr uint32_t kK = 0;
     static constexpr uint32_t kRing = kK + kKeySlots * kTile;
-    static constexpr uint32_t kStats = kRing + kSlots * kTile;     // [groups][2][2][128] M, then 1 / l
-    static constexpr uint32_t kSum = kStats + 2 * 2 * 128 * 8;     // [128] the second group's sums
-    static constexpr uint32_t kBars = kSum + 128 * 4;
+    static constexpr uint32_t kStats = kRing + kSlots * kTile;     // [groups][2][128]
+    static constexpr uint32_t kSum = kStats + kGroups * 2 * 128 * 4;  // [groups - 1][128] the other groups' sums
+    static constexpr uint32_t kBars = kSum + (kGroups - 1) * 128 * 4;
     static constexpr std::size_t kBytes = 1024 + kBars + 256;
     static_assert(kBytes <= 232448, "shared memory of a CTA");
 };
@@ -1140,17 +1146,20 @@ __device__ __forceinline__ KeyRange key_range(const CacheAttentionParams& p, int
     return r;
 }
 
-// Products of key tiles [kt0, kt0 + 32) of a sequence's head, one tile a lane.
-__device__ __forceinline__ int lane_products(const CacheAttentionParams& p, const KeyRange& r, int kt0) {
+// A unit's share of the line: its products, and before them kUnitSetUp pieces without any for what it costs besides.
+constexpr int kUnitSetUp = 3;
+
+// Pieces of key tiles [kt0, kt0 + 32) of a sequence's head, one tile a lane.
+__device__ __forceinline__ int lane_pieces(const CacheAttentionParams& p, const KeyRange& r, int kt0) {
     const int kt = kt0 + static_cast<int>(threadIdx.x & 31);
-    return kt < r.key_tiles ? r.q_tiles - r.first(kt, p.by_tile_tokens) : 0;
+    return kt < r.key_tiles ? r.q_tiles - r.first(kt, p.by_tile_tokens) + kUnitSetUp : 0;
 }
 
-// Products of one head of a sequence, by a whole warp.
-__device__ __forceinline__ int head_products(const CacheAttentionParams& p, const KeyRange& r) {
+// Pieces of one head of a sequence, by a whole warp.
+__device__ __forceinline__ int head_pieces(const CacheAttentionParams& p, const KeyRange& r) {
     int sum = 0;
     for (int kt0 = 0; kt0 < r.key_tiles; kt0 += 32) {
-        sum += lane_products(p, r, kt0);
+        sum += lane_pieces(p, r, kt0);
     }
     return __reduce_add_sync(0xffffffffu, sum);
 }
@@ -1165,14 +1174,14 @@ __device__ __forceinline__ KeyRange from_lane(const KeyRange& r, int lane) {
     return other;
 }
 
-// The line of products is cut like the attention's; a unit is one key tile of one head.
+// The line of pieces is cut like the attention's; a unit is one key tile of one head.
 struct UnitWalk {
     int b;
     int kt;
     int h;
-    int q;       // first query tile of the current segment, counted from the unit's first
+    int piece;   // the current unit's first piece that the part has
     int left;
-    int begin;   // the current segment's place on the line
+    int begin;   // that piece's place on the line
     int total;
     uint32_t products;  // before the current segment
     int index;
@@ -1196,14 +1205,14 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
     uint64_t* bar_free = bar_s + L::kBuffers;      // [buffers] and read
     __shared__ uint32_t s_tmem;
     __shared__ uint32_t s_stop;
-    __shared__ uint32_t s_last[2];
+    __shared__ uint32_t s_last[L::kGroups];
     __shared__ UnitWalk s_walk;
 
     const int tid = threadIdx.x;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int lane = tid & 31;
     const int columns = p.q_box_tokens * p.group;       // rows of a query tile, columns of the product
-    const int chunks = (columns + 63) / 64;             // of 64 columns
+    const int chunks = (columns + 31) / 32;             // of 32 columns
     if (tid == 0) {
         s_stop = 0u;
         for (int i = 0; i < L::kSlots; ++i) {
@@ -1242,7 +1251,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
             if (b > 0 && b % 32 == 0) {
                 mine = ranges_of(b);
             }
-            total += head_products(p, from_lane(mine, b % 32)) * heads;
+            total += head_pieces(p, from_lane(mine, b % 32)) * heads;
         }
         const Cuts cuts(total, static_cast<int>(gridDim.x));
         const int begin = cuts.begin(static_cast<int>(blockIdx.x));
@@ -1260,14 +1269,14 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
                     mine = ranges_of(w.b);
                 }
                 r = from_lane(mine, w.b % 32);
-                const int here = head_products(p, r) * heads;
+                const int here = head_pieces(p, r) * heads;
                 if (rest < here) {
                     break;
                 }
                 rest -= here;
             }
             for (int kt0 = 0;; kt0 += 32) {  // the key tile; order within a sequence: key tile, head, query tile
-                const int here = lane_products(p, r, kt0) * heads;
+                const int here = lane_pieces(p, r, kt0) * heads;
                 int sum = here;
                 for (int offset = 1; offset < 32; offset <<= 1) {
                     const int other = __shfl_up_sync(0xffffffffu, sum, offset);
@@ -1282,9 +1291,9 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
                 }
                 rest -= __shfl_sync(0xffffffffu, sum, 31);
             }
-            const int each = r.q_tiles - r.first(w.kt, p.by_tile_tokens);
+            const int each = r.q_tiles - r.first(w.kt, p.by_tile_tokens) + kUnitSetUp;
             w.h = rest / each;
-            w.q = rest - w.h * each;
+            w.piece = rest - w.h * each;
             w.left = end - begin;
             w.begin = begin;
         }
@@ -1299,17 +1308,18 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
     const Waiter wait{p.error, p.poll_limit, &s_stop};
     UnitWalk at = s_walk;
     KeyRange r = at.left > 0 ? key_range(p, at.b) : KeyRange{};
-    const auto step = [&](int count, int tiles) {
-        at.left -= count;
-        at.begin += count;
-        at.products += static_cast<uint32_t>(count);
-        ++at.index;
-        at.q += count;
-        if (at.q < tiles) {
-            return;
-        }
-        at.q = 0;
-        if (++at.h < static_cast<int>(p.kv_heads)) {
+    // The current segment: its unit's first query tile and their number, the first of those that it takes, counted from
+    // the unit's first, and how many.
+    int q0 = 0;
+    int tiles = 0;
+    int tile0 = 0;
+    int count = 0;
+    const auto advance_unit = [&]() {
+        const int rest = tiles + kUnitSetUp - at.piece;
+        at.left -= rest;
+        at.begin += rest;
+        at.piece = 0;
+        if (at.left <= 0 || ++at.h < static_cast<int>(p.kv_heads)) {
             return;
         }
         at.h = 0;
@@ -1317,20 +1327,37 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
             return;
         }
         at.kt = 0;
-        while (at.left > 0 && ++at.b < static_cast<int>(p.batch)) {
+        while (++at.b < static_cast<int>(p.batch)) {
             r = key_range(p, at.b);
             if (r.key_tiles > 0) {
                 break;
             }
         }
     };
+    const auto segment = [&]() {
+        for (;; advance_unit()) {
+            if (at.left <= 0) {
+                return false;
+            }
+            q0 = r.first(at.kt, p.by_tile_tokens);
+            tiles = r.q_tiles - q0;
+            tile0 = at.piece > kUnitSetUp ? at.piece - kUnitSetUp : 0;
+            const int end = at.piece + at.left - kUnitSetUp;
+            count = (end < tiles ? end : tiles) - tile0;
+            if (count > 0) {
+                return true;
+            }
+        }
+    };
+    const auto next = [&]() {
+        ++at.index;
+        at.products += static_cast<uint32_t>(count);
+        advance_unit();
+    };
 
     if (warp == 0) {
         {  // ---- loads
-            while (at.left > 0) {
-                const int q0 = r.first(at.kt, p.by_tile_tokens);
-                const int tiles = r.q_tiles - q0;
-                const int count = tiles - at.q < at.left ? tiles - at.q : at.left;
+            for (; segment(); next()) {
                 const uint32_t ks = static_cast<uint32_t>(at.index) % L::kKeySlots;
                 const uint32_t kr = static_cast<uint32_t>(at.index) / L::kKeySlots;
                 if (kr > 0) {
@@ -1356,20 +1383,17 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
 #pragma unroll
                         for (int a = 0; a < L::kAtoms; ++a) {
                             tma_load_4d(sm + L::kRing + slot * L::kTile + a * L::kAtom, &map_q, a * 64, at.h * p.group,
-                                        (q0 + at.q + i) * p.tile_tokens, at.b, bar_full + slot);
+                                        (q0 + tile0 + i) * p.tile_tokens, at.b, bar_full + slot);
                         }
                     }
                     __syncwarp();
                 }
-                step(count, tiles);
             }
         }
     } else if (warp == 1) {
         {  // ---- matrix products
-            const uint32_t idesc = idesc_bf16_f32(chunks * 64);
-            while (at.left > 0) {
-                const int tiles = r.q_tiles - r.first(at.kt, p.by_tile_tokens);
-                const int count = tiles - at.q < at.left ? tiles - at.q : at.left;
+            const uint32_t idesc = idesc_bf16_f32(chunks * 32);
+            for (; segment(); next()) {
                 const uint32_t ks = static_cast<uint32_t>(at.index) % L::kKeySlots;
                 wait(bar_k_full + ks, static_cast<uint32_t>(at.index) / L::kKeySlots & 1u);
                 for (int i = 0; i < count; ++i) {
@@ -1398,75 +1422,71 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
                     }
                     __syncwarp();
                 }
-                step(count, tiles);
             }
         }
-    } else if (warp >= 4) {  // ---- probabilities: one thread per key, the products in turn with the other group
+    } else if (warp >= 4) {  // ---- probabilities: one thread per key, the groups' products in turn
         const int w = (warp - 4) >> 2;
         const int row = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const float c2 = 1.4426950408889634f / sqrtf(static_cast<float>(D));
         uint32_t turn = 0;  // which of the group's two copies of the statistics
-        // Starts the copy of a query tile's statistics into the group's next place; zeros for columns that count for
+        // Starts the copy of a query tile's statistics into the group's next place; infinity for columns that count for
         // nothing.
         const auto fetch = [&](int token0) {
             const int inside = r.valid - token0 < p.tile_tokens ? r.valid - token0 : p.tile_tokens;
-            const float2* st = p.stats + ((at.b * p.kv_heads + at.h) * p.tokens + token0) * p.group + row;
-            float* to = s_stats + (w * 2 + turn) * 256 + row;
-            const bool there = row < inside * p.group;
-            cp_async4(to, there ? &st->x : &p.stats->x, there);
-            cp_async4(to + 128, there ? &st->y : &p.stats->x, there);
+            float* to = s_stats + (w * 2 + turn) * 128 + row;
+            if (row < inside * p.group) {
+                cp_async4(to, p.stats + ((at.b * p.kv_heads + at.h) * p.tokens + token0) * p.group + row);
+            } else {
+                *to = INFINITY;
+            }
         };
-        while (at.left > 0) {
-            const int q0 = r.first(at.kt, p.by_tile_tokens);
-            const int tiles = r.q_tiles - q0;
-            const int count = tiles - at.q < at.left ? tiles - at.q : at.left;
+        for (; segment(); next()) {
             const int key = at.kt * 128 + row;
-            const int first = (at.products & 1u) == static_cast<uint32_t>(w) ? 0 : 1;  // of the segment's products
+            const int first = (w - static_cast<int>(at.products)) & (L::kGroups - 1);  // of the segment's products
             float2 part[2] = {};
             if (first < count) {
-                fetch((q0 + at.q + first) * p.tile_tokens);
+                fetch((q0 + tile0 + first) * p.tile_tokens);
             }
-            for (int i = first; i < count; i += 2) {
+            for (int i = first; i < count; i += L::kGroups) {
                 const uint32_t n = at.products + static_cast<uint32_t>(i);
                 const uint32_t buffer = n % L::kBuffers;
-                const int token0 = (q0 + at.q + i) * p.tile_tokens;
+                const int token0 = (q0 + tile0 + i) * p.tile_tokens;
                 const int inside = r.valid - token0 < p.tile_tokens ? r.valid - token0 : p.tile_tokens;
-                const float* stats = s_stats + (w * 2 + turn) * 256;
+                const float* stats = s_stats + (w * 2 + turn) * 128;
                 turn ^= 1u;
                 cp_async_wait_all();
                 named_barrier(1 + w, 128);  // the statistics are there, and nobody reads the ones before
-                if (i + 2 < count) {
-                    fetch(token0 + 2 * p.tile_tokens);
+                if (i + L::kGroups < count) {
+                    fetch(token0 + L::kGroups * p.tile_tokens);
                 }
                 wait(bar_s + buffer, n / L::kBuffers & 1u);
                 tc_fence_after();
-                const bool partial = inside < p.tile_tokens || at.kt * 128 + 127 - r.len > token0;
+                const bool partial = inside < p.tile_tokens || columns < chunks * 32 || at.kt * 128 + 127 - r.len > token0;
                 const int low = (key - r.len - token0) * p.group;  // columns below do not see the key
                 const int high = inside * p.group;                 // columns from here on count for nothing
 #pragma unroll 1
                 for (int c = 0; c < chunks; ++c) {
-                    float x[64];
-                    tmem_load_begin<64>(tmem + lanes + buffer * 128 + c * 64, x);
-                    tmem_load_end<64>(x);
+                    float x[32];
+                    tmem_load_begin<32>(tmem + lanes + buffer * 128 + c * 32, x);
+                    tmem_load_end<32>(x);
 #pragma unroll
-                    for (int j = 0; j < 64; j += 4) {
-                        const float4 top = *reinterpret_cast<const float4*>(stats + c * 64 + j);
-                        const float4 inv = *reinterpret_cast<const float4*>(stats + 128 + c * 64 + j);
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 top = *reinterpret_cast<const float4*>(stats + c * 32 + j);
                         float2 e0 = __ffma2_rn(make_float2(x[j], x[j + 1]), make_float2(c2, c2), make_float2(-top.x, -top.y));
                         float2 e1 = __ffma2_rn(make_float2(x[j + 2], x[j + 3]), make_float2(c2, c2),
                                                make_float2(-top.z, -top.w));
                         e0 = make_float2(exp2_approx(e0.x), exp2_approx(e0.y));
                         e1 = make_float2(exp2_approx(e1.x), exp2_approx(e1.y));
                         if (partial) {
-                            const int column = c * 64 + j;
+                            const int column = c * 32 + j;
                             e0.x = column >= low && column < high ? e0.x : 0.0f;
                             e0.y = column + 1 >= low && column + 1 < high ? e0.y : 0.0f;
                             e1.x = column + 2 >= low && column + 2 < high ? e1.x : 0.0f;
                             e1.y = column + 3 >= low && column + 3 < high ? e1.y : 0.0f;
                         }
-                        part[0] = __ffma2_rn(e0, make_float2(inv.x, inv.y), part[0]);
-                        part[1] = __ffma2_rn(e1, make_float2(inv.z, inv.w), part[1]);
+                        part[0] = __fadd2_rn(part[0], e0);
+                        part[1] = __fadd2_rn(part[1], e1);
                     }
                 }
                 tc_fence_before();
@@ -1477,14 +1497,16 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
             }
             float sum = (part[0].x + part[0].y) + (part[1].x + part[1].y);
             bool writes = first < count;
-            if (count > 1) {  // both groups had products of the unit: the second hands its sums to the first
-                if (w == 1) {
-                    s_sum[row] = sum;
+            if (count > 1) {  // several groups had products of the unit: they hand their sums to the first
+                if (w > 0) {
+                    s_sum[(w - 1) * 128 + row] = sum;
                 }
-                named_barrier(3, 256);
-                sum = w == 0 ? sum + s_sum[row] : sum;
+                named_barrier(1 + L::kGroups, 128 * L::kGroups);
+                for (int other = 0; w == 0 && other < L::kGroups - 1; ++other) {
+                    sum += s_sum[other * 128 + row];
+                }
                 writes = w == 0;
-                named_barrier(3, 256);
+                named_barrier(1 + L::kGroups, 128 * L::kGroups);
             }
             if (writes) {
                 const bool seen = key < r.len + r.valid;
@@ -1495,12 +1517,12 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
                     }
                 } else {
                     // A cut went through the unit: whoever leaves the last of its parts adds them up in their order.
-                    const int first = at.begin - at.q;
+                    const int first = at.begin - at.piece;
                     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (at.index == 0 ? 0 : 1);
                     p.part_sums[slot * 128 + row] = sum;
                     const Cuts cuts(at.total, static_cast<int>(gridDim.x));
-                    const int c0 = cuts.of(first);
-                    const int c1 = cuts.of(first + tiles - 1);  // parts between them are not empty
+                    const int c0 = cuts.of(first + kUnitSetUp);
+                    const int c1 = cuts.of(first + kUnitSetUp + tiles - 1);  // parts between them are not empty
                     __threadfence();
                     named_barrier(1 + w, 128);
                     if (row == 0) {
@@ -1519,7 +1541,6 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
                     }
                 }
             }
-            step(count, tiles);
         }
     }
     tc_fence_before();
@@ -1534,7 +1555,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
 // The weights from kept scores: a thread takes four keys of a head and adds their probabilities over the head's rows.
 // Scores that a row does not see were kept as -inf.
 __global__ void __launch_bounds__(256) cache_weights_kept_kernel(const CacheAttentionParams p, float c2) {
-    __shared__ float2 s_stats[kMaxKeptRows];
+    __shared__ float s_stats[kMaxKeptRows];
     grid_dependency_begin();
     const unsigned blocks = static_cast<unsigned>((p.capacity + 1023) / 1024);  // of a head
     const int64_t head = blockIdx.x / blocks;                                     // of all sequences
@@ -1557,11 +1578,11 @@ __global__ void __launch_bounds__(256) cache_weights_kept_kernel(const CacheAtte
 #pragma unroll 4
         for (int i = 0; i < rows; ++i) {
             const float4 x = __ldcg(reinterpret_cast<const float4*>(scores + i * p.score_stride));
-            const float2 st = s_stats[i];
-            sum[0] = __fmaf_rn(exp2_approx(__fmaf_rn(x.x, c2, -st.x)), st.y, sum[0]);
-            sum[1] = __fmaf_rn(exp2_approx(__fmaf_rn(x.y, c2, -st.x)), st.y, sum[1]);
-            sum[2] = __fmaf_rn(exp2_approx(__fmaf_rn(x.z, c2, -st.x)), st.y, sum[2]);
-            sum[3] = __fmaf_rn(exp2_approx(__fmaf_rn(x.w, c2, -st.x)), st.y, sum[3]);
+            const float st = s_stats[i];
+            sum[0] += exp2_approx(__fmaf_rn(x.x, c2, -st));
+            sum[1] += exp2_approx(__fmaf_rn(x.y, c2, -st));
+            sum[2] += exp2_approx(__fmaf_rn(x.z, c2, -st));
+            sum[3] += exp2_approx(__fmaf_rn(x.w, c2, -st));
         }
     }
     float* out = p.weights + head * p.capacity + key;
@@ -1615,8 +1636,8 @@ Plan plan(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads, int6
     const int64_t pieces = pl.whole_items ? items : pl.pair || head_dim == 256 ? most : (most + 1) / 2;
     pl.ctas = static_cast<int>(pieces < runtime::sm_count() ? pieces : runtime::sm_count());
     const int64_t products = batch * kv_heads * runtime::ceil_div(capacity, 128) * runtime::ceil_div(tokens, pl.tile_tokens);
-    // A line has up to four pieces for each tile (kSetUp and the tile itself).
-    pl.fits = batch * pl.row_tiles <= kMostEntries && most * (kSetUp + 1) < (int64_t{1} << 31) && products < (int64_t{1} << 31);
+    // A line has up to four pieces for each tile or product, its set-up's and itself.
+    pl.fits = batch * pl.row_tiles <= kMostEntries && most * (kSetUp + 1) < (int64_t{1} << 31) && products * (kUnitSetUp + 1) < (int64_t{1} << 31);
     const auto up = [](int64_t n) { return (n + 127) / 128 * 128; };
     const int64_t parts = pl.whole_items ? 0 : 2 * pl.ctas;
     pl.ml = pl.whole_items ? 0 : up(pl.ctas * static_cast<int64_t>(sizeof(Cut)));
@@ -1624,7 +1645,7 @@ Plan plan(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads, int6
     pl.stats = pl.o + parts * pl.part_rows * head_dim * static_cast<int64_t>(sizeof(float));
     pl.bytes = pl.stats;
     if (with_stats) {
-        pl.sums = pl.stats + up(batch * tokens * q_heads * static_cast<int64_t>(sizeof(float2)));
+        pl.sums = pl.stats + up(batch * tokens * q_heads * static_cast<int64_t>(sizeof(float)));
         // Keeping a key's scores for the weights moves 8 bytes for each row, mostly within L2; forming them again reads
         // the key's 2 * head_dim bytes of K from memory and takes a tile's products. Eight sequences of 16000 rows, 8
         // heads of 128: 106 against 162 us with 2 rows, 125 against 163 with 16, 149 against 164 with 32, 223 against
@@ -1773,7 +1794,7 @@ int run_attention(const char* op, CacheAttentionParams& p, int64_t head_dim, voi
     p.part_ml = reinterpret_cast<float2*>(base + pl.ml);
     p.part_o = reinterpret_cast<float*>(base + pl.o);
     if (p.weights != nullptr) {
-        p.stats = reinterpret_cast<float2*>(base + pl.stats);
+        p.stats = reinterpret_cast<float*>(base + pl.stats);
         p.scores = pl.score_stride > 0 ? reinterpret_cast<float*>(base + pl.scores) : nullptr;
         p.score_stride = pl.score_stride;
         p.weight_ctas = pl.weight_ctas;
