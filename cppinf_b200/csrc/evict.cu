@@ -2,13 +2,12 @@
 // `sinks`, the last `recent` and the heaviest of the others stay, `keep` in all, in their order.
 //
 // Two kernels. The first finds the kept rows, one CTA per sequence and head: weights map to unsigned keys of the same
-// order (NaN lowest, -0 as +0), the weights read once into shared memory; a radix select of three digits finds the key of the
-// last row that stays and how many rows of that very key do (the lowest rows first; digits of 11 bits, since weights
-// have few exponents and the counters of a shorter digit are hit by many threads at once); then each thread counts the
-// kept rows of its own stretch of keys, one scan over the block places them, and their indices and weights are written.
-// Stretches are of odd length, so that the threads' reads fall on different banks. Its time is a chain of a few dozen
-// shared-memory round trips and barriers. The second copies the kept K and V rows, one 16-byte vector per thread and
-// step, the source rows of a CTA's share looked up once, and is bound by their bytes.
+// order (NaN lowest, -0 as +0), which are put into shared memory; a radix select of three digits finds the key of the last
+// row that stays and how many rows of that very key do (the lowest rows first; digits of 11 bits, since weights have few
+// exponents and the counters of a shorter digit are hit by many threads at once); then each warp counts the kept rows
+// of its own stretch of keys, one scan over the warps places them, and their indices are written, 32 keys a step. Its
+// time is a chain of a few dozen shared-memory round trips and barriers. The second copies the kept rows' weights, K and
+// V, one 16-byte vector per thread and step, the source rows of a CTA's share looked up once, and is bound by their bytes.
 #include "common.cuh"
 #include "runtime.h"
 
@@ -53,13 +52,13 @@ __device__ __forceinline__ uint32_t order_key(float w) {
 }
 
 constexpr int kDigits = 2048;       // values of a digit
-constexpr int kSharedKeys = 49152;  // weights of a head that fit into shared memory beside the rest
+constexpr int kSharedKeys = 49152;  // keys of a head that fit into shared memory beside the rest
 
-// The kept rows of one head. The weights lie in shared memory, or, where the cache is too long for that, are read again
-// each time; their keys cost a few instructions.
+// The kept rows of one head. The keys lie in shared memory, or, where the cache is too long for that, are made again from
+// the weights each time.
 template <bool kShared>
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictParams p) {
-    extern __shared__ float s_weights[];
+    extern __shared__ uint4 s_fours[];  // the keys, and zeros (the lowest key) up to the next multiple of four
     __shared__ int histogram[kDigits];
     __shared__ int warp_sums[kSelectThreads / 32];
     __shared__ int warp_ties[kSelectThreads / 32];
@@ -72,63 +71,78 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
     const int64_t head = blockIdx.x;  // of all sequences
     const int64_t b = head / p.kv_heads;
     const int len = static_cast<int>(cached_rows(p, b));
-    const float* w = p.weights + head * p.capacity;
-    float* w_out = p.weights_out + head * p.out_capacity;
     int64_t* index = p.index + head * p.keep;
     const int keep = static_cast<int>(p.keep);
-    const int left = len < keep ? len : keep;
     if (head == b * p.kv_heads && tid == 0) {
-        p.lengths_out[b] = left;
-    }
-    for (int i = left + tid; i < p.out_capacity; i += kSelectThreads) {
-        w_out[i] = 0.0f;
+        p.lengths_out[b] = len < keep ? len : keep;
     }
     if (len <= keep) {
         for (int i = tid; i < keep; i += kSelectThreads) {
             index[i] = i < len ? i : -1;
-            if (i < len) {
-                w_out[i] = w[i];
-            }
         }
         return;
     }
     const int sinks = static_cast<int>(p.sinks);
     const int recent = static_cast<int>(p.recent);
     const int n = len - sinks - recent;  // rows [sinks, sinks + n) are ranked
-    const float* ranked = w + sinks;
-    if (kShared) {
-#pragma unroll 8
-        for (int i = tid; i < n; i += kSelectThreads) {
-            s_weights[i] = ranked[i];
-        }
-    }
-    const auto weight_of = [&](int i) { return kShared ? s_weights[i] : ranked[i]; };
-    const auto key_of = [&](int i) { return order_key(weight_of(i)); };
+    const int fours = (n + 3) / 4;
+    const float* ranked = p.weights + head * p.capacity + sinks;
+    uint32_t* s_keys = reinterpret_cast<uint32_t*>(s_fours);
     for (int i = tid; i < sinks; i += kSelectThreads) {
         index[i] = i;
-        w_out[i] = w[i];
     }
     for (int i = tid; i < recent; i += kSelectThreads) {
         index[keep - recent + i] = len - recent + i;
-        w_out[keep - recent + i] = w[len - recent + i];
     }
-    uint32_t prefix = 0;
-    uint32_t known = 0;
     int need = keep - sinks - recent;
     if (need == 0) {
         return;
     }
+    if (kShared) {
+        constexpr int kBatch = 16;  // loads in flight
+        for (int i0 = tid; i0 < fours * 4; i0 += kBatch * kSelectThreads) {
+            float x[kBatch];
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                const int i = i0 + j * kSelectThreads;
+                x[j] = i < n ? ranked[i] : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                const int i = i0 + j * kSelectThreads;
+                if (i < fours * 4) {
+                    s_keys[i] = i < n ? order_key(x[j]) : 0u;
+                }
+            }
+        }
+    }
+    const auto key_of = [&](int i) { return kShared ? s_keys[i] : order_key(ranked[i]); };
+    uint32_t prefix = 0;
+    uint32_t known = 0;
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
         const uint32_t digits = pass == 2 ? 1023u : 2047u;
         histogram[tid] = 0;
         histogram[tid + kSelectThreads] = 0;
         __syncthreads();
-#pragma unroll 4
-        for (int i = tid; i < n; i += kSelectThreads) {
-            const uint32_t key = key_of(i);
+        const auto count = [&](uint32_t key) {
             if ((key & known) == prefix) {
                 atomicAdd(&histogram[(key >> shift) & digits], 1);
+            }
+        };
+        if (kShared) {
+#pragma unroll 4
+            for (int i = tid; i < fours; i += kSelectThreads) {
+                const uint4 keys = s_fours[i];
+                count(keys.x);
+                count(keys.y);
+                count(keys.z);
+                count(keys.w);
+            }
+        } else {
+#pragma unroll 4
+            for (int i = tid; i < n; i += kSelectThreads) {
+                count(order_key(ranked[i]));
             }
         }
         __syncthreads();
@@ -156,43 +170,40 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
         need = s_need;
         known |= digits << shift;
     }
-    // Of the rows of key `prefix` the first `need` stay (none where no ranked row does), and all of higher keys.
-    const int stretch = ((n + kSelectThreads - 1) / kSelectThreads) | 1;
-    const int i0 = tid * stretch;
-    const int i1 = i0 + stretch < n ? i0 + stretch : n;
+    // Of the rows of key `prefix` the first `need` stay, and all of higher keys. A warp's stretch is whole steps of 32.
+    const int stretch = (n + kSelectThreads - 1) / kSelectThreads * 32;
+    const int begin = warp * stretch;
+    const int end = begin + stretch < n ? begin + stretch : n;
     int higher = 0;
     int ties = 0;
-    for (int i = i0; i < i1; ++i) {
+#pragma unroll 4
+    for (int i = begin + lane; i < end; i += 32) {
         const uint32_t key = key_of(i);
         higher += key > prefix ? 1 : 0;
         ties += key == prefix ? 1 : 0;
     }
-    int out = higher;  // becomes the number before the thread's stretch, as `equal` does of the ties
-    int equal = ties;
-    for (int offset = 1; offset < 32; offset <<= 1) {
-        const int a = __shfl_up_sync(0xffffffffu, out, offset);
-        const int b = __shfl_up_sync(0xffffffffu, equal, offset);
-        out += lane >= offset ? a : 0;
-        equal += lane >= offset ? b : 0;
-    }
-    if (lane == 31) {
-        warp_sums[warp] = out;
-        warp_ties[warp] = equal;
+    higher = __reduce_add_sync(0xffffffffu, higher);
+    ties = __reduce_add_sync(0xffffffffu, ties);
+    if (lane == 0) {
+        warp_sums[warp] = higher;
+        warp_ties[warp] = ties;
     }
     __syncthreads();
-    out += __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[lane] : 0) - higher;
-    equal += __reduce_add_sync(0xffffffffu, lane < warp ? warp_ties[lane] : 0) - ties;
-    out += sinks + (equal < need ? equal : need);
-    for (int i = i0; i < i1; ++i) {
-        const float weight = weight_of(i);
-        const uint32_t key = order_key(weight);
-        const bool tie = key == prefix;
-        if (key > prefix || (tie && equal < need)) {
-            index[out] = sinks + i;
-            w_out[out] = weight;
-            ++out;
+    higher = __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[lane] : 0);  // now of the keys before a step
+    ties = __reduce_add_sync(0xffffffffu, lane < warp ? warp_ties[lane] : 0);
+    const uint32_t lower_lanes = (1u << lane) - 1u;
+#pragma unroll 4
+    for (int i = begin; i < end; i += 32) {
+        const bool inside = i + lane < end;
+        const uint32_t key = inside ? key_of(i + lane) : 0u;
+        const uint32_t highers = __ballot_sync(0xffffffffu, inside && key > prefix);
+        const uint32_t equals = __ballot_sync(0xffffffffu, inside && key == prefix);
+        const int equal = ties + __popc(equals & lower_lanes);
+        if (inside && (key > prefix || (key == prefix && equal < need))) {
+            index[sinks + higher + __popc(highers & lower_lanes) + (equal < need ? equal : need)] = sinks + i + lane;
         }
-        equal += tie ? 1 : 0;
+        higher += __popc(highers);
+        ties += __popc(equals);
     }
 }
 
@@ -210,7 +221,11 @@ __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const EvictPar
     const int left = static_cast<int>(len < p.keep ? len : p.keep);
     if (threadIdx.x < kCopyRows) {
         const int row = row0 + static_cast<int>(threadIdx.x);
-        s_from[threadIdx.x] = row < left ? static_cast<int>(p.index[head * p.keep + row]) : -1;
+        const int64_t from = row < left ? p.index[head * p.keep + row] : -1;
+        s_from[threadIdx.x] = static_cast<int>(from);
+        if (row < p.out_capacity) {
+            p.weights_out[head * p.out_capacity + row] = from >= 0 ? p.weights[head * p.capacity + from] : 0.0f;
+        }
     }
     __syncthreads();
     const int rows = p.out_capacity - row0 < kCopyRows ? static_cast<int>(p.out_capacity - row0) : kCopyRows;
@@ -303,7 +318,7 @@ int cppinf_cache_evict(cppinf_dtype dtype, const void* k_cache, const int64_t* k
     const unsigned heads = static_cast<unsigned>(batch * kv_heads);
     cudaError_t err = cudaSuccess;
     if (capacity <= kSharedKeys) {
-        const std::size_t bytes = static_cast<std::size_t>(capacity) * sizeof(uint32_t);
+        const std::size_t bytes = static_cast<std::size_t>(rt::ceil_div(capacity, 4)) * sizeof(uint4);
         static rt::SharedMemoryLimit limit;
         CPPINF_CUDA_TRY(limit.raise(evict_select_kernel<true>, kSharedKeys * sizeof(uint32_t)));
         err = rt::launch_smem(evict_select_kernel<true>, dim3(heads), dim3(kSelectThreads), bytes, s, 1u, p);
