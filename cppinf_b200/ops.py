@@ -479,11 +479,13 @@ def _row_counts(t: torch.Tensor | None, batch: int, op: str, name: str) -> torch
     return t.contiguous()
 
 
-def _cache_strides(t: torch.Tensor) -> tuple[int, int, int] | None:
-    """Element strides {batch, row, head} of a cache that the kernels can read and write in place, else None. The
-    stride of a dimension of one entry is never followed and is given as if the tensor were dense."""
-    b, n, h, d = t.shape
-    sb, sn, sh, sd = t.stride()
+_Strides = ctypes.c_int64 * 3
+
+
+@functools.lru_cache(maxsize=256)
+def _layout(shape: tuple, strides: tuple, element_size: int) -> tuple[tuple[int, int, int], ctypes.Array] | None:
+    b, n, h, d = shape
+    sb, sn, sh, sd = strides
     if sd != 1 and d != 1:
         return None
     if h <= 1:
@@ -492,10 +494,20 @@ def _cache_strides(t: torch.Tensor) -> tuple[int, int, int] | None:
         sn = max(h, 1) * sh
     if b <= 1:
         sb = max(n, 1) * sn
-    vec = 16 // t.element_size()
-    if sh < d or sb < d or sn < d or (sb | sn | sh) % vec or t.data_ptr() % 16:
+    if sh < d or sb < d or sn < d or (sb | sn | sh) % (16 // element_size):
         return None
-    return sb, sn, sh
+    return (sb, sn, sh), _Strides(sb, sn, sh)
+
+
+def _cache_layout(t: torch.Tensor) -> tuple[tuple[int, int, int], ctypes.Array] | None:
+    return None if t.data_ptr() % 16 else _layout(t.shape, t.stride(), t.element_size())
+
+
+def _cache_strides(t: torch.Tensor) -> tuple[int, int, int] | None:
+    """Element strides {batch, row, head} of a cache that the kernels can read and write in place, else None. The
+    stride of a dimension of one entry is never followed and is given as if the tensor were dense."""
+    layout = _cache_layout(t)
+    return None if layout is None else layout[0]
 
 
 def _validate_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, op: str) -> None:
@@ -505,15 +517,12 @@ def _validate_caches(k_cache: torch.Tensor, v_cache: torch.Tensor, op: str) -> N
         raise ValueError(f"{op} requires matching tensor dtypes.")
 
 
-_Strides = ctypes.c_int64 * 3
-
-
 def _readable_cache(t: torch.Tensor) -> tuple[torch.Tensor, ctypes.Array]:
-    strides = _cache_strides(t)
-    if strides is None:
-        t = materialize(t) if not t.is_contiguous() else t.clone()
-        strides = t.stride()[:3]
-    return t, _Strides(*strides)
+    layout = _cache_layout(t)
+    if layout is not None:
+        return t, layout[1]
+    t = materialize(t) if not t.is_contiguous() else t.clone()
+    return t, _Strides(*t.stride()[:3])
 
 
 def _cache_attention(op: str, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
@@ -541,7 +550,7 @@ def _address(t: torch.Tensor | None) -> int | None:
 
 def _elsewhere(device: int) -> torch.cuda.device | None:
     """What makes the tensors' device the current one, where another is."""
-    return None if torch.cuda.current_device() == device else torch.cuda.device(device)
+    return None if torch._C._cuda_getDevice() == device else torch.cuda.device(device)
 
 
 def _stream_of(device: int) -> int:
@@ -568,8 +577,9 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     as nodes[b] (int64 [B]) reaches. Returns the bf16 context [B, T, Hq, D], zeros where a node is padding or sees
     nothing. `error` (int32 [1]) is set when a wait of the kernel ran out of its poll limit."""
     op = "tree_attention"
-    if mask.dtype != torch.bool or q.dim() != 4 or mask.dim() not in (2, 3) or \
-            mask.shape[-2:] != (q.shape[1], q.shape[1]) or (mask.dim() == 3 and mask.shape[0] != q.shape[0]):
+    shape = q.shape
+    square = (shape[1], shape[1]) if len(shape) == 4 else None
+    if mask.dtype != torch.bool or square is None or (mask.shape != square and mask.shape != (shape[0], *square)):
         raise ValueError("tree_attention requires a bool mask of [tokens, tokens], shared or one per sequence.")
     device, lengths, nodes = _cache_attention(op, q, k_cache, v_cache, lengths, nodes, mask, error)
     if (other := _elsewhere(device)) is not None:
@@ -626,14 +636,14 @@ def tree_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Ten
     device = _same_device(op, k_cache, v_cache, lengths, path, counts)
     lengths = _row_counts(lengths, batch, op, "lengths")
     counts = _row_counts(counts, batch, op, "counts")
-    ks, vs = _cache_strides(k_cache), _cache_strides(v_cache)
-    if ks is None or vs is None:
+    k_layout, v_layout = _cache_layout(k_cache), _cache_layout(v_cache)
+    if k_layout is None or v_layout is None:
         raise ValueError("tree_commit requires caches with dense 16-byte aligned rows.")
     if (other := _elsewhere(device)) is not None:
         with other:
             return tree_commit(k_cache, v_cache, lengths, path, counts)
     path = path.contiguous()
-    capi.call("cppinf_tree_commit", code, k_cache.data_ptr(), _Strides(*ks), v_cache.data_ptr(), _Strides(*vs),
+    capi.call("cppinf_tree_commit", code, k_cache.data_ptr(), k_layout[1], v_cache.data_ptr(), v_layout[1],
               lengths.data_ptr(), path.data_ptr(), counts.data_ptr(), batch, path.shape[1], heads, d, capacity,
               _stream_of(device))
 
