@@ -754,3 +754,24 @@ def test_commit_of_an_empty_cache(ops):
     k = torch.zeros(1, 0, 2, 64, dtype=torch.bfloat16, device="cuda")
     n = torch.zeros(1, dtype=torch.int64, device="cuda")
     ops.tree_commit(k, k.clone(), n, torch.zeros(1, 4, dtype=torch.int64, device="cuda"), n)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("tokens,group", [(10, 3), (150, 3), (150, 2), (90, 5)])
+def test_weights_of_a_row_whose_scores_are_minus_infinity(ops, tokens, group, d):
+    """Such a row counts for nothing, as does one of a very low score, in every query tile, those with unused rows too."""
+    g = torch.Generator(device="cuda").manual_seed(tokens + d)
+    q = torch.randn((1, tokens, 2 * group, d), generator=g, device="cuda").bfloat16()
+    q[..., 0] = 1.0
+    k, v = caches(g, 1, 300 + tokens, 2, d, "dense")
+    n = torch.tensor([300], device="cuda")
+    results = []
+    for low in (-1e30, -math.inf):
+        k[0, 20, :, 0] = low
+        k[0, 300 + tokens // 2, :, 0] = low
+        w = torch.ones((1, 2, 300 + tokens), device="cuda")
+        results.append((ops.decoder_attention_weights(q, k, v, n, w), w))
+    assert torch.isfinite(results[0][0]).all()
+    assert torch.equal(results[0][0], results[1][0])
+    assert torch.equal(results[0][1], results[1][1])
+    assert (results[1][1][0, :, 20] == 1).all()
