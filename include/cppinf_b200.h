@@ -341,8 +341,8 @@ CPPINF_API int cppinf_decoder_attention_weights(const void* q, const void* k_cac
 /* Cuts each sequence of a cache to `keep` rows, per key-value head: the first `sinks` rows, the last `recent` and, of
  * the others, those of the highest weight (f32 dense [batch, kv_heads, capacity]; equal weights: the lowest rows; NaN
  * below every number) stay, in their order; a sequence of no more than `keep` rows stays whole. Kept rows go to k_out
- * and v_out (dense [batch, out_capacity, kv_heads, head_dim], out_capacity >= keep, not overlapping the cache), their
- * weights to weights_out (f32 [batch, kv_heads, out_capacity]); what follows the kept rows is zeros. lengths_out
+ * and v_out (dense [batch, out_capacity, kv_heads, head_dim], out_capacity >= keep), their weights to weights_out (f32
+ * [batch, kv_heads, out_capacity]); what follows the kept rows is zeros. No output overlaps an input. lengths_out
  * [batch] = min(lengths, keep); index (int64 [batch, kv_heads, keep]) the kept rows, then -1. Keys carry their rotary
  * position with them, so later queries keep their own positions. Needs keep >= 1, sinks + recent <= keep. */
 CPPINF_API int cppinf_cache_evict(cppinf_dtype dtype, const void* k_cache, const int64_t* k_strides,
