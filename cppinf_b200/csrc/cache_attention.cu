@@ -1468,8 +1468,11 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
                 wait(bar_s + buffer, n / L::kBuffers & 1u);
                 tc_fence_after();
                 const bool partial = inside < p.tile_tokens || columns < chunks * 32 || at.kt * 128 + 127 - r.len > token0;
-                const int low = (key - r.len - token0) * p.group;  // columns below do not see the key
-                const int high = inside * p.group;                 // columns from here on count for nothing
+                // A committed key lies up to 2^30 rows before the tile's first query: only a later one is multiplied, by
+                // less than two tiles of tokens.
+                const int later = key - r.len - token0;
+                const int low = later > 0 ? later * p.group : 0;  // columns below do not see the key
+                const int high = inside * p.group;                // columns from here on count for nothing
 #pragma unroll 1
                 for (int c = 0; c < chunks; ++c) {
                     float x[32];

@@ -775,3 +775,43 @@ def test_weights_of_a_row_whose_scores_are_minus_infinity(ops, tokens, group, d)
     assert torch.equal(results[0][0], results[1][0])
     assert torch.equal(results[0][1], results[1][1])
     assert (results[1][1][0, :, 20] == 1).all()
+
+
+def check_weights_of_a_long_cache(ops, rows, group, tokens):
+    """Weights of one key-value head over `rows` committed rows (K and V are one tensor) against the formula in 64 bits, a
+    piece of the rows at a time. Besides the file's bounds, l is a long sum: a CTA adds two halves of each of its key
+    tiles to it, 32 terms in a half's partial sums, and the parts of all CTAs are joined, with at least 100 CTAs at work and
+    at most 160."""
+    g = torch.Generator(device="cuda").manual_seed(19)
+    d = 64
+    cache = torch.empty((1, rows + tokens, 1, d), dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    q = torch.randn((1, tokens, group, d), generator=g, device="cuda").bfloat16()
+    w = torch.zeros((1, 1, rows + tokens), device="cuda")
+    ops.decoder_attention_weights(q, cache, cache, torch.tensor([rows], device="cuda"), w)
+    qq = q[0].double().reshape(tokens * group, d)
+    see = rows + torch.arange(tokens, device="cuda").repeat_interleave(group)  # each row's last key
+
+    def pieces():
+        for i in range(0, rows + tokens, 1 << 18):
+            keys = cache[0, i:i + (1 << 18), 0].double()
+            at = torch.arange(i, i + len(keys), device="cuda")
+            s = (qq @ keys.T / math.sqrt(d)).masked_fill_(at > see[:, None], -math.inf)
+            yield i, s, float((qq.abs() @ keys.abs().T).max()) / math.sqrt(d)
+
+    top = torch.full((tokens * group, 1), -math.inf, dtype=torch.float64, device="cuda")
+    size = 0.0
+    for _, s, largest in pieces():
+        top, size = torch.maximum(top, s.amax(1, keepdim=True)), max(size, largest)
+    total = sum(torch.exp(s - top).sum(1, keepdim=True) for _, s, _ in pieces())
+    adds = 2 * math.ceil((rows + tokens) / 128 / 100) + 32 + 160
+    rel = 4.5 * 2 * (d + 3) * U * size + 2.0 ** -18 + adds * U
+    for i, s, _ in pieces():
+        want = (torch.exp(s - top) / total).sum(0)
+        off = (w[0, 0, i:i + len(want)].double() - want).abs()
+        assert (off <= want * (rel + (tokens * group + 2) * U)).all(), f"rows from {i} on"
+
+
+def test_weights_of_rows_far_before_the_queries(ops):
+    """Committed rows times query heads pass 2^31, and the query tile has columns that no query fills."""
+    check_weights_of_a_long_cache(ops, (1 << 31) // 120 + 5000, 120, 1)
+    torch.cuda.empty_cache()
