@@ -28,8 +28,8 @@
 //
 // Rows past a sequence's end and drafted rows that only some queries see may hold anything: scores there are replaced
 // before the softmax, and V tiles in which some row is hidden from some query are cleared of such values in shared
-// memory before the product (0 * NaN would be NaN); values that are not finite in a row that a query does see are added
-// to its O afterwards.
+// memory before the product (0 * NaN would be NaN); a value that is not finite in a row that a query does see is added
+// to its O afterwards, times its probability, so that it counts as in a tile that all queries see.
 #include <cmath>
 
 #include "common.cuh"
@@ -898,31 +898,43 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 for (int i = 0; i < 16; ++i) {
                     flagged |= s_flags[w * 16 + i] | (kPair && chains == 2 ? s_flags[(1 - w) * 16 + i] : 0u);
                 }
-                if (flagged != 0u && busy) {  // values that are not finite, added to the O of the rows that see them
+                if (flagged != 0u && busy) {
+                    // Values that are not finite, added to the O of the rows that see them by what the product makes of
+                    // them, infinity or NaN, with their probability formed again: NaN where it is 0.
+                    const float shift = top == -INFINITY ? 0.0f : top * c2;
+                    const bf16* q = p.q + ((at.b * p.tokens + t) * p.q_heads + at.h * p.group + g) * D;
+                    for (int i = 0; i < 16; ++i) {
+                        uint32_t word = s_flags[w * 16 + i] | (kPair && chains == 2 ? s_flags[(1 - w) * 16 + i] : 0u);
+                        while (word != 0u) {
+                            const int key = part0 + i * 32 + __ffs(word) - 1;
+                            word &= word - 1u;
+                            const bool seen = valid && (visible_bits(bits_row, key, r.len, limit) & 1u) != 0u;
+                            const bf16* k = p.k + at.b * p.ks[0] + key * p.ks[1] + at.h * p.ks[2];
+                            const bf16* v = p.v + at.b * p.vs[0] + key * p.vs[1] + at.h * p.vs[2];
+                            float s = 0.0f;
 #pragma unroll 1
-                    for (int c = 0; c < D / 16; ++c) {
-                        uint32_t o[16];
-                        tmem_load16(t_o + c * 16, o);
-                        for (int i = 0; i < 16; ++i) {
-                            uint32_t word = s_flags[w * 16 + i] | (kPair && chains == 2 ? s_flags[(1 - w) * 16 + i] : 0u);
-                            while (word != 0u) {
-                                const int key = part0 + i * 32 + __ffs(word) - 1;
-                                word &= word - 1u;
-                                const bool seen = valid && (visible_bits(bits_row, key, r.len, limit) & 1u) != 0u;
-                                const bf16* v = p.v + at.b * p.vs[0] + key * p.vs[1] + at.h * p.vs[2] + c * 16;
+                            for (int c = 0; seen && c < D; ++c) {
+                                s = __fmaf_rn(__bfloat162float(q[c]), __bfloat162float(k[c]), s);
+                            }
+                            const float weight = exp2_approx(__fmaf_rn(s, c2, -shift));
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 16) {
+                                uint32_t o[16];
+                                __syncwarp();
+                                tmem_load16(t_o + c, o);
 #pragma unroll
                                 for (int j = 0; j < 16; ++j) {
-                                    const float x = __bfloat162float(v[j]);
+                                    const float x = __bfloat162float(v[c + j]);
                                     if (seen && !(fabsf(x) < INFINITY)) {
-                                        o[j] = __float_as_uint(__uint_as_float(o[j]) + x);
+                                        o[j] = __float_as_uint(__fmaf_rn(x, weight, __uint_as_float(o[j])));
                                     }
                                 }
+                                __syncwarp();
+                                tmem_store16(t_o + c, o);
                             }
+                            tmem_store_wait();
                         }
-                        __syncwarp();
-                        tmem_store16(t_o + c * 16, o);
                     }
-                    tmem_store_wait();
                 }
             }
             float scaled_top = top == -INFINITY ? -INFINITY : top * c2;

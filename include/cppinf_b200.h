@@ -279,7 +279,8 @@ CPPINF_API int cppinf_decoder_attention_tc(const void* q, const void* k_cache, c
  * follows them from replay to replay; they cannot be refused there, so a length is taken as 0 below 0 and as the
  * capacity above it, and a new token whose row would lie past the capacity counts as padding. Query head h reads
  * key-value head h / (q_heads / kv_heads); up to 128 query heads share one. Rows of a cache that no query sees may hold
- * anything, NaN and infinities included.
+ * anything, NaN and infinities included; in a row that a query does see, a value that is not finite makes its context NaN
+ * or infinite, as the product with the row's f32 probability does (NaN where that is 0).
  * ------------------------------------------------------------------------------------------------------------- */
 
 /* Device scratch, in bytes, that cppinf_tree_attention (with_weights 0) or cppinf_decoder_attention_weights (1) needs

@@ -815,3 +815,35 @@ def test_weights_of_rows_far_before_the_queries(ops):
     """Committed rows times query heads pass 2^31, and the query tile has columns that no query fills."""
     check_weights_of_a_long_cache(ops, (1 << 31) // 120 + 5000, 120, 1)
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("tokens", [6, 140])
+@pytest.mark.parametrize("committed", [250, 3050])
+@pytest.mark.parametrize("row", ["early", "last committed", "drafted"])
+def test_an_infinite_value_of_no_probability(ops, row, committed, tokens, d):
+    """Its product with the probability 0 is NaN wherever the row lies: in a tile of committed rows alone, in the tile where
+    the drafted rows begin, among those. Scores of -6000 and less leave a probability of 0 in 64 bits too."""
+    g = torch.Generator(device="cuda").manual_seed(20)
+    q = torch.randn((1, tokens, 4, d), generator=g, device="cuda").bfloat16()
+    q[..., 0] = 1.0
+    k, v = caches(g, 1, committed + tokens + 60, 2, d, "dense")
+    n = torch.tensor([committed], device="cuda")
+    mask = torch.ones((tokens, tokens), dtype=torch.bool, device="cuda").tril()
+    first = 3 if row == "drafted" else 0  # the first node that sees the row
+    at = {"early": 10, "last committed": committed - 1, "drafted": committed + 3}[row]
+    k[0, at, :, 0] = -1e5
+    want = ops.tree_attention(q, k, v, n, mask)
+    assert torch.isfinite(want).all()
+    v[0, at, 1, 5] = math.inf
+    want[0, first:, 2:, 5] = math.nan
+    got = ops.tree_attention(q, k, v, n, mask)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+    w = torch.zeros((1, 2, k.shape[1]), device="cuda")
+    v[0, at, 1, 5] = 0.0
+    want = ops.decoder_attention_weights(q, k, v, n, w)
+    v[0, at, 1, 5] = math.inf
+    want[0, first:, 2:, 5] = math.nan
+    got = ops.decoder_attention_weights(q, k, v, n, w.zero_())
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+    assert torch.isfinite(w).all() and w[0, 0, at] == 0
