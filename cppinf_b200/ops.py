@@ -525,6 +525,12 @@ def _readable_cache(t: torch.Tensor) -> tuple[torch.Tensor, ctypes.Array]:
     return t, _Strides(*t.stride()[:3])
 
 
+def _readable_queries(q: torch.Tensor) -> torch.Tensor:
+    """Dense queries on the 16-byte grid: q itself, or a copy."""
+    q = materialize(q)
+    return q.clone() if q.data_ptr() % 16 else q
+
+
 def _cache_attention(op: str, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
                      counts: torch.Tensor | None, extra: torch.Tensor, error: torch.Tensor | None):
     """Checks that tree_attention and decoder_attention_weights share; returns what their calls need."""
@@ -587,7 +593,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
             return tree_attention(q, k_cache, v_cache, lengths, mask, nodes, error)
     batch, tokens, q_heads, d = q.shape
     _, capacity, kv_heads, _ = k_cache.shape
-    q, mask = materialize(q), mask.contiguous()
+    q, mask = _readable_queries(q), mask.contiguous()
     k, ks = _readable_cache(k_cache)
     v, vs = _readable_cache(v_cache)
     ctx = torch.empty_like(q)
@@ -665,7 +671,7 @@ def decoder_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     if (other := _elsewhere(device)) is not None:
         with other:
             return decoder_attention_weights(q, k_cache, v_cache, lengths, weights, counts, error)
-    q = materialize(q)
+    q = _readable_queries(q)
     k, ks = _readable_cache(k_cache)
     v, vs = _readable_cache(v_cache)
     ctx = torch.empty_like(q)

@@ -847,3 +847,18 @@ def test_an_infinite_value_of_no_probability(ops, row, committed, tokens, d):
     got = ops.decoder_attention_weights(q, k, v, n, w.zero_())
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
     assert torch.isfinite(w).all() and w[0, 0, at] == 0
+
+
+def test_queries_off_the_16_byte_grid(ops):
+    """Dense queries at any address give what a copy of them gives, as caches do."""
+    g = torch.Generator(device="cuda").manual_seed(21)
+    q = torch.randn((2 * 3 * 4 * 64 + 1,), generator=g, device="cuda").bfloat16()[1:].view(2, 3, 4, 64)
+    assert q.is_contiguous() and q.data_ptr() % 16 == 2
+    k, v = caches(g, 2, 100, 2, 64, "dense")
+    n = torch.tensor([90, 13], device="cuda")
+    mask = torch.ones((3, 3), dtype=torch.bool, device="cuda").tril()
+    w, w2 = torch.zeros((2, 2, 2, 100), device="cuda")
+    assert torch.equal(ops.tree_attention(q, k, v, n, mask), ops.tree_attention(q.clone(), k, v, n, mask))
+    assert torch.equal(ops.decoder_attention_weights(q, k, v, n, w),
+                       ops.decoder_attention_weights(q.clone(), k, v, n, w2))
+    assert torch.equal(w, w2)
