@@ -44,6 +44,7 @@ using namespace tc;
 constexpr int kMaxNodes = 256;  // drafted tokens of a sequence
 constexpr int kMaxGroup = 128;  // query heads of a key-value head
 constexpr int kMaxKeptRows = 32;  // rows of a head whose scores are kept for the weights
+constexpr int64_t kMostScoreBytes = int64_t{1} << 30;  // of kept scores, unless they are few beside K and V
 
 // Where a CTA's part of the line begins, for the kernel that joins the parts.
 struct __align__(16) Cut {
@@ -1669,11 +1670,17 @@ Plan plan(int64_t batch, int64_t tokens, int64_t q_heads, int64_t kv_heads, int6
         // Keeping a key's scores for the weights moves 8 bytes for each row, mostly within L2; forming them again reads
         // the key's 2 * head_dim bytes of K from memory and takes a tile's products. Eight sequences of 16000 rows, 8
         // heads of 128: 106 against 162 us with 2 rows, 125 against 163 with 16, 149 against 164 with 32, 223 against
-        // 166 with 64.
-        if (tokens * group <= kMaxKeptRows) {
-            pl.score_stride = runtime::ceil_div(capacity, 128) * 128;
+        // 166 with 64. Scores go by the capacity, not by the lengths: past kMostScoreBytes they are kept only where they
+        // take a sixteenth of K and V at most, so that the call needs little memory beside its caches. 32 sequences of 8
+        // heads of 128: 1054 us kept and 1063 us formed again with 32 rows (33000 cached, 1.01 GB of scores), 1685 and 2103
+        // with 16 (65500, 1.00 GB), 1546 and 2101 with 8, which stay kept.
+        const int64_t stride = runtime::ceil_div(capacity, 128) * 128;
+        const int64_t score_bytes = batch * kv_heads * pl.part_rows * stride * static_cast<int64_t>(sizeof(float));
+        const bool few = score_bytes <= kMostScoreBytes || tokens * group * 16 <= head_dim;
+        if (tokens * group <= kMaxKeptRows && few) {
+            pl.score_stride = stride;
             pl.scores = pl.sums;
-            pl.bytes = pl.scores + batch * kv_heads * pl.part_rows * pl.score_stride * static_cast<int64_t>(sizeof(float));
+            pl.bytes = pl.scores + score_bytes;
             return pl;
         }
         pl.weight_ctas = static_cast<int>(products < runtime::sm_count() ? products : runtime::sm_count());

@@ -285,7 +285,9 @@ CPPINF_API int cppinf_decoder_attention_tc(const void* q, const void* k_cache, c
 
 /* Device scratch, in bytes, that cppinf_tree_attention (with_weights 0) or cppinf_decoder_attention_weights (1) needs
  * for these sizes on the current device; 16-byte aligned, contents arbitrary, not shared by calls that overlap in time.
- * A negative number: sizes that the entry points refuse. */
+ * Some tens of MB for the sums of split sequences and, with weights, 4 bytes for each query and query head and, where a
+ * key-value head has up to 32 of those, 4 more for each of them and each cached row of the capacity, as long as that stays
+ * below 1 GiB or a sixteenth of K and V. A negative number: sizes that the entry points refuse. */
 CPPINF_API int64_t cppinf_cache_attention_scratch_bytes(int64_t batch, int64_t tokens, int64_t q_heads,
                                                         int64_t kv_heads, int64_t head_dim, int64_t capacity,
                                                         int with_weights);

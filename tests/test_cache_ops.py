@@ -227,3 +227,16 @@ def test_attention_sizes_that_pass_the_index_range(lib):
     assert lib.cppinf_cache_attention_scratch_bytes(1, 1 << 61, *args, 1) == -1
     # 2^16 * 2^13 heads of one tile each: 2^29 tiles, and with an item's set-up before each 2^31 pieces.
     assert lib.cppinf_cache_attention_scratch_bytes(1 << 16, 1, 1 << 13, 1 << 13, 64, 16, 0) == -1
+
+
+def test_scratch_of_long_caches_is_bounded(lib):
+    """Kept scores, 4 bytes a row of a head and a cached row, take 1 GiB or a sixteenth of K and V at most; beside them lie
+    the parts of 148 CTAs (2 * 148 * 32 rows of 128) and the rows' statistics, below 2^26 bytes together."""
+    def scratch(tokens):  # 32 sequences of 131072 rows, 16 over 8 heads of 128: K and V take 16 GiB
+        return lib.cppinf_cache_attention_scratch_bytes(32, tokens, 16, 8, 128, 131072, 1)
+
+    assert scratch(16) < (1 << 30) + (1 << 26)  # 4 GiB of scores
+    assert scratch(8) < (1 << 30) + (1 << 26)   # 2 GiB
+    assert scratch(4) <= (1 << 30) + (1 << 26)  # 1 GiB
+    assert 1 << 28 <= scratch(1) < (1 << 28) + (1 << 26)
+    assert lib.cppinf_cache_attention_scratch_bytes(64, 4, 16, 8, 128, 131072, 1) < (1 << 31) + (1 << 26)

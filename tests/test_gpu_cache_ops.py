@@ -862,3 +862,11 @@ def test_queries_off_the_16_byte_grid(ops):
     assert torch.equal(ops.decoder_attention_weights(q, k, v, n, w),
                        ops.decoder_attention_weights(q.clone(), k, v, n, w2))
     assert torch.equal(w, w2)
+
+
+@pytest.mark.parametrize("group,tokens", [(1, 2), (16, 2)])
+def test_weights_of_a_cache_whose_scores_are_too_many_to_keep(ops, group, tokens):
+    """8.5 million rows of a head of 64: 68 MB of scores with two rows a head, which are kept, and more than 1 GiB with 32,
+    which are not."""
+    check_weights_of_a_long_cache(ops, 8_500_000, group, tokens)
+    torch.cuda.empty_cache()
