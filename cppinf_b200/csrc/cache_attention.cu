@@ -239,11 +239,14 @@ struct Cuts {
 };
 
 // Bounded waits: one that runs out of the poll limit sets the error word and waits again with the default limit; if
-// that runs out too, `stop` ends all later waits of the CTA at once, so that it always comes to its end.
+// that runs out too, `stop` ends all later waits of the CTA at once, so that it always comes to its end. Its loads end
+// then, and it waits for the copies and products in flight, again with the limit, before it frees its tensor memory.
 struct Waiter {
     unsigned int* error;
     uint32_t limit;
     volatile uint32_t* stop;
+
+    __device__ __forceinline__ bool stopped() const { return *stop != 0u; }
 
     __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t phase) const {
         if (limit == 0u || !mbar_try_wait(bar, phase)) {
@@ -252,7 +255,7 @@ struct Waiter {
     }
 
     __device__ __forceinline__ void slow(uint64_t* bar, uint32_t phase) const {
-        if (*stop != 0u || mbar_wait_bounded(bar, phase, limit)) {
+        if (stopped() || mbar_wait_bounded(bar, phase, limit)) {
             return;
         }
         if (error != nullptr) {
@@ -263,6 +266,19 @@ struct Waiter {
         }
     }
 };
+
+// Waits until the last of a slot's fills has landed; an odd number of them leaves its bit set in `filled`.
+__device__ __forceinline__ void wait_landed(uint64_t* full, uint32_t filled, int slots) {
+    for (int i = 0; i < slots; ++i) {
+        mbar_wait_bounded(full + i, (filled >> i & 1u) ^ 1u);
+    }
+}
+
+// Waits for the matrix products that this thread has issued.
+__device__ __forceinline__ void wait_products(uint64_t* bar) {
+    umma_commit(bar);
+    mbar_wait_bounded(bar, 0u);
+}
 
 // Visible keys [key, key + 32) of a row as a bit mask. Tree: committed keys, then the row's mask bits (9 words, the last
 // empty); causal: keys below `limit`.
@@ -393,6 +409,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
     uint64_t* bar_s = bar_q_empty + 1;            // [chains][2] S is complete
     uint64_t* bar_pv = bar_s + 2 * kStreams;      // [chains][2] the product of its P with V is complete
     uint64_t* bar_p = bar_pv + 2 * kStreams;      // [chains][2][2] half of P is written
+    uint64_t* bar_end = bar_p + 4 * kStreams;     // products in flight at the end of a CTA that gave up
     __shared__ uint32_t s_tmem;
     __shared__ uint32_t s_stop;
     __shared__ Walk s_walk;
@@ -417,6 +434,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
             mbar_init(bar_pv + 2 * w, 1);
             mbar_init(bar_pv + 2 * w + 1, 1);
         }
+        mbar_init(bar_end, 1);
     }
     if (warp == 2) {
         tmem_alloc(&s_tmem, kTmemAll);
@@ -550,6 +568,7 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
         ++at.index;
         advance(p, at, tiles);
     };
+    uint32_t filled = 0;  // a bit for each slot of the ring, then Q: whether it was filled an odd number of times
     if (warp < 4) {
         if (warp == 0) {  // ---- loads
             uint32_t k_tiles[L::kRings] = {};  // loaded so far
@@ -558,7 +577,8 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 if (n >= static_cast<uint32_t>(L::kDepth)) {
                     wait(bar_empty + slot, L::parity(n) ^ 1u);
                 }
-                if (elect_one()) {
+                if (elect_one() && !wait.stopped()) {
+                    filled ^= 1u << slot;
                     mbar_arrive_expect_tx(bar_full + slot, L::kSlot);
                     unsigned char* dst = sm + L::kRing + slot * L::kSlot;
 #pragma unroll
@@ -589,7 +609,8 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
                 }
                 const int q_tiles = kPair ? chains : 1;
                 const uint32_t box = static_cast<uint32_t>(p.q_box_tokens * p.group) * 128u;
-                if (elect_one()) {
+                if (elect_one() && !wait.stopped()) {
+                    filled ^= 1u << L::kSlots;
                     mbar_arrive_expect_tx(bar_q_full, box * L::kAtoms * q_tiles);
                     for (int i = 0; i < q_tiles; ++i) {
 #pragma unroll
@@ -1015,6 +1036,15 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
     tc_fence_before();
     __syncwarp();
     __syncthreads();
+    if (s_stop != 0u) {
+        if (warp == 0 && elect_one()) {
+            wait_landed(bar_full, filled, L::kSlots);
+            wait_landed(bar_q_full, filled >> L::kSlots, 1);
+        } else if (warp == 1 && elect_one()) {
+            wait_products(bar_end);
+        }
+        __syncthreads();
+    }
     if (warp == 2) {
         tc_fence_after();
         tmem_dealloc(tmem, kTmemAll);
@@ -1221,6 +1251,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
     uint64_t* bar_k_empty = bar_k_full + L::kKeySlots;
     uint64_t* bar_s = bar_k_empty + L::kKeySlots;  // [buffers] a product is complete
     uint64_t* bar_free = bar_s + L::kBuffers;      // [buffers] and read
+    uint64_t* bar_end = bar_free + L::kBuffers;    // products in flight at the end of a CTA that gave up
     __shared__ uint32_t s_tmem;
     __shared__ uint32_t s_stop;
     __shared__ uint32_t s_last[L::kGroups];
@@ -1245,6 +1276,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
             mbar_init(bar_s + i, 1);
             mbar_init(bar_free + i, 4);
         }
+        mbar_init(bar_end, 1);
     }
     if (warp == 2) {
         tmem_alloc(&s_tmem, kTmemAll);
@@ -1373,6 +1405,7 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
         advance_unit();
     };
 
+    uint32_t filled = 0;  // a bit for each slot of the ring, then of K: whether it was filled an odd number of times
     if (warp == 0) {
         {  // ---- loads
             for (; segment(); next()) {
@@ -1381,7 +1414,8 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
                 if (kr > 0) {
                     wait(bar_k_empty + ks, (kr - 1) & 1u);
                 }
-                if (elect_one()) {
+                if (elect_one() && !wait.stopped()) {
+                    filled ^= 1u << (L::kSlots + ks);
                     mbar_arrive_expect_tx(bar_k_full + ks, L::kTile);
 #pragma unroll
                     for (int a = 0; a < L::kAtoms; ++a) {
@@ -1396,7 +1430,8 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
                     if (fill >= static_cast<uint32_t>(L::kSlots)) {
                         wait(bar_empty + slot, (fill / L::kSlots - 1) & 1u);
                     }
-                    if (elect_one()) {
+                    if (elect_one() && !wait.stopped()) {
+                        filled ^= 1u << slot;
                         mbar_arrive_expect_tx(bar_full + slot, static_cast<uint32_t>(columns) * 128u * L::kAtoms);
 #pragma unroll
                         for (int a = 0; a < L::kAtoms; ++a) {
@@ -1567,6 +1602,15 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
     tc_fence_before();
     __syncwarp();
     __syncthreads();
+    if (s_stop != 0u) {
+        if (warp == 0 && elect_one()) {
+            wait_landed(bar_full, filled, L::kSlots);
+            wait_landed(bar_k_full, filled >> L::kSlots, L::kKeySlots);
+        } else if (warp == 1 && elect_one()) {
+            wait_products(bar_end);
+        }
+        __syncthreads();
+    }
     if (warp == 2) {
         tc_fence_after();
         tmem_dealloc(tmem, kTmemAll);
