@@ -870,3 +870,56 @@ def test_weights_of_a_cache_whose_scores_are_too_many_to_keep(ops, group, tokens
     which are not."""
     check_weights_of_a_long_cache(ops, 8_500_000, group, tokens)
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("tokens", [5, 150])
+def test_weights_of_calls_on_two_streams(ops, tokens):
+    """Twenty calls on each of two streams at once add the bits that they add one after the other: from kept scores, and in
+    units that are cut between CTAs."""
+    g = torch.Generator(device="cuda").manual_seed(22)
+    sets = []
+    for i in range(2):
+        k, v = caches(g, 3, 3000, 4, 128, "dense")
+        q = torch.randn((3, tokens, 8, 128), generator=g, device="cuda").bfloat16()
+        n = torch.tensor([2800 - 700 * i, 100, 1500], device="cuda")
+        sets.append((q, k, v, n, torch.zeros((3, 4, 3000), device="cuda")))
+    want = []
+    for q, k, v, n, w in sets:
+        want.append(w.clone())
+        for _ in range(20):
+            ops.decoder_attention_weights(q, k, v, n, want[-1])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(20):
+        for s, (q, k, v, n, w) in zip(streams, sets):
+            with torch.cuda.stream(s):
+                ops.decoder_attention_weights(q, k, v, n, w)
+    torch.cuda.synchronize()
+    for (_, _, _, _, w), same in zip(sets, want):
+        assert w.any() and torch.equal(w, same)
+
+
+@pytest.mark.parametrize("kind", ["smooth", "ties", "special"])
+@pytest.mark.parametrize("layout,dtype", [("dense", torch.float32), ("packed", torch.float32), ("layer", torch.bfloat16),
+                                          ("shifted", torch.float32)])
+def test_cache_evict_of_more_rows_than_shared_memory_holds(ops, layout, dtype, kind):
+    """Keys of more than 49152 rows are made again in each pass; equal weights, zeros of both signs, infinities and NaN."""
+    g = torch.Generator(device="cuda").manual_seed(23)
+    batch, h, d, capacity, lengths, keep, recent, sinks, out = 2, 2, 16, 50003, [50003, 49151], 20000, 50, 4, 20007
+    k, v = caches(g, batch, capacity, h, d, layout, dtype)
+    w = torch.rand((batch, h, capacity), generator=g, device="cuda") ** 8
+    if kind == "ties":
+        w = (w * 6).round()
+    elif kind == "special":
+        some = torch.randint(0, 8, w.shape, generator=g, device="cuda")
+        for i, x in enumerate([0.0, -0.0, math.inf, -math.inf, math.nan, -1.0]):
+            w[some == i] = x
+    k2, v2, w2, left, index = ops.cache_evict(k, v, w, torch.tensor(lengths).cuda(), keep, recent, sinks, out)
+    assert left.tolist() == [keep, keep]
+    for b in range(batch):
+        for head in range(h):
+            rows = torch.tensor(kept_rows(w[b, head].tolist(), lengths[b], keep, recent, sinks), dtype=torch.int64).cuda()
+            assert torch.equal(index[b, head], rows)
+            assert torch.equal(k2[b, :keep, head], k[b, rows, head]) and torch.equal(v2[b, :keep, head], v[b, rows, head])
+            assert torch.equal(w2[b, head, :keep].view(torch.int32), w[b, head, rows].view(torch.int32))
+    assert not k2[:, keep:].any() and not v2[:, keep:].any() and not w2[:, :, keep:].any()
