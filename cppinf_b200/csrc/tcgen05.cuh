@@ -291,7 +291,7 @@ __device__ __forceinline__ bool elect_one() {
     return picked != 0u;
 }
 
-// 2^x of the hardware, within 2 ulp.
+// 2^x of the hardware, within 2 ulp; results below 2^-126 become 0.
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -9,7 +9,9 @@
 //
 // tree_commit: cache row len + i takes row len + path[i]. A path ascends from path[i] >= i, so going through it in
 // order never overwrites a row that is still to be read; every 16-byte column of a head's rows is one thread's, which
-// loads eight rows before it stores them, and the columns of all sequences, heads and both caches run side by side.
+// loads eight rows before it stores them, and the columns of all sequences, heads and both caches run side by side. Bound
+// by the latency of a chain of loads: length and count, then a path's entries and their rows for each eight accepted
+// nodes (one sequence of two accepted nodes of 8 x 128: 1.8 us; 64 of about 17: 4.9 us).
 #include "common.cuh"
 #include "runtime.h"
 

@@ -581,7 +581,9 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     drafted node, whose keys and values are cache rows lengths[b] .. lengths[b] + T - 1 of [B, capacity, Hkv, D]; node t
     sees every committed row and the nodes j with mask[b, t, j] (bool [B, T, T], or [T, T] for one tree shape), as far
     as nodes[b] (int64 [B]) reaches. Returns the bf16 context [B, T, Hq, D], zeros where a node is padding or sees
-    nothing. `error` (int32 [1]) is set when a wait of the kernel ran out of its poll limit."""
+    nothing. Caches whose rows of D are dense and start at multiples of 16 bytes are read in place; others, and queries that
+    are not dense, are copied whole in each call. `error` (int32 [1]) is set to 1 when a wait of the kernel ran out of its
+    poll limit: the context is then to be thrown away. Without it such a wait goes unreported."""
     op = "tree_attention"
     shape = q.shape
     square = (shape[1], shape[1]) if len(shape) == 4 else None
@@ -660,8 +662,8 @@ def decoder_attention_weights(q: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     """Causal attention of new tokens over a batch of caches (cppinf_decoder_attention_weights): query t of
     q [B, T, Hq, D] sees rows 0 .. lengths[b] + t of caches [B, capacity, Hkv, D]. Adds to weights (f32
     [B, Hkv, capacity], in place) each row's probabilities, summed over the queries and the query heads of its
-    key-value head, and returns the bf16 context [B, T, Hq, D]. Queries from counts[b] (int64 [B]) on are padding.
-    `error` as in tree_attention."""
+    key-value head, and returns the bf16 context [B, T, Hq, D]. Queries from counts[b] (int64 [B]) on are padding. Copies
+    and `error` as in tree_attention; where it is set, weights are to be thrown away too."""
     op = "decoder_attention_weights"
     device, lengths, counts = _cache_attention(op, q, k_cache, v_cache, lengths, counts, weights, error)
     batch, tokens, q_heads, d = q.shape
@@ -687,7 +689,8 @@ def cache_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, weights: torch.Ten
     """Cuts each sequence of a cache to `keep` rows, per key-value head (cppinf_cache_evict): the first `sinks`, the
     last `recent` and the rows of the highest weight (f32 [B, Hkv, capacity]) between them stay, in their order.
     Returns a new cache of `capacity` (default: keep) rows: (K [B, capacity, Hkv, D], V, weights [B, Hkv, capacity],
-    lengths [B], index [B, Hkv, keep] of the kept rows, -1 behind a shorter sequence's); unused rows are zeros."""
+    lengths [B], index [B, Hkv, keep] of the kept rows, -1 behind a shorter sequence's); unused rows are zeros. Caches
+    that tree_attention would copy are copied here too."""
     op = "cache_evict"
     _validate_caches(k_cache, v_cache, op)
     code = _dtype_code(k_cache, op)

@@ -297,9 +297,10 @@ CPPINF_API int64_t cppinf_cache_attention_scratch_bytes(int64_t batch, int64_t t
  * drafted node j where mask[b * mask_batch_stride + t * tokens + j] is not 0 (DEVICE bytes; stride 0 shares one mask;
  * a tree's mask has each node's ancestors and the node itself). `nodes` (DEVICE int64, may be NULL: all) counts each
  * sequence's nodes; later ones are padding, seen by none, and their rows of ctx are zeros, as is the row of a node that
- * sees nothing. ctx [batch, tokens, q_heads, head_dim] bf16 = softmax(q k^T / sqrt(head_dim)) v. tokens <= 256,
- * head_dim 64, 128 or 256. `error` (DEVICE, may be NULL) is set to 1 when a wait of the kernel ran out of its poll
- * limit (cppinf_set_wait_poll_limit). */
+ * sees nothing. ctx [batch, tokens, q_heads, head_dim] bf16 = softmax(q k^T / sqrt(head_dim)) v: scores, maxima and sums
+ * in f32, probabilities rounded to bf16 for their product with v, context rounded once. tokens <= 256, head_dim 64, 128
+ * or 256. `error` (DEVICE, may be NULL) is set to 1 when a wait of the kernel ran out of its poll limit
+ * (cppinf_set_wait_poll_limit); ctx is then to be thrown away. NULL leaves such a wait unreported. */
 CPPINF_API int cppinf_tree_attention(const void* q, const void* k_cache, const int64_t* k_strides,
                                      const void* v_cache, const int64_t* v_strides, const int64_t* lengths,
                                      const uint8_t* mask, int64_t mask_batch_stride, const int64_t* nodes, void* ctx,
@@ -330,10 +331,10 @@ CPPINF_API int cppinf_tree_commit(cppinf_dtype dtype, void* k_cache, const int64
 /* Causal attention of new tokens over a batch of caches, with the weight that each cached row received: query t of
  * sequence b (q [batch, tokens, q_heads, head_dim] bf16) sees rows 0 .. lengths[b] + t, ctx as in
  * cppinf_tree_attention, and weights[b, h, j] (f32 dense [batch, kv_heads, capacity]) grows by the sum, over the
- * sequence's queries and the query heads of key-value head h, of row j's probability (f32, in an order that does not
- * change from call to call). Rows past the new tokens keep their weight. `counts` (DEVICE int64, may be NULL: all)
- * are the valid queries of each sequence; later ones are padding: zero rows of ctx, no weight. head_dim 64, 128 or
- * 256; any number of tokens. `error` as in cppinf_tree_attention. */
+ * sequence's queries and the query heads of key-value head h, of row j's probability (f32, not rounded to bf16, in an
+ * order that does not change from call to call). Rows past the new tokens keep their weight. `counts` (DEVICE int64, may
+ * be NULL: all) are the valid queries of each sequence; later ones are padding: zero rows of ctx, no weight. head_dim 64, 128 or
+ * 256; any number of tokens. `error` as in cppinf_tree_attention; where it is set, weights are to be thrown away too. */
 CPPINF_API int cppinf_decoder_attention_weights(const void* q, const void* k_cache, const int64_t* k_strides,
                                                 const void* v_cache, const int64_t* v_strides, const int64_t* lengths,
                                                 const int64_t* counts, void* ctx, float* weights, int64_t batch,
