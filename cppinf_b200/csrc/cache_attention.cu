@@ -439,7 +439,10 @@ __global__ void __launch_bounds__(Tiling<D, kPair>::kThreads, 1)
     if (warp == 2) {
         tmem_alloc(&s_tmem, kTmemAll);
     }
-    grid_dependency_begin();
+    grid_dependency_wait();
+    if (warp == 2) {  // after its allocation: the next grid could take tensor memory first, and waits for this one to end
+        grid_dependency_release();
+    }
     // The line's length, and where this CTA's part of it begins. Entries (sequence, row tile) go in groups of 32, a lane
     // each; all warps count the groups' tiles, the first finds its place among them (1024 sequences of up to 300 rows:
     // 425 us against 436 us with one warp). With one group the first warp does without the others.
@@ -1289,7 +1292,10 @@ __global__ void __launch_bounds__(WeightTiling<D>::kThreads, 1)
         *reinterpret_cast<uint4*>(sm + L::kRing + atom * L::kAtom + row * 128 + chunk * 16) = make_uint4(0u, 0u, 0u, 0u);
     }
     fence_proxy_async_smem();
-    grid_dependency_begin();
+    grid_dependency_wait();
+    if (warp == 2) {  // after its allocation, as in cache_attention_kernel
+        grid_dependency_release();
+    }
     if (warp == 0) {
         // Sequences in groups of 32, a lane each; each one's products are then counted by the whole warp.
         const int heads = static_cast<int>(p.kv_heads);

@@ -19,12 +19,20 @@ using bf16 = __nv_bfloat16;
 
 // ---- programmatic dependent launch -------------------------------------------------------------------------------
 
-// First statement of every kernel: waits until the previous grid in the stream has completed and its memory writes
+// First statement of every kernel, in one or in two steps: waits until the previous grid in the stream has completed and its memory writes
 // are visible (a no-op when the launch did not allow programmatic overlap), then lets the next grid be scheduled
 // as soon as all CTAs of this one have started.
-__device__ __forceinline__ void grid_dependency_begin() {
+__device__ __forceinline__ void grid_dependency_wait() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+__device__ __forceinline__ void grid_dependency_release() {  // one thread of each CTA is enough
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+__device__ __forceinline__ void grid_dependency_begin() {
+    grid_dependency_wait();
+    grid_dependency_release();
 }
 
 // ---- 128-bit memory access -------------------------------------------------------------------------------------
