@@ -582,7 +582,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     sees every committed row and the nodes j with mask[b, t, j] (bool [B, T, T], or [T, T] for one tree shape), as far
     as nodes[b] (int64 [B]) reaches. Returns the bf16 context [B, T, Hq, D], zeros where a node is padding or sees
     nothing. Caches whose rows of D are dense and start at multiples of 16 bytes are read in place; others, and queries that
-    are not dense, are copied whole in each call. `error` (int32 [1]) is set to 1 when a wait of the kernel ran out of its
+    are not dense on that grid, are copied whole in each call. `error` (int32 [1]) is set to 1 when a wait of the kernel ran out of its
     poll limit: the context is then to be thrown away. Without it such a wait goes unreported."""
     op = "tree_attention"
     shape = q.shape
